@@ -44,7 +44,7 @@ typedef enum {
   NL_ERR_TOO_LARGE = -7  /* problem exceeds a fixed built-in scratch limit   */
 } nl_status;
 
-typedef enum { NL_F32 = 0, NL_BF16 = 1 } nl_dtype;
+typedef enum { NL_F32 = 0, NL_BF16 = 1, NL_E4M3 = 2 /* paged key-value caches only */ } nl_dtype;
 
 /* GEMM epilogue selector for nl_gemm_ex. */
 typedef enum {
@@ -62,7 +62,7 @@ typedef enum {
 NL_API const char* nl_version(void);
 /* Reads and clears the device-side error word (1 = a bounded wait timed out,
  * 2 = misaligned shared memory, 3 = a decode position outside the KV cache or
- * the output row).  Synchronises `stream`. */
+ * the output row, 4 = a page or slot outside a paged cache).  Synchronises `stream`. */
 NL_API int nl_get_device_error(cudaStream_t stream);
 /* Kernels launched by this library so far in this process (host-side count). */
 NL_API long long nl_launch_count(void);
@@ -313,6 +313,89 @@ NL_API int nl_decode_advance(int* pos, cudaStream_t stream);
 NL_API int nl_linear_ln_small(const void* x, long long ldx, const float* gamma, const float* beta, float eps,
                               const void* W, long long ldw, void* C, long long ldc, int c_dtype, int M, int N, int K,
                               int epilogue, const float* bias, void* aux, const void* resid, cudaStream_t stream);
+
+/* ---------------------------------------------------------------- paged key-value cache
+ * Serving of ragged batches (no reference counterpart: nlearn/model.py:417-465
+ * recomputes the whole buffer of one sequence length per token).  A layer's
+ * keys and its values are two arrays of n_pages pages of page_size tokens, each
+ * addressed by a page, a kv-head and a token stride (in elements, the same for
+ * both arrays; elements of a row are contiguous): [page][head][token][d] and
+ * [page][token][head][d] are both strides.  Rows and strides lie on 16-byte
+ * boundaries.  cache_dtype is NL_BF16, or NL_E4M3 with an optional f32 scale
+ * per kv head (value = e4m3 * scale).  Row b of `block_table` (int32, pitch
+ * table_ld) lists the pages of sequence b in order; slot = page * page_size +
+ * row inside the page.  Any page_size >= 1.
+ *
+ * Attention of ONE new token per sequence: for query head h of Hq (kv head
+ * h / (Hq / Hk)), o[b, h] = softmax(scale q[b, h] . k_j) v_j over j < lens[b].
+ *   q, o     bf16 [B, Hq, d], strides q_b, q_h / o_b, o_h; d is 64 or 128
+ *   lens     int32 [B], the new token included; 0: o = 0, lse = -inf
+ *   k_new, v_new  (both or neither NULL) bf16 [B, Hk, d], strides n_b, n_h: key
+ *            lens[b] - 1 is taken from here and written into its slot, rounded
+ *            to e4m3 first where the cache is.  The page that takes it is in no
+ *            other place of the tables.
+ *   lse      f32 [B, Hq], pitch lse_b (may be NULL): natural log of the sum of
+ *            exp(scaled scores)
+ * lens above max_blocks * page_size or below 0 set device error 3 (the length is
+ * clamped and nothing is appended); a page outside [0, n_pages) sets 4 and its
+ * keys take no part.  Workspace: nl_paged_attention_workspace_bytes (0 for a
+ * shape that is refused), 256-byte aligned, any contents; calls that may
+ * overlap on the GPU need one each. */
+NL_API size_t nl_paged_attention_workspace_bytes(int B, int Hq, int Hk, int d, int page_size, int max_blocks,
+                                                 int cache_dtype);
+NL_API int nl_paged_attention(const void* q, long long q_b, long long q_h, void* k_cache, void* v_cache,
+                              int cache_dtype, long long page_stride, long long head_stride, long long tok_stride,
+                              const int* block_table, long long table_ld, const int* lens, const void* k_new,
+                              const void* v_new, long long n_b, long long n_h, const float* k_scale,
+                              const float* v_scale, float scale, void* o, long long o_b, long long o_h, float* lse,
+                              long long lse_b, void* workspace, size_t ws_bytes, int B, int Hq, int Hk, int d,
+                              int page_size, int max_blocks, int n_pages, cudaStream_t stream);
+/* Keys and values of T tokens (bf16 [T, Hk, d], strides n_t, n_h; d a multiple
+ * of 8, of 16 for e4m3) into slots[t].  A negative slot is padding and skipped;
+ * one past the cache sets device error 4 and is skipped.  No slot occurs twice. */
+NL_API int nl_paged_kv_write(const void* k, const void* v, long long n_t, long long n_h, void* k_cache, void* v_cache,
+                             int cache_dtype, long long page_stride, long long head_stride, long long tok_stride,
+                             const int* slots, const float* k_scale, const float* v_scale, int T, int Hk, int d,
+                             int page_size, int n_pages, cudaStream_t stream);
+/* One serving step of the block tables, all int32 in device memory.  With
+ * len0 = 0 for rows whose done[b] is not 0 (done may be NULL), lens[b] for others:
+ *   - the pages of the rows that are done go on top of the stack
+ *     free_pages[0 .. *n_free) (capacity n_pages), row after row;
+ *   - row b grows by new_lens[b] tokens: its table row gets the pages that
+ *     takes, from the top of the stack, lower rows first; lens_out[b] = len0 + new;
+ *   - token i of row b is token cu[b] + i of the flat list (cu [B + 1]: prefix
+ *     sums of new_lens, saturating), and slots / positions [n_tokens] get its slot and its
+ *     position; -1 past the last token and for rows that were refused.
+ * status[b]: 0; or the row was refused and only its done took effect: 1 not
+ * enough free pages, 2 longer than its table row, 3 tokens past n_tokens, 4 a
+ * negative count or a length that is negative or past the table.
+ * Every row of the table past a sequence's last page keeps what it held.
+ * lens_out and n_free_out may be lens and n_free.  B <= 8192. */
+NL_API int nl_update_block_tables(int* block_table, long long table_ld, const int* lens, const int* new_lens,
+                                  const int* done, int* free_pages, const int* n_free, int* lens_out,
+                                  int* n_free_out, int* slots, int* positions, int* cu, int* status, int B,
+                                  int max_blocks, int page_size, int n_pages, int n_tokens, cudaStream_t stream);
+
+/* ---------------------------------------------------------------- logits processing
+ * Penalties, biases and masks before sampling (nlearn/model.py:440-444 samples
+ * the raw logits).  logits, out: [B, V] of dtype NL_F32 or NL_BF16, pitches ldx
+ * and ldy; out may be logits.  In this order, each part optional (NULL):
+ *   tokens [B, L] int32 (pitch ldt), of which row b has lens[b], the first
+ *   prompt_lens[b] of them its prompt (NULL: none): a column that occurs is
+ *   divided (x > 0) or multiplied by repetition[b]; one generated c times after the
+ *   prompt loses frequency[b] * c + presence[b];
+ *   bias_ids, bias [B, n_bias] (pitch ldb): bias added to column bias_ids, in
+ *   list order where an id is listed again;
+ *   mask [n_masks, (V + 31) / 32] 32-bit words (pitch ldm): a column whose bit
+ *   (bit v % 32 of word v / 32) is 0 becomes -inf; row b uses mask row
+ *   mask_rows[b] (below 0 or past n_masks: none), or b where mask_rows is NULL.
+ * Tokens and bias ids outside [0, V) are ignored.  Arithmetic is f32, rounded
+ * once.  B <= 65535. */
+NL_API int nl_process_logits(const void* logits, long long ldx, int dtype, void* out, long long ldy,
+                             const int* tokens, long long ldt, const int* lens, const int* prompt_lens, int L,
+                             const float* repetition, const float* frequency, const float* presence,
+                             const int* bias_ids, const float* bias, long long ldb, int n_bias, const void* mask,
+                             long long ldm, int n_masks, const int* mask_rows, int B, int V, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

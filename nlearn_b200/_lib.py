@@ -19,7 +19,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libnl_ops.so")
 
 STATUS = {0: "NL_OK", -1: "NL_ERR_SHAPE", -2: "NL_ERR_ALIGN", -3: "NL_ERR_LAUNCH", -4: "NL_ERR_CUDA",
           -5: "NL_ERR_DTYPE", -6: "NL_ERR_WORKSPACE", -7: "NL_ERR_TOO_LARGE"}
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
 EPI_STORE, EPI_ACCUM, EPI_BIAS, EPI_BIAS_GELU, EPI_RESID, EPI_DGELU = 0, 1, 2, 3, 4, 5
 
 # name -> argtypes (restype is int unless listed in _RESTYPE)
@@ -66,6 +66,17 @@ SIGNATURES: dict[str, list] = {
     "nl_decode_advance": [c_void_p, c_void_p],
     "nl_linear_ln_small": [c_void_p, c_longlong, c_void_p, c_void_p, c_float, c_void_p, c_longlong, c_void_p,
                            c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    "nl_paged_attention_workspace_bytes": [c_int] * 7,
+    "nl_paged_attention": [c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_int] + [c_longlong] * 3 +
+                          [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p,
+                           c_void_p, c_float, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_void_p,
+                           c_size_t] + [c_int] * 7 + [c_void_p],
+    "nl_paged_kv_write": [c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_int] + [c_longlong] * 3 +
+                         [c_void_p] * 3 + [c_int] * 5 + [c_void_p],
+    "nl_update_block_tables": [c_void_p, c_longlong] + [c_void_p] * 11 + [c_int] * 5 + [c_void_p],
+    "nl_process_logits": [c_void_p, c_longlong, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p,
+                          c_void_p, c_int] + [c_void_p] * 5 + [c_longlong, c_int, c_void_p, c_longlong, c_int,
+                                                               c_void_p, c_int, c_int, c_void_p],
     "nl_cast_bf16": [c_void_p, c_void_p, c_longlong, c_void_p],
     "nl_rows_mark": [c_void_p, c_longlong, c_void_p, c_int, c_void_p],
     "nl_rows_compact": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
@@ -83,7 +94,7 @@ SIGNATURES: dict[str, list] = {
 }
 _RESTYPE = {"nl_version": ctypes.c_char_p, "nl_launch_count": c_longlong,
             "nl_flash_attention_bwd_noalloc_max_rows": c_longlong, "nl_flash_attention_workspace_bytes": c_size_t, "nl_lce_workspace_bytes": ctypes.c_size_t,
-            "nl_decode_workspace_bytes": ctypes.c_size_t}
+            "nl_decode_workspace_bytes": ctypes.c_size_t, "nl_paged_attention_workspace_bytes": ctypes.c_size_t}
 
 
 class NlError(RuntimeError):
@@ -135,10 +146,11 @@ def device_error() -> int:
     up, 2 = misaligned shared memory, 3 = a decode position outside the cache
     or the output row (the cache and the output row are not written; the
     attention output keeps its previous contents, the sampled token is still
-    written)."""
+    written), 4 = a page or slot outside a paged cache (its keys take no part,
+    nothing is written to it)."""
     return lib.nl_get_device_error(stream_handle())
 
 
 __all__ = ["lib", "check", "ptr", "stream_handle", "device_error", "NlError", "LIB_PATH", "SIGNATURES",
-           "F32", "BF16", "EPI_STORE", "EPI_ACCUM", "EPI_BIAS", "EPI_BIAS_GELU", "EPI_RESID", "EPI_DGELU",
+           "F32", "BF16", "E4M3", "EPI_STORE", "EPI_ACCUM", "EPI_BIAS", "EPI_BIAS_GELU", "EPI_RESID", "EPI_DGELU",
            "c_longlong"]

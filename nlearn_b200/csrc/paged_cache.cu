@@ -1,0 +1,317 @@
+// paged_cache.cu — the bookkeeping of a paged key-value cache: block tables and
+// slot maps built from request lengths, and the write of keys and values into
+// their slots.  No reference counterpart (nlearn keeps no cache).
+//
+// update_tables_kernel: one serving step.  With len0 = 0 for rows that ended and
+// up(x) = ceil(x / P):
+//   freed pages  the up(len) pages of each row that ended go on top of the
+//                stack of free pages, row after row;
+//   taken pages  row b takes up(len0 + new) - up(len0) pages from the top, at
+//                the prefix sum of the rows before it; a row whose pages do not
+//                all fit is refused and takes none, and so is every later row
+//                that needs pages (the prefix sums only grow);
+//   slots        token i of the flat list (rows back to back, by the prefix sum
+//                of new) has slot page * P + pos % P.
+// All of it is prefix sums over the rows, which every CTA of the one cluster
+// makes for itself, so the CTAs share no state but the two sides of the
+// cluster barrier: lengths, stack and tables are read before it and rewritten
+// after it (the outputs may then be the inputs).  Latency-bound: one launch.
+//
+// kv_write_kernel: a thread per 16 bytes of a key row and of its value row.
+// Bound by HBM: each element is read and written once.
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "host_common.h"
+#include "sm100.cuh"
+
+namespace nl {
+namespace pc {
+
+constexpr int kThreads = 1024;
+constexpr int kMaxRows = 8192;  // rows of a block table: 16 bytes of shared memory each
+
+enum : int { kOk = 0, kNoPages = 1, kTooLong = 2, kNoSlots = 3, kInvalid = 4 };  // status of a row
+enum : int { kErrPage = 4 };                                                      // device error word
+
+struct TableParams {
+  int* table;
+  long long ld;
+  const int* lens;
+  const int* new_lens;
+  const int* done;  // may be null: no row ended
+  int* free_pages;
+  const int* n_free;
+  int* lens_out;
+  int* n_free_out;
+  int* slots;
+  int* positions;
+  int* cu;
+  int* status;
+  int B, max_blocks, page, n_pages, tokens;
+};
+
+// Exclusive prefix sums of one value per thread over the block; total of all.
+__device__ __forceinline__ long long block_scan(long long v, long long* warp_sum, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) warp_sum[warp] = inc;
+  __syncthreads();
+  long long s = warp_sum[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += y;
+  }
+  total = __shfl_sync(0xffffffffu, s, 31);
+  const long long before = warp == 0 ? 0 : __shfl_sync(0xffffffffu, s, warp == 0 ? 0 : warp - 1);
+  __syncthreads();
+  return before + inc - v;
+}
+
+__device__ __forceinline__ int sat(long long x) { return x > INT32_MAX ? INT32_MAX : static_cast<int>(x); }
+
+template <bool CLUSTER>
+__global__ void __launch_bounds__(kThreads) update_tables_kernel(const TableParams p) {
+  extern __shared__ int4 s_row[];  // {first token, len0 or -1 if refused, first page from the top, pages held}
+  __shared__ long long s_sum[32];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int rank = blockIdx.x, nctas = gridDim.x;
+  griddep_sync();
+
+  const int P = p.page;
+  const long long cap = static_cast<long long>(p.max_blocks) * P;
+  auto up = [P](int x) { return static_cast<int>((static_cast<long long>(x) + P - 1) / P); };
+  const int stack0 = max(0, min(*p.n_free, p.n_pages));
+  const int warps = nctas * (kThreads / 32), gw = rank * (kThreads / 32) + (tid >> 5);
+
+  // ---- first tokens, and the pages of rows that ended
+  long long tok = 0, freed = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    const int b = b0 + tid;
+    int n = 0, back = 0, len = 0;
+    if (b < p.B) {
+      len = p.lens[b];
+      n = max(0, p.new_lens[b]);
+      if (p.done && p.done[b] && len > 0 && len <= cap) back = up(len);
+    }
+    long long t, f;
+    const long long at = tok + block_scan(n, s_sum, t);
+    const long long top = freed + block_scan(back, s_sum, f);
+    if (b < p.B) {
+      s_row[b] = make_int4(sat(at), len, sat(top), back);
+      if (rank == 0) p.cu[b] = sat(at);
+    }
+    tok += t;
+    freed += f;
+  }
+  if (rank == 0 && tid == 0) p.cu[p.B] = sat(tok);
+  __syncthreads();
+  if (freed > 0)
+    for (int b = gw; b < p.B; b += warps) {
+      const int4 r = s_row[b];
+      for (int i = lane; i < r.w; i += 32) {
+        const long long at = static_cast<long long>(stack0) + r.z + i;
+        if (at < p.n_pages) p.free_pages[at] = p.table[b * p.ld + i];
+      }
+    }
+  __syncthreads();
+  const int avail = static_cast<int>(min(static_cast<long long>(p.n_pages), stack0 + freed));
+
+  // ---- refusals and the pages each row takes (from the top of the stack)
+  long long taken = 0;
+  int used = 0;  // pages taken by rows that were not refused: this thread's rows
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    const int b = b0 + tid;
+    int st = kOk, len0 = 0, n = 0, take = 0, first = 0, len = 0;
+    if (b < p.B) {
+      len = s_row[b].y;
+      first = s_row[b].x;
+      n = p.new_lens[b];
+      const bool ended = p.done && p.done[b];
+      const bool bad = len < 0 || len > cap;
+      len0 = ended && !bad ? 0 : len;
+      if (bad || n < 0) st = kInvalid;
+      else if (static_cast<long long>(len0) + n > cap) st = kTooLong;
+      else if (n > 0 && static_cast<long long>(first) + n > p.tokens) st = kNoSlots;
+      if (st == kOk) take = up(len0 + n) - up(len0);
+    }
+    long long t;
+    const long long off = taken + block_scan(take, s_sum, t);
+    taken += t;
+    if (b < p.B) {
+      if (take > 0 && off + take > avail) st = kNoPages;
+      if (st != kOk) take = 0;
+      used += take;
+      s_row[b] = make_int4(first, st == kOk ? len0 : -1, sat(off), st == kOk ? up(len0) : 0);
+      if (rank == 0) p.status[b] = st;
+    }
+  }
+  long long total_used;
+  block_scan(used, s_sum, total_used);
+  if constexpr (CLUSTER) cluster_sync();  // stack written, lengths and stack size read by every CTA
+  else __syncthreads();
+
+  // ---- the taken pages into the tables, new lengths
+  for (int b = gw; b < p.B; b += warps) {
+    const int4 r = s_row[b];
+    if (r.y < 0) continue;
+    const int n = p.new_lens[b];
+    const int take = up(r.y + n) - r.w;
+    for (int i = lane; i < take; i += 32) p.table[b * p.ld + r.w + i] = __ldcg(p.free_pages + avail - 1 - r.z - i);
+  }
+  if (rank == 0) {
+    for (int b = tid; b < p.B; b += kThreads) {
+      const int4 r = s_row[b];
+      const int len = r.y >= 0 ? r.y + p.new_lens[b] : 0;
+      if (r.y >= 0) p.lens_out[b] = len;
+      else {  // refused: a row that ended still gave its pages back
+        const int old = p.lens[b];
+        p.lens_out[b] = (p.done && p.done[b] && old >= 0 && old <= cap) ? 0 : old;
+      }
+    }
+    if (tid == 0) *p.n_free_out = avail - static_cast<int>(total_used);
+  }
+
+  // ---- slots
+  for (int t = rank * kThreads + tid; t < p.tokens; t += nctas * kThreads) {
+    int slot = -1, pos = -1;
+    if (t < tok) {
+      int lo = 0, hi = p.B - 1;  // last row whose first token is not after t
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_row[mid].x <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int4 r = s_row[lo];
+      if (r.y >= 0) {
+        pos = r.y + t - r.x;
+        const int blk = pos / P;
+        // (pages already held are not rewritten by this call; the others come off the stack)
+        const int page = blk < r.w ? __ldcg(p.table + lo * p.ld + blk)
+                                   : __ldcg(p.free_pages + avail - 1 - r.z - (blk - r.w));
+        slot = (page >= 0 && page < p.n_pages) ? page * P + (pos - blk * P) : -1;
+      }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+  }
+}
+
+struct WriteParams {
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  long long n_t, n_h;  // token and head strides (elements)
+  uint8_t* kc;
+  uint8_t* vc;
+  long long page_bytes, head_bytes, tok_bytes;
+  const int* slots;
+  const float* k_scale;  // [Hk], e4m3 only
+  const float* v_scale;
+  int T, Hk, cpr, page;
+  long long n_slots;
+  int* err;
+};
+
+template <bool FP8>
+__device__ __forceinline__ uint4 convert(const __nv_bfloat16* x, float scale) {
+  if constexpr (!FP8) {
+    return *reinterpret_cast<const uint4*>(x);
+  } else {
+    uint4 in[2] = {reinterpret_cast<const uint4*>(x)[0], reinterpret_cast<const uint4*>(x)[1]};
+    const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(in);
+    uint4 out;
+    uint8_t* o = reinterpret_cast<uint8_t*>(&out);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = __nv_cvt_float_to_fp8(__bfloat162float(e[i]) / scale, __NV_SATFINITE, __NV_E4M3);
+    return out;
+  }
+}
+
+template <bool FP8>
+__global__ void __launch_bounds__(256) kv_write_kernel(const WriteParams p) {
+  griddep_sync();
+  const int per_tok = p.Hk * p.cpr;
+  const long long n = static_cast<long long>(p.T) * per_tok;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const int t = static_cast<int>(i / per_tok), r = static_cast<int>(i - static_cast<long long>(t) * per_tok);
+    const int h = r / p.cpr, c = r - h * p.cpr;
+    const int slot = p.slots[t];
+    if (slot < 0) continue;  // padding
+    if (slot >= p.n_slots) {
+      if (p.err) atomicExch(p.err, kErrPage);
+      continue;
+    }
+    const int page = slot / p.page, off = slot - page * p.page;
+    const long long src = t * p.n_t + h * p.n_h + c * (FP8 ? 16 : 8);
+    const long long dst = page * p.page_bytes + h * p.head_bytes + off * p.tok_bytes + c * 16;
+    const uint4 kx = convert<FP8>(p.k + src, FP8 && p.k_scale ? p.k_scale[h] : 1.f);
+    const uint4 vx = convert<FP8>(p.v + src, FP8 && p.v_scale ? p.v_scale[h] : 1.f);
+    *reinterpret_cast<uint4*>(p.kc + dst) = kx;
+    *reinterpret_cast<uint4*>(p.vc + dst) = vx;
+  }
+}
+
+}  // namespace pc
+}  // namespace nl
+
+using namespace nl;
+
+extern "C" int nl_update_block_tables(int* block_table, long long table_ld, const int* lens, const int* new_lens,
+                                      const int* done, int* free_pages, const int* n_free, int* lens_out,
+                                      int* n_free_out, int* slots, int* positions, int* cu, int* status, int B,
+                                      int max_blocks, int page_size, int n_pages, int n_tokens, cudaStream_t stream) {
+  if (B <= 0 || B > pc::kMaxRows || max_blocks <= 0 || page_size <= 0 || n_pages <= 0 || n_tokens < 0 ||
+      table_ld < max_blocks || static_cast<long long>(max_blocks) * page_size > INT32_MAX ||
+      static_cast<long long>(n_pages) * page_size > INT32_MAX)
+    return NL_ERR_SHAPE;
+  if (!block_table || !lens || !new_lens || !free_pages || !n_free || !lens_out || !n_free_out || !cu || !status ||
+      (n_tokens > 0 && (!slots || !positions)))
+    return NL_ERR_SHAPE;
+  pc::TableParams p{block_table, table_ld, lens, new_lens, done, free_pages, n_free, lens_out, n_free_out, slots,
+                    positions,   cu,       status, B,      max_blocks, page_size, n_pages, n_tokens};
+  const size_t smem = static_cast<size_t>(B) * sizeof(int4);
+  const bool wide = n_tokens > 4 * pc::kThreads;
+  auto kern = wide ? pc::update_tables_kernel<true> : pc::update_tables_kernel<false>;
+  if (smem > 40 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
+    return NL_ERR_LAUNCH;
+  const int ctas = wide ? 8 : 1;
+  launch_kernel(kern, dim3(ctas), dim3(pc::kThreads), smem, stream, ctas, p);
+  return launch_status();
+}
+
+extern "C" int nl_paged_kv_write(const void* k, const void* v, long long n_t, long long n_h, void* k_cache,
+                                 void* v_cache, int cache_dtype, long long page_stride, long long head_stride,
+                                 long long tok_stride, const int* slots, const float* k_scale, const float* v_scale,
+                                 int T, int Hk, int d, int page_size, int n_pages, cudaStream_t stream) {
+  if (T <= 0 || Hk <= 0 || d <= 0 || page_size <= 0 || n_pages <= 0 || !k || !v || !k_cache || !v_cache || !slots ||
+      n_t < 0 || n_h < 0 || page_stride <= 0 || head_stride < 0 || tok_stride <= 0)
+    return NL_ERR_SHAPE;
+  if (cache_dtype != NL_BF16 && cache_dtype != NL_E4M3) return NL_ERR_DTYPE;
+  const bool fp8 = cache_dtype == NL_E4M3;
+  const int el = fp8 ? 1 : 2, per = fp8 ? 16 : 8;  // elements of a 16-byte store
+  if (d % per || static_cast<long long>(Hk) * (d / per) > INT32_MAX) return NL_ERR_SHAPE;
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                         reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache);
+  if ((ptrs & 15) || ((n_t | n_h) & 7) || ((page_stride | head_stride | tok_stride) * el & 15)) return NL_ERR_ALIGN;
+  pc::WriteParams p{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), n_t, n_h,
+                    static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), page_stride * el,
+                    head_stride * el, tok_stride * el, slots, k_scale, v_scale, T, Hk, d / per, page_size,
+                    static_cast<long long>(n_pages) * page_size, device_error_word()};
+  const long long n = static_cast<long long>(T) * Hk * (d / per);
+  long long blocks = (n + 255) / 256;
+  const long long most = static_cast<long long>(sm_count()) * 32;
+  if (blocks > most) blocks = most;
+  launch_kernel(fp8 ? pc::kv_write_kernel<true> : pc::kv_write_kernel<false>, dim3(static_cast<int>(blocks)),
+                dim3(256), 0, stream, 1, p);
+  return launch_status();
+}
