@@ -10,24 +10,35 @@
 // nlearn recomputes the whole sequence for every token (nlearn/model.py:417-447).
 //
 // Bound: HBM.  Every cached element is used once per query head of its group,
-// 2 FLOP per element and head, so the kernel is built to keep loads in flight:
+// 2 FLOP per element and head, so the kernel is built to keep loads in flight
+// and to spend few instructions on a byte:
 //   * a warp works on tiles of 16 keys, gathered row by row with 16-byte
-//     cp.async (any page size, any strides) into a ring of tiles of its own:
-//     no block barrier between tiles, only the warp's own wait;
-//   * the group's query heads are the 16 rows of m16n8k16 products (q k^T, then
-//     p v with the running maximum and sum in registers): with at most 16 rows
-//     a 128-row tcgen05 tile would be mostly padding, and the keys would have
-//     to be transposed through TMEM; mma.sync takes them straight from the tile;
-//   * the work of all sequences and heads is one flat list of units of 64 keys
-//     (four warps, one tile each), cut into equal ranges, one per CTA: lengths
-//     are read on the device, so ragged batches balance without the host.  A
-//     range's cut ends leave partials (max, sum, o) that join_kernel merges in
-//     the order of the cache, so results do not depend on timing.
-// p is split into two bf16 terms (p = hi + lo, error 2^-17) for the second
-// product: the tensor pipe is idle anyway and the output then keeps the accuracy of
+//     cp.async (any page size, any strides) into a ring of tiles of its own: no
+//     block barrier between tiles, and the ring is filled across the ends of
+//     sequences, so a new sequence finds its first tiles on the way;
+//   * both products are m16n8k16 with the group's heads as the 8 columns:
+//     s^T = k q^T takes the key tile as its 16 rows, o^T += v^T p^T the value
+//     tile.  A tcgen05 tile needs 64 or 128 rows of keys in one piece of shared
+//     memory and its result back from TMEM for the softmax, for 8 columns of
+//     work; mma.sync takes a warp's own tile, and the tensor pipe is idle most
+//     of the time either way;
+//   * the running maximum moves only when a score passes it by 2^8 (the sums
+//     hold that in f32), so the cross-lane maximum and the rescaling of o are
+//     rare.
+// p is split into two bf16 terms (p = hi + lo, error 2^-16) for the second
+// product: the tensor pipe has room and the output then keeps the accuracy of
 // f32 probabilities.  With an e4m3 cache both products run in f16: e4m3 values
-// are exact in f16, q is scaled by a power of two per row (exact), and p, kept
-// in [0, 2^15], is rounded to f16's 11 bits, a quarter of the bf16 output's step.
+// are exact in f16, q is scaled by a power of two per head (exact), and p, kept
+// below 2^15, is rounded to f16's 11 bits, an eighth of the bf16 output's step.
+//
+// Two ways of dividing the work, both with lengths read on the device only:
+//   * flat: the work of all sequences and heads is one list of units of 64 keys
+//     (four warps, one tile each), cut into equal ranges, one per CTA, so any mix of
+//     lengths balances.  The cut ends leave partials (max, sum, o) that
+//     join_kernel merges in the order of the cache;
+//   * clustered, for short caches: a cluster of up to 8 CTAs per (sequence,
+//     head) merges over distributed shared memory: one launch, no prefix sums.
+// Neither depends on the order in which CTAs finish.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -45,10 +56,12 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;                 // keys a warp takes at a time
 constexpr int kUnit = kTile * kWarps;     // keys of one unit of work
-constexpr int kStages = 3;                // tiles in a warp's ring
-constexpr int kRows = 16;                 // query heads of one product
+constexpr int kHeads = 8;                 // query heads of one product (its columns)
+constexpr int kMaxTiles = 2;              // products of 8 heads a CTA keeps: groups of up to 16 read the keys once
+constexpr int kMaxCluster = 8;
 constexpr int kJoinThreads = 256;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.f;             // log2 of how far p may grow before the maximum moves
 constexpr uint32_t kNoRow = 0xffffffffu;
 
 enum : int { kErrPos = 3, kErrPage = 4 };  // device error word
@@ -75,7 +88,7 @@ struct Params {
   float* part_o;                    // [2 * ctas][rows][HD]
   float2* part_ml;                  // [2 * ctas][rows]
   int4* desc;                       // [ctas]
-  int B, Hq, Hk, group, mtiles, rows;  // rows = min(group, 16): rows kept of a product
+  int B, Hq, Hk, group, mtiles, rows;  // rows: query heads of one CTA's product, at most 16
   int page, page_shift, max_blocks, n_pages;
   float scale_log2;
   int* err;
@@ -101,6 +114,12 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
+// 8x8 transpose of 16-bit elements across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
 template <bool F16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (F16)
@@ -118,8 +137,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 // two e4m3 values (low 16 bits of x) as f16x2; exact
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t x) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(x), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -127,95 +147,156 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 
+__device__ __forceinline__ int cap_of(const Params& p) { return p.max_blocks * p.page; }
 __device__ __forceinline__ int clamp_len(const Params& p, int b) {
-  const int cap = p.max_blocks * p.page;
-  const int n = p.lens[b];
+  const int n = p.lens[b], cap = cap_of(p);
   return n < 0 ? 0 : (n > cap ? cap : n);
 }
 __device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
 
-// Range of CTA i of n over U units: [i U / n, (i + 1) U / n).
-__device__ __forceinline__ long long cut(long long i, long long U, long long n) { return i * U / n; }
+// First unit of CTA i of n over U units.
+__device__ __forceinline__ int cut(int i, int U, int n) {
+  return static_cast<int>(static_cast<long long>(i) * U / n);
+}
 
-// State of one warp's pass over a run of units of one (sequence, kv head).
-template <int HD, bool FP8>
-struct Warp {
-  static constexpr int EL = FP8 ? 1 : 2;
-  static constexpr int RB = HD * EL;             // bytes of a key row
-  static constexpr int CPR = RB / 16;            // 16-byte chunks of a row
-  static constexpr int RPI = 32 / CPR;           // rows a warp's copy instruction covers
-  static constexpr int NI = kTile / RPI;         // copy instructions of a tile
-  static constexpr int TB = kTile * RB;          // bytes of a tile
-  static constexpr int SB = 2 * TB;              // K and V tiles of a stage
-  static constexpr int KS = HD / 16;             // k steps of q k^T
-  static constexpr int NT = HD / 8;              // n tiles of p v
-
-  // byte offset of 16-byte chunk c of row r: chunks are permuted inside groups
-  // of eight rows so that the eight rows of an ldmatrix hit different banks
-  __device__ static __forceinline__ uint32_t at(int r, int c) {
-    if constexpr (RB >= 128) return r * RB + ((c ^ (r & 7)) << 4);
-    // 64-byte rows: two rows share 128 bytes
-    return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ ((r >> 1) & 3)) << 4);
+// A run: consecutive units [c0, c1) of one (sequence, tile of query heads).
+struct Run {
+  int b, hm, len, nu, c0, c1;
+};
+// Walks a CTA's range of the flat list, run by run.
+struct Walk {
+  int u, u1;     // next unit, end of the range
+  int b, base;   // sequence of unit u (or an earlier one), units before it
+  __device__ __forceinline__ bool next(const Params& p, Run& r) {
+    if (u >= u1) return false;
+    const int heads = p.Hk * p.mtiles;
+    int len, nu;
+    for (;; ++b) {
+      len = clamp_len(p, b);
+      nu = units_of(len);
+      if (u - base < nu * heads) break;
+      base += nu * heads;
+    }
+    const int local = u - base;
+    r.b = b;
+    r.len = len;
+    r.nu = nu;
+    r.hm = local / nu;
+    r.c0 = local - r.hm * nu;
+    r.c1 = min(nu, r.c0 + (u1 - u));
+    u += r.c1 - r.c0;
+    return true;
   }
 };
 
 template <int HD, bool FP8>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
-  using W = Warp<HD, FP8>;
-  constexpr int OS = HD + 8;  // row pitch of the warps' o in shared memory (floats)
+struct Shape {
+  static constexpr int RB = HD * (FP8 ? 1 : 2);  // bytes of a key row
+  static constexpr int CPR = RB / 16;            // 16-byte chunks of a row
+  static constexpr int RPI = 32 / CPR;           // rows one copy instruction of a warp covers
+  static constexpr int NI = kTile / RPI;         // copy instructions of a tile
+  static constexpr int TB = kTile * RB;          // bytes of a tile
+  static constexpr int SB = 2 * TB;              // K and V tiles of a stage
+  static constexpr int KS = HD / 16;             // k steps of k q^T; row tiles of v^T p^T
+  static constexpr int STAGES = SB <= 2048 ? 4 : 3;
+  static constexpr int MT = SB > 4096 ? 4 : 2;   // row tiles joined at a time (shared memory)
+  static constexpr int RING = kWarps * STAGES * SB;
+  static constexpr int SMEM = RING + kWarps * MT * 4 * 32 * 4;
+  // Byte offset of chunk c of row r.  Chunks are permuted inside 128 bytes so
+  // that the eight rows of an ldmatrix hit different banks.
+  __device__ static __forceinline__ uint32_t at(int r, int c) {
+    if constexpr (RB >= 128) return r * RB + ((c ^ (r & 7)) << 4);
+    return (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ ((r >> 1) & 3)) << 4);  // two 64-byte rows a line
+  }
+};
+
+// Resident CTAs an SM is meant to hold (shared memory allows them; caps registers).
+template <int HD, bool FP8, int NH>
+constexpr int min_ctas() {
+  if (HD == 128) return FP8 ? (NH == 1 ? 4 : 3) : 2;
+  return FP8 ? (NH == 1 ? 5 : 4) : 4;
+}
+
+template <int HD, bool FP8, int NH, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kernel(const Params p) {
+  using S = Shape<HD, FP8>;
+  constexpr float kUp = FP8 ? 7.f : 0.f;  // p is kept as 2^(y - m + kUp): below 2^15 with the slack
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
-  __shared__ uint32_t s_valid[kWarps][kStages];
-  __shared__ int s_scan[kWarps + 1];
+  __shared__ float s_m[kWarps][kHeads * NH], s_l[kWarps][kHeads * NH];
+  __shared__ uint32_t s_valid[kWarps][S::STAGES];
+  __shared__ int s_scan[kWarps];
   __shared__ int s_start[2];
+  __shared__ float2 s_ml[kHeads * NH];  // clustered: this CTA's (max, sum)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   griddep_sync();
 
-  // ---- units of all sequences: where this CTA's range begins
-  const int per = (p.B + kThreads - 1) / kThreads;
-  const int sb0 = min(tid * per, p.B), sb1 = min(sb0 + per, p.B);
-  int mine = 0;
-  for (int b = sb0; b < sb1; ++b) {
-    const int n = p.lens[b];
-    if (blockIdx.x == 0 && (n < 0 || n > p.max_blocks * p.page) && p.err) atomicExch(p.err, kErrPos);
-    mine += units_of(clamp_len(p, b));
-  }
-  int inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += y;
-  }
-  if (lane == 31) s_scan[warp] = inc;
-  __syncthreads();
-  int before = inc - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
   const int heads = p.Hk * p.mtiles;
-  const long long U = static_cast<long long>(total) * heads;
-  const long long ctas = U < gridDim.x ? U : gridDim.x;
-  const long long cta = blockIdx.x;
-
-  // sequences with no key: zeros (the sum over nothing), lse = -inf
-  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    if (clamp_len(p, b) > 0) continue;
-    for (int i = tid; i < p.Hq * HD; i += kThreads)
-      p.o[b * p.o_b + (i / HD) * p.o_h + i % HD] = __float2bfloat16_rn(0.f);
-    if (p.lse)
-      for (int i = tid; i < p.Hq; i += kThreads) p.lse[b * p.lse_b + i] = -INFINITY;
-  }
-  if (cta >= ctas) {
-    if (tid == 0) p.desc[cta] = make_int4(-1, 0, 0, 0);
-    return;
-  }
-  const long long u0 = cut(cta, U, ctas), u1 = cut(cta + 1, U, ctas);
-  {
-    const int x = static_cast<int>(u0 / heads);
+  int U = 0, ctas = 0, rank = 0, csize = 1;
+  const int cta = blockIdx.x;
+  Walk walk;   // of the copies
+  Run first;   // of the products
+  Walk cwalk;
+  bool live;
+  if constexpr (CLUSTER) {
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+    rank = cluster_ctarank();
+    const int seg = cta / csize;
+    first.b = seg / heads;
+    first.hm = seg - first.b * heads;
+    first.len = clamp_len(p, first.b);
+    first.nu = units_of(first.len);
+    first.c0 = rank * first.nu / csize;
+    first.c1 = (rank + 1) * first.nu / csize;
+    live = first.c1 > first.c0;
+    if (seg == 0 && rank == 0)
+      for (int b = tid; b < p.B; b += kThreads)
+        if ((p.lens[b] < 0 || p.lens[b] > cap_of(p)) && p.err) atomicExch(p.err, kErrPos);
+  } else {
+    // units of all sequences, and where this CTA's range begins
+    const int per = (p.B + kThreads - 1) / kThreads;
+    const int sb0 = min(tid * per, p.B), sb1 = min(sb0 + per, p.B);
+    int mine = 0;
+    for (int b = sb0; b < sb1; ++b) {
+      const int n = p.lens[b];
+      if (cta == 0 && (n < 0 || n > cap_of(p)) && p.err) atomicExch(p.err, kErrPos);
+      mine += units_of(clamp_len(p, b));
+    }
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    int before = inc - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_scan[w];
+      total += s_scan[w];
+    }
+    U = total * heads;
+    ctas = min(U, static_cast<int>(gridDim.x));
+    // sequences with no key: zeros (the sum over nothing), lse = -inf
+    for (int b = cta; b < p.B; b += gridDim.x) {
+      if (clamp_len(p, b) > 0) continue;
+      for (int i = tid; i < p.Hq * HD; i += kThreads)
+        p.o[b * p.o_b + (i / HD) * p.o_h + i % HD] = __float2bfloat16_rn(0.f);
+      if (p.lse)
+        for (int i = tid; i < p.Hq; i += kThreads) p.lse[b * p.lse_b + i] = -INFINITY;
+    }
+    if (cta >= ctas) {
+      if (tid == 0) p.desc[cta] = make_int4(-1, 0, 0, 0);
+      return;
+    }
+    const int u0 = cut(cta, U, ctas), x = u0 / heads;
     if (x >= before && x < before + mine) {
       int b = sb0, pre = before;
       for (; b < sb1; ++b) {
@@ -226,353 +307,406 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       s_start[0] = b;
       s_start[1] = pre;
     }
-  }
-  __syncthreads();
-  int b = s_start[0];
-  long long base = static_cast<long long>(s_start[1]) * heads;
-  int4 my_desc = make_int4(-1, 0, 0, 0);
-
-  uint8_t* ring = smem + warp * (kStages * W::SB);
-  const uint32_t ring_s = smem_u32(ring);
-  float* my_o = reinterpret_cast<float*>(ring);
-  bool bad_page = false;
-
-  for (long long u = u0; u < u1;) {
-    const int len = clamp_len(p, b);
-    const int nu = units_of(len);
-    const long long local = u - base;
-    if (local >= static_cast<long long>(nu) * heads) {
-      base += static_cast<long long>(nu) * heads;
-      ++b;
-      continue;
-    }
-    const int hm = static_cast<int>(local / nu);
-    const int c0 = static_cast<int>(local % nu);
-    const int c1 = static_cast<int>(min(static_cast<long long>(nu), c0 + (u1 - u)));
-    const int h = hm / p.mtiles, mt = hm % p.mtiles;
-    const int row0 = h * p.group + mt * kRows;          // first query head of this product
-    const int nrows = min(kRows, p.group - mt * kRows);
-
-    // ---- tile copies
-    const uint8_t* kb = p.k + h * p.head_bytes;
-    const uint8_t* vb = p.v + h * p.head_bytes;
-    const int* trow = p.table + b * p.table_ld;
-    const int cpr_row = lane / W::CPR, cpr_c = lane % W::CPR;
-    const bool append = p.k_new != nullptr && len > 0 && p.lens[b] <= p.max_blocks * p.page;
-    const int ntiles = c1 - c0;
-    auto pos_of = [&](int it) { return (c0 + it) * kUnit + warp * kTile + (lane & 15); };
-    auto block_of = [&](int pos) { return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page; };
-    auto page_at = [&](int it) {
-      const int pos = pos_of(it);
-      return (it < ntiles && pos < len) ? __ldg(trow + block_of(pos)) : 0;
-    };
-    int pg = page_at(0);
-    auto issue = [&](int it) {
-      if (it < ntiles) {
-        const int pos = pos_of(it);
-        const bool in = pos < len;
-        const bool ok = in && pg >= 0 && pg < p.n_pages;
-        if (in && !ok) bad_page = true;
-        const uint32_t off =
-            ok ? static_cast<uint32_t>(pg) * p.page16 + static_cast<uint32_t>(pos - block_of(pos) * p.page) * p.tok16
-               : kNoRow;
-        const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        const int stage = it % kStages;
-        if (lane == 0) s_valid[warp][stage] = mask;
-        const uint32_t dst = ring_s + stage * W::SB;
-        const int arow = append ? len - 1 - (c0 + it) * kUnit - warp * kTile : -1;  // row of the new token, if here
-        const bool here = arow >= 0 && arow < kTile && (mask >> arow & 1);
-#pragma unroll
-        for (int i = 0; i < W::NI; ++i) {
-          const int r = i * W::RPI + cpr_row;
-          const uint32_t o = __shfl_sync(0xffffffffu, off, r);
-          const uint32_t sz = o == kNoRow ? 0u : 16u;
-          const size_t src = o == kNoRow ? 0 : static_cast<size_t>(o) * 16 + cpr_c * 16;
-          const uint32_t d = dst + W::at(r, cpr_c);
-          if (here && r == arow) {
-            const long long nb = b * p.n_b + h * p.n_h;
-            if constexpr (!FP8) {
-              const uint4 nk = reinterpret_cast<const uint4*>(p.k_new + nb)[cpr_c];
-              const uint4 nv = reinterpret_cast<const uint4*>(p.v_new + nb)[cpr_c];
-              *reinterpret_cast<uint4*>(ring + stage * W::SB + W::at(r, cpr_c)) = nk;
-              *reinterpret_cast<uint4*>(ring + stage * W::SB + W::TB + W::at(r, cpr_c)) = nv;
-              if (mt == 0) {
-                *reinterpret_cast<uint4*>(const_cast<uint8_t*>(kb) + src) = nk;
-                *reinterpret_cast<uint4*>(const_cast<uint8_t*>(vb) + src) = nv;
-              }
-            } else {
-#pragma unroll
-              for (int which = 0; which < 2; ++which) {
-                const float sc = which ? (p.v_scale ? p.v_scale[h] : 1.f) : (p.k_scale ? p.k_scale[h] : 1.f);
-                const __nv_bfloat16* x = (which ? p.v_new : p.k_new) + nb + cpr_c * 16;
-                uint4 out;
-                uint8_t* ob = reinterpret_cast<uint8_t*>(&out);
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  ob[e] = __nv_cvt_float_to_fp8(__bfloat162float(x[e]) / sc, __NV_SATFINITE, __NV_E4M3);
-                *reinterpret_cast<uint4*>(ring + stage * W::SB + which * W::TB + W::at(r, cpr_c)) = out;
-                if (mt == 0) *reinterpret_cast<uint4*>(const_cast<uint8_t*>(which ? vb : kb) + src) = out;
-              }
-            }
-          } else {
-            cp_async16(d, kb + src, sz);
-            cp_async16(d + W::TB, vb + src, sz);
-          }
-        }
-        pg = page_at(it + 1);
-      }
-      cp_commit();  // an empty group past the end keeps the count
-    };
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) issue(s);
-
-    // ---- q of this product: 16 rows, rows past the group are zero
-    uint32_t qf[W::KS][4];
-    float sl0 = p.scale_log2, sl1 = p.scale_log2;  // per-row factor of the scores (rows g, g + 8)
-    {
-      const __nv_bfloat16* q0 = p.q + b * p.q_b + static_cast<long long>(row0 + g) * p.q_h;
-      const __nv_bfloat16* q1 = q0 + 8 * p.q_h;
-      const bool r0 = g < nrows, r1 = g + 8 < nrows;
-      if constexpr (!FP8) {
-#pragma unroll
-        for (int ks = 0; ks < W::KS; ++ks) {
-          const int d = ks * 16 + t4 * 2;
-          qf[ks][0] = r0 ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
-          qf[ks][1] = r1 ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
-          qf[ks][2] = r0 ? *reinterpret_cast<const uint32_t*>(q0 + d + 8) : 0u;
-          qf[ks][3] = r1 ? *reinterpret_cast<const uint32_t*>(q1 + d + 8) : 0u;
-        }
-      } else {
-        // the k index of a product is any fixed order of the 16 dims: lane t4
-        // takes dims 4 t4 .. 4 t4 + 3, the four e4m3 bytes it gets of a key row
-        float m0 = 0.f, m1 = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < W::KS; ++ks) {
-          const int d = ks * 16 + t4 * 4;
-          const uint2 x0 = r0 ? *reinterpret_cast<const uint2*>(q0 + d) : make_uint2(0, 0);
-          const uint2 x1 = r1 ? *reinterpret_cast<const uint2*>(q1 + d) : make_uint2(0, 0);
-          qf[ks][0] = x0.x;
-          qf[ks][1] = x1.x;
-          qf[ks][2] = x0.y;
-          qf[ks][3] = x1.y;
-          m0 = fmaxf(m0, fmaxf(fmaxf(fabsf(bf16_lo(x0.x)), fabsf(bf16_hi(x0.x))),
-                               fmaxf(fabsf(bf16_lo(x0.y)), fabsf(bf16_hi(x0.y)))));
-          m1 = fmaxf(m1, fmaxf(fmaxf(fabsf(bf16_lo(x1.x)), fabsf(bf16_hi(x1.x))),
-                               fmaxf(fabsf(bf16_lo(x1.y)), fabsf(bf16_hi(x1.y)))));
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-        }
-        // largest |q| of the row to [2^14, 2^15): a power of two, exact
-        auto pow2_to = [](float m) {
-          int e = 0;
-          if (m > 0.f && m < INFINITY) frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
-          return 15 - e;
-        };
-        const int e0 = pow2_to(m0), e1 = pow2_to(m1);
-#pragma unroll
-        for (int ks = 0; ks < W::KS; ++ks) {
-          qf[ks][0] = pack_f16x2(ldexpf(bf16_lo(qf[ks][0]), e0), ldexpf(bf16_hi(qf[ks][0]), e0));
-          qf[ks][1] = pack_f16x2(ldexpf(bf16_lo(qf[ks][1]), e1), ldexpf(bf16_hi(qf[ks][1]), e1));
-          qf[ks][2] = pack_f16x2(ldexpf(bf16_lo(qf[ks][2]), e0), ldexpf(bf16_hi(qf[ks][2]), e0));
-          qf[ks][3] = pack_f16x2(ldexpf(bf16_lo(qf[ks][3]), e1), ldexpf(bf16_hi(qf[ks][3]), e1));
-        }
-        const float ksc = p.k_scale ? p.k_scale[h] : 1.f;
-        sl0 = ldexpf(p.scale_log2 * ksc, -e0);
-        sl1 = ldexpf(p.scale_log2 * ksc, -e1);
-      }
-    }
-
-    float acc[W::NT][4];
-#pragma unroll
-    for (int n = 0; n < W::NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // base-2 running max; this lane's share of the sum
-    constexpr float kUp = FP8 ? 15.f : 0.f;                    // p is kept as 2^(y - m + kUp)
-
-    for (int it = 0; it < ntiles; ++it) {
-      cp_wait<kStages - 2>();
-      __syncwarp();
-      issue(it + kStages - 1);
-      const int stage = it % kStages;
-      const uint32_t valid = s_valid[warp][stage];
-      if (valid == 0) continue;
-      const uint32_t kt = ring_s + stage * W::SB, vt = kt + W::TB;
-
-      // ---- scores: two n tiles of 8 keys
-      float s[2][4];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
-      if constexpr (!FP8) {
-#pragma unroll
-        for (int ks = 0; ks < W::KS; ++ks) {
-          uint32_t kf[4];
-          ldsm4(kf, kt + W::at(kr, 2 * ks + kc));
-          mma16816<false>(s[0], qf[ks], kf[0], kf[1]);
-          mma16816<false>(s[1], qf[ks], kf[2], kf[3]);
-        }
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < W::KS / 2; ++kk) {  // 32 dims
-          uint32_t kf[4];
-          ldsm4(kf, kt + W::at(kr, 2 * kk + kc));
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            mma16816<true>(s[0], qf[2 * kk + e], e4m3x2_f16x2(kf[e] & 0xffff), e4m3x2_f16x2(kf[e] >> 16));
-            mma16816<true>(s[1], qf[2 * kk + e], e4m3x2_f16x2(kf[2 + e] & 0xffff), e4m3x2_f16x2(kf[2 + e] >> 16));
-          }
-        }
-      }
-      // ---- running maximum and sum (base 2)
-      float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool ok = valid >> (n * 8 + t4 * 2 + e) & 1;
-          s[n][e] = ok ? s[n][e] * sl0 : -INFINITY;
-          s[n][2 + e] = ok ? s[n][2 + e] * sl1 : -INFINITY;
-          x0 = fmaxf(x0, s[n][e]);
-          x1 = fmaxf(x1, s[n][2 + e]);
-        }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
-      }
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-        const float f0 = n0 == -INFINITY ? 1.f : ex2_approx(m0 - n0), f1 = n1 == -INFINITY ? 1.f : ex2_approx(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= f0;
-        l1 *= f1;
-#pragma unroll
-        for (int n = 0; n < W::NT; ++n) {
-          acc[n][0] *= f0;
-          acc[n][1] *= f0;
-          acc[n][2] *= f1;
-          acc[n][3] *= f1;
-        }
-      }
-      const float r0 = (m0 == -INFINITY ? 0.f : m0) - kUp, r1 = (m1 == -INFINITY ? 0.f : m1) - kUp;
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[n][e] = ex2_approx(s[n][e] - r0);
-          s[n][2 + e] = ex2_approx(s[n][2 + e] - r1);
-          l0 += s[n][e];
-          l1 += s[n][2 + e];
-        }
-      // ---- o += p v
-      const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;
-      if constexpr (!FP8) {
-        uint32_t ph[4], pl[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t hi = pack_bf16x2(s[n][2 * e], s[n][2 * e + 1]);
-            ph[2 * n + e] = hi;
-            pl[2 * n + e] = pack_bf16x2(s[n][2 * e] - bf16_lo(hi), s[n][2 * e + 1] - bf16_hi(hi));
-          }
-#pragma unroll
-        for (int dd = 0; dd < HD / 16; ++dd) {
-          uint32_t vf[4];
-          ldsm4_t(vf, vt + W::at(vr, 2 * dd + vc));
-          mma16816<false>(acc[2 * dd], ph, vf[0], vf[1]);
-          mma16816<false>(acc[2 * dd + 1], ph, vf[2], vf[3]);
-          mma16816<false>(acc[2 * dd], pl, vf[0], vf[1]);
-          mma16816<false>(acc[2 * dd + 1], pl, vf[2], vf[3]);
-        }
-      } else {
-        uint32_t ph[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) ph[2 * n + e] = pack_f16x2(s[n][2 * e], s[n][2 * e + 1]);
-        // a transposed 8x8 of 16-bit units holds, per key, two neighbouring
-        // dims: n tile 2 dd takes the even dims of 16, tile 2 dd + 1 the odd ones
-#pragma unroll
-        for (int d2 = 0; d2 < HD / 32; ++d2) {
-          uint32_t vf[4];
-          ldsm4_t(vf, vt + W::at(vr, 2 * d2 + vc));
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t a = __byte_perm(vf[2 * e], 0, 0x3120), c = __byte_perm(vf[2 * e + 1], 0, 0x3120);
-            mma16816<true>(acc[4 * d2 + 2 * e], ph, e4m3x2_f16x2(a & 0xffff), e4m3x2_f16x2(c & 0xffff));
-            mma16816<true>(acc[4 * d2 + 2 * e + 1], ph, e4m3x2_f16x2(a >> 16), e4m3x2_f16x2(c >> 16));
-          }
-        }
-      }
-    }
-    cp_wait<0>();
-    __syncwarp();
-
-    // ---- the four warps' (max, sum, o) of this run, joined in shared memory
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-    }
-    if (t4 == 0) {
-      s_m[warp][g] = m0;
-      s_m[warp][g + 8] = m1;
-      s_l[warp][g] = l0;
-      s_l[warp][g + 8] = l1;
-    }
-#pragma unroll
-    for (int n = 0; n < W::NT; ++n) {
-      if constexpr (!FP8) {
-        if (g < nrows) *reinterpret_cast<float2*>(my_o + g * OS + n * 8 + t4 * 2) = make_float2(acc[n][0], acc[n][1]);
-        if (g + 8 < nrows)
-          *reinterpret_cast<float2*>(my_o + (g + 8) * OS + n * 8 + t4 * 2) = make_float2(acc[n][2], acc[n][3]);
-      } else if ((n & 1) == 0) {
-        if (g < nrows)
-          *reinterpret_cast<float4*>(my_o + g * OS + n * 8 + t4 * 4) =
-              make_float4(acc[n][0], acc[n + 1][0], acc[n][1], acc[n + 1][1]);
-        if (g + 8 < nrows)
-          *reinterpret_cast<float4*>(my_o + (g + 8) * OS + n * 8 + t4 * 4) =
-              make_float4(acc[n][2], acc[n + 1][2], acc[n][3], acc[n + 1][3]);
-      }
-    }
     __syncthreads();
-    const bool first = c0 == 0, last = c1 == nu;
-    const int slot = static_cast<int>(2 * cta) + (first ? 1 : 0);  // a run that began earlier goes to slot 0
-    if (first && !last) {
-      const long long end = u - c0 + nu;  // unit after this (sequence, head)'s last
-      my_desc = make_int4(b, hm, static_cast<int>((end * ctas - 1) / U), 0);
-    }
-    const float vsc = (FP8 && p.v_scale) ? p.v_scale[h] : 1.f;
-    for (int i = tid; i < nrows * HD; i += kThreads) {
-      const int r = i / HD, d = i % HD;
-      float M = s_m[0][r];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[w][r]);
-      const float ref = M == -INFINITY ? 0.f : M;
-      float L = 0.f, O = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2_approx(s_m[w][r] - ref);
-        L += f * s_l[w][r];
-        O += f * reinterpret_cast<const float*>(smem + w * (kStages * W::SB))[r * OS + d];
-      }
-      if (first && last) {
-        p.o[b * p.o_b + (row0 + r) * p.o_h + d] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * vsc);
-        if (d == 0 && p.lse)
-          p.lse[b * p.lse_b + row0 + r] = L == 0.f ? -INFINITY : (M + log2f(L) - kUp) * kLn2;
-      } else {
-        p.part_o[(static_cast<long long>(slot) * p.rows + r) * HD + d] = O;
-        if (d == 0) p.part_ml[static_cast<long long>(slot) * p.rows + r] = make_float2(M, L);
-      }
-    }
-    __syncthreads();  // the next run's copies overwrite the warps' o
-    u += c1 - c0;
+    walk.u = u0;
+    walk.u1 = cut(cta + 1, U, ctas);
+    walk.b = s_start[0];
+    walk.base = s_start[1] * heads;
+    live = walk.next(p, first);
+    cwalk = walk;
   }
-  if (tid == 0) p.desc[cta] = my_desc;
+
+  // ---- copies: the ring is filled STAGES - 1 tiles ahead, run after run
+  uint8_t* ring = smem + warp * (S::STAGES * S::SB);
+  const uint32_t ring_s = smem_u32(ring);
+  const int my_row = lane / S::CPR, my_chunk = lane % S::CPR;
+  const bool whole = p.page % kTile == 0;  // a tile lies in one page
+  bool bad_page = false;
+  bool more = live;         // tiles left to copy
+  Run in = first;           // run being copied
+  int unit = first.c0;      // its next unit
+  int in_stage = 0;
+  int pg = 0;               // page of the next tile (of key lane % 16 of it, if tiles are not whole)
+  auto block_of = [&](int pos) { return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page; };
+  auto look_up = [&]() {
+    const int pos = unit * kUnit + warp * kTile + (whole ? 0 : (lane & 15));
+    pg = (more && pos < in.len) ? __ldg(p.table + in.b * p.table_ld + block_of(pos)) : 0;
+  };
+  auto copy_tile = [&]() {
+    if (more) {
+      const int h = in.hm / p.mtiles;
+      const int k0 = unit * kUnit + warp * kTile;
+      const int left = in.len - k0;  // keys of the tile that exist
+      const bool in_cache = pg >= 0 && pg < p.n_pages;
+      const size_t head_off = h * p.head_bytes + my_chunk * 16;
+      const uint8_t* kb = p.k + head_off;
+      const uint8_t* vb = p.v + head_off;
+      const uint32_t dst = ring_s + in_stage * S::SB;
+      uint32_t mask, off;
+      if (whole) {
+        mask = left >= kTile ? 0xffffu : (left > 0 ? (1u << left) - 1 : 0u);
+        if (mask && !in_cache) {
+          bad_page = true;
+          mask = 0;
+        }
+        off = static_cast<uint32_t>(pg) * p.page16 + static_cast<uint32_t>(k0 - block_of(k0) * p.page) * p.tok16;
+      } else {
+        const int pos = k0 + (lane & 15);
+        const bool here = pos < in.len;
+        if (here && !in_cache) bad_page = true;
+        mask = __ballot_sync(0xffffffffu, here && in_cache) & 0xffffu;
+        off = static_cast<uint32_t>(pg) * p.page16 + static_cast<uint32_t>(pos - block_of(pos) * p.page) * p.tok16;
+      }
+      if (lane == 0) s_valid[warp][in_stage] = mask;
+      // row of the new token, if it is in this tile (and has a page)
+      int arow = -1;
+      if (p.k_new != nullptr && left > 0 && left <= kTile && (mask >> (left - 1) & 1) && p.lens[in.b] <= cap_of(p))
+        arow = left - 1;
+#pragma unroll
+      for (int i = 0; i < S::NI; ++i) {
+        const int r = i * S::RPI + my_row;
+        const uint32_t o = whole ? off + r * p.tok16 : __shfl_sync(0xffffffffu, off, r);
+        const bool ok = mask >> r & 1;
+        const size_t src = ok ? static_cast<size_t>(o) * 16 : 0;
+        const uint32_t d = dst + S::at(r, my_chunk);
+        if (r != arow) {
+          cp_async16(d, kb + src, ok ? 16u : 0u);
+          cp_async16(d + S::TB, vb + src, ok ? 16u : 0u);
+        } else {
+          // the new token: from k_new, v_new into the tile, and into its slot
+          const long long nb = in.b * p.n_b + h * p.n_h + my_chunk * (FP8 ? 16 : 8);
+#pragma unroll
+          for (int which = 0; which < 2; ++which) {
+            const __nv_bfloat16* x = (which ? p.v_new : p.k_new) + nb;
+            uint4 val;
+            if constexpr (!FP8) {
+              val = *reinterpret_cast<const uint4*>(x);
+            } else {
+              const float* scp = which ? p.v_scale : p.k_scale;
+              const float sc = scp ? scp[h] : 1.f;
+              uint8_t* ob = reinterpret_cast<uint8_t*>(&val);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                ob[e] = __nv_cvt_float_to_fp8(__bfloat162float(x[e]) / sc, __NV_SATFINITE, __NV_E4M3);
+            }
+            *reinterpret_cast<uint4*>(ring + in_stage * S::SB + which * S::TB + S::at(r, my_chunk)) = val;
+            if (in.hm % p.mtiles == 0)
+              *reinterpret_cast<uint4*>(const_cast<uint8_t*>(which ? vb : kb) + src) = val;
+          }
+        }
+      }
+      if (++unit == in.c1) {
+        if constexpr (CLUSTER) more = false;
+        else more = walk.next(p, in);
+        unit = in.c0;
+      }
+      look_up();
+    }
+    in_stage = in_stage + 1 == S::STAGES ? 0 : in_stage + 1;
+    cp_commit();  // an empty group past the end keeps the count
+  };
+
+  // ---- q of a run: column g of tile n is query head row0 + 8 n + g; zero past the group
+  uint32_t qf[NH][S::KS][2];
+  float sl[NH][2];  // factor of the scores of columns 2 t4, 2 t4 + 1
+  auto load_q = [&](const Run& r) {
+    const int h = r.hm / p.mtiles, mt = r.hm - h * p.mtiles;
+    const int have = min(p.rows, p.group - mt * p.rows);
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const bool in_group = n * kHeads + g < have;
+      const __nv_bfloat16* qr = p.q + r.b * p.q_b + (h * p.group + mt * p.rows + n * kHeads + g) * p.q_h;
+#pragma unroll
+      for (int ks = 0; ks < S::KS; ++ks) {
+        if constexpr (!FP8) {
+          qf[n][ks][0] = in_group ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + t4 * 2) : 0u;
+          qf[n][ks][1] = in_group ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + t4 * 2 + 8) : 0u;
+        } else {
+          // the k index of a product may run over the 16 dims in any fixed order:
+          // lane t4 takes dims 4 t4 .. 4 t4 + 3, the four e4m3 bytes it gets of a key row
+          const uint2 x = in_group ? *reinterpret_cast<const uint2*>(qr + ks * 16 + t4 * 4) : make_uint2(0, 0);
+          qf[n][ks][0] = x.x;
+          qf[n][ks][1] = x.y;
+        }
+      }
+    }
+  };
+  auto scale_q = [&](const Run& r) {
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      if constexpr (!FP8) {
+        sl[n][0] = sl[n][1] = p.scale_log2;
+      } else {
+        float m = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            m = fmaxf(m, fmaxf(fabsf(bf16_lo(qf[n][ks][e])), fabsf(bf16_hi(qf[n][ks][e]))));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        // 2^e takes the head's largest |q| to [2^14, 2^15): exponent of m from its bits
+        // (m is a bf16 value; below 2^-100 it is scaled by 2^114 at most)
+        const int ex = max(static_cast<int>(__float_as_uint(m) >> 23), 27) - 127;
+        const float up = m < INFINITY ? __uint_as_float(static_cast<uint32_t>(min(14 - ex, 127) + 127) << 23) : 1.f;
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            qf[n][ks][e] = pack_f16x2(bf16_lo(qf[n][ks][e]) * up, bf16_hi(qf[n][ks][e]) * up);
+        const float ksc = p.k_scale ? p.k_scale[r.hm / p.mtiles] : 1.f;
+        const float down = p.scale_log2 * ksc / up;
+        sl[n][0] = __shfl_sync(0xffffffffu, down, 8 * t4);      // column 2 t4 is lane 4 (2 t4)'s
+        sl[n][1] = __shfl_sync(0xffffffffu, down, 8 * t4 + 4);
+      }
+    }
+  };
+
+  look_up();
+  if (live) load_q(first);
+#pragma unroll
+  for (int s = 0; s < S::STAGES - 1; ++s) copy_tile();
+
+  int4 my_desc = make_int4(-1, 0, 0, 0);
+  Run r = first;
+  int stage = 0;
+  while (live || CLUSTER) {
+    if (live) scale_q(r);
+    float acc[NH][S::KS][4];
+    float m[NH][2], l[NH][2];  // columns 2 t4, 2 t4 + 1: maximum (base 2), this lane's share of the sum
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < S::KS; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
+    }
+
+    for (int c = r.c0; c < r.c1; ++c) {
+      cp_wait<S::STAGES - 2>();
+      __syncwarp();
+      copy_tile();
+      const uint32_t kt = ring_s + stage * S::SB, vt = kt + S::TB;
+      const uint32_t valid = s_valid[warp][stage];
+      stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+      if (valid == 0) continue;
+
+      // ---- scores: rows (keys) g, g + 8; columns (heads) 2 t4, 2 t4 + 1
+      float y[NH][4];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
+      if constexpr (!FP8) {
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ++ks) {
+          uint32_t a[4];
+          ldsm4(a, kt + S::at(lane & 15, 2 * ks + (lane >> 4)));
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma16816<false>(y[n], a, qf[n][ks][0], qf[n][ks][1]);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < S::KS / 2; ++kk) {  // 32 dims
+          uint32_t x[4];
+          ldsm4(x, kt + S::at(lane & 15, 2 * kk + (lane >> 4)));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t a[4] = {e4m3x2_f16x2(x[2 * e]), e4m3x2_f16x2(x[2 * e + 1]), e4m3x2_f16x2(x[2 * e] >> 16),
+                                   e4m3x2_f16x2(x[2 * e + 1] >> 16)};
+#pragma unroll
+            for (int n = 0; n < NH; ++n) mma16816<true>(y[n], a, qf[n][2 * kk + e][0], qf[n][2 * kk + e][1]);
+          }
+        }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[n][e] *= sl[n][e & 1];
+          if (valid != 0xffffu && !(valid >> (g + 8 * (e >> 1)) & 1)) y[n][e] = -INFINITY;
+          grow = grow || y[n][e] > m[n][e & 1] + kSlack;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(y[n][e], y[n][2 + e]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            x = fmaxf(x, m[n][e]);
+            const float f = x == -INFINITY ? 1.f : ex2_approx(m[n][e] - x);
+            m[n][e] = x;
+            l[n][e] *= f;
+#pragma unroll
+            for (int i = 0; i < S::KS; ++i) {
+              acc[n][i][e] *= f;
+              acc[n][i][2 + e] *= f;
+            }
+          }
+      }
+      uint32_t ph[NH][2], pl[NH][2];  // p^T as the second product's columns; its low part
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ref = (m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1]) - kUp;
+          y[n][e] = ex2_approx(y[n][e] - ref);
+          l[n][e & 1] += y[n][e];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if constexpr (FP8) {
+            ph[n][e] = transpose8(pack_f16x2(y[n][2 * e], y[n][2 * e + 1]));
+          } else {
+            const uint32_t hi = pack_bf16x2(y[n][2 * e], y[n][2 * e + 1]);
+            ph[n][e] = transpose8(hi);
+            pl[n][e] = transpose8(pack_bf16x2(y[n][2 * e] - bf16_lo(hi), y[n][2 * e + 1] - bf16_hi(hi)));
+          }
+        }
+      }
+      // ---- o^T += v^T p^T
+      if constexpr (!FP8) {
+#pragma unroll
+        for (int i = 0; i < S::KS; ++i) {
+          uint32_t a[4];
+          ldsm4_t(a, vt + S::at((lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int n = 0; n < NH; ++n) {
+            mma16816<false>(acc[n][i], a, ph[n][0], ph[n][1]);
+            mma16816<false>(acc[n][i], a, pl[n][0], pl[n][1]);
+          }
+        }
+      } else {
+        // a transposed 8x8 of 16-bit units holds, per key, two neighbouring dims:
+        // rows g of a tile are the even dims of 16, rows g + 8 the odd ones
+#pragma unroll
+        for (int ii = 0; ii < S::KS / 2; ++ii) {
+          uint32_t x[4];
+          ldsm4_t(x, vt + S::at(lane & 15, 2 * ii + (lane >> 4)));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t lo = __byte_perm(x[2 * e], 0, 0x3120), hi = __byte_perm(x[2 * e + 1], 0, 0x3120);
+            const uint32_t a[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2(lo >> 16), e4m3x2_f16x2(hi),
+                                   e4m3x2_f16x2(hi >> 16)};
+#pragma unroll
+            for (int n = 0; n < NH; ++n) mma16816<true>(acc[n][2 * ii + e], a, ph[n][0], ph[n][1]);
+          }
+        }
+      }
+    }
+
+    // ---- the next run's q is on its way while this run's four warps are joined
+    Run nr = r;
+    bool again = false;
+    if constexpr (!CLUSTER) {
+      again = cwalk.next(p, nr);
+      if (again) load_q(nr);
+    }
+    const int h = r.hm / p.mtiles, mt = r.hm - h * p.mtiles;
+    const int row0 = h * p.group + mt * p.rows, nrows = min(p.rows, p.group - mt * p.rows);
+    const bool begins = r.c0 == 0, ends = r.c1 == r.nu;
+    const int slot = 2 * cta + (begins ? 1 : 0);  // a run that began in an earlier CTA goes to slot 0
+    if constexpr (!CLUSTER)
+      if (begins && !ends) {
+        const int end = cut(cta + 1, U, ctas) - r.c1 + r.nu;  // unit after this segment's last
+        my_desc = make_int4(r.b, r.hm, static_cast<int>((static_cast<long long>(end) * ctas - 1) / U), 0);
+      }
+    const float vsc = (FP8 && p.v_scale) ? p.v_scale[h] : 1.f;
+#pragma unroll
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+        if (g == 0) {
+          s_m[warp][n * kHeads + 2 * t4 + e] = m[n][e];
+          s_l[warp][n * kHeads + 2 * t4 + e] = l[n][e];
+        }
+      }
+    float* scratch = reinterpret_cast<float*>(smem + S::RING);
+    float* part = reinterpret_cast<float*>(smem);  // clustered: [rows][HD] over the ring, which is idle by then
+    if constexpr (CLUSTER) {
+      cp_wait<0>();
+      __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      // warp w sums element w of every accumulator: column 2 t4 + (w & 1), row g or g + 8
+      const int col = n * kHeads + 2 * t4 + (warp & 1);
+      float f[kWarps], M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int i0 = 0; i0 < S::KS; i0 += S::MT) {
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) scratch[((warp * S::MT + i) * 4 + e) * 32 + lane] = acc[n][i0 + i][e];
+        __syncthreads();
+        if (i0 == 0) {
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][col]);
+          const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            f[w] = ex2_approx(s_m[w][col] - ref);
+            L += f[w] * s_l[w][col];
+          }
+        }
+        if (col < nrows) {
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i) {
+            float O = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) O += f[w] * scratch[((w * S::MT + i) * 4 + warp) * 32 + lane];
+            const int d = (i0 + i) * 16 + (FP8 ? 2 * g + (warp >> 1) : g + 8 * (warp >> 1));
+            if constexpr (CLUSTER) {
+              part[col * HD + d] = O;
+              if (d == 0) s_ml[col] = make_float2(M, L);
+            } else if (begins && ends) {
+              p.o[r.b * p.o_b + (row0 + col) * p.o_h + d] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * vsc);
+              if (d == 0 && p.lse)
+                p.lse[r.b * p.lse_b + row0 + col] = L == 0.f ? -INFINITY : (M + log2f(L) - kUp) * kLn2;
+            } else {
+              p.part_o[(static_cast<long long>(slot) * p.rows + col) * HD + d] = O;
+              if (d == 0) p.part_ml[static_cast<long long>(slot) * p.rows + col] = make_float2(M, L);
+            }
+          }
+        }
+        __syncthreads();  // scratch and s_m are written again
+      }
+    }
+    if constexpr (CLUSTER) {
+      // ---- every CTA of the cluster joins its share of the elements
+      cluster_sync();
+      for (int i = rank * kThreads + tid; i < nrows * HD; i += csize * kThreads) {
+        const int col = i / HD, d = i - col * HD;
+        float M = -INFINITY, L = 0.f, O = 0.f;
+        float cm[kMaxCluster];
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+          cm[k] = k < csize ? ld_cluster(mapa_shared(smem_u32(&s_ml[col]), k)) : -INFINITY;
+          M = fmaxf(M, cm[k]);
+        }
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k)
+          if (k < csize) {
+            const float f = ex2_approx(cm[k] - ref);
+            L += f * ld_cluster(mapa_shared(smem_u32(&s_ml[col].y), k));
+            O += f * ld_cluster(mapa_shared(smem_u32(part + i), k));
+          }
+        p.o[r.b * p.o_b + (row0 + col) * p.o_h + d] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * vsc);
+        if (d == 0 && p.lse)
+          p.lse[r.b * p.lse_b + row0 + col] = L == 0.f ? -INFINITY : (M + log2f(L) - kUp) * kLn2;
+      }
+      cluster_sync();  // no CTA leaves while another reads its shared memory
+      break;
+    }
+    r = nr;
+    live = again;
+  }
+  if constexpr (!CLUSTER)
+    if (tid == 0) p.desc[cta] = my_desc;
   if (bad_page && p.err) atomicExch(p.err, kErrPage);
 }
 
@@ -583,7 +717,7 @@ template <int HD, bool FP8>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   constexpr int LPR = HD / 4;                     // lanes (of float4) that cover a row
   constexpr int GR = kJoinThreads / LPR;          // groups of lanes
-  constexpr float kUp = FP8 ? 15.f : 0.f;
+  constexpr float kUp = FP8 ? 7.f : 0.f;
   __shared__ float4 s_o[GR][LPR];
   __shared__ float s_ml[GR];
   griddep_sync();
@@ -591,8 +725,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   const int4 d = p.desc[j];
   if (d.x < 0) return;
   const int b = d.x, h = d.y / p.mtiles, mt = d.y % p.mtiles, n = d.z - j + 1;
-  const int nrows = min(kRows, p.group - mt * kRows);
-  const int row0 = h * p.group + mt * kRows;
+  const int nrows = min(p.rows, p.group - mt * p.rows);
+  const int row0 = h * p.group + mt * p.rows;
   const int li = threadIdx.x % LPR, gi = threadIdx.x / LPR;
   // partial i of this segment: slot 2 j + 1, then slot 0 of the CTAs that follow
   auto slot = [&](int i) { return i == 0 ? 2LL * j + 1 : 2LL * (j + i); };
@@ -643,48 +777,108 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
 }
 
 // Resident CTAs of an SM, asked once per device (0: the query failed).
-template <int HD, bool FP8>
+template <int HD, bool FP8, int NH>
 int ctas_per_sm() {
-  constexpr int smem = kWarps * kStages * Warp<HD, FP8>::SB;
   constexpr int kMaxDev = 64;
+  constexpr int smem = Shape<HD, FP8>::SMEM;
   static int known[kMaxDev] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return 0;
   if (known[dev] == 0) {
     int k = 0;
-    if (cudaFuncSetAttribute(decode_kernel<HD, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+    if (cudaFuncSetAttribute(decode_kernel<HD, FP8, NH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
             cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&k, decode_kernel<HD, FP8>, kThreads, smem) != cudaSuccess)
+        cudaFuncSetAttribute(decode_kernel<HD, FP8, NH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&k, decode_kernel<HD, FP8, NH, false>, kThreads, smem) !=
+            cudaSuccess)
       return 0;
     known[dev] = k;
   }
   return known[dev];
 }
 
-// CTAs of a call: what the card holds at once, or fewer where even full block
-// tables have fewer units.
-template <int HD, bool FP8>
-int grid_of(int B, int Hk, int mtiles, int max_blocks, int page) {
-  const int occ = ctas_per_sm<HD, FP8>();
-  if (occ <= 0) return 0;
-  const long long most = static_cast<long long>(B) * Hk * mtiles *
-                         ((static_cast<long long>(max_blocks) * page + kUnit - 1) / kUnit);
+// How a call is launched: clustered with `cluster` CTAs per (sequence, head
+// tile), or (cluster 0) flat with `grid` CTAs.
+struct Plan {
+  int grid, cluster;
+};
+
+template <int HD, bool FP8, int NH>
+Plan plan_of(int B, int heads, int max_blocks, int page) {
+  const int occ = ctas_per_sm<HD, FP8, NH>();
+  if (occ <= 0) return {0, 0};
   const long long card = static_cast<long long>(sm_count()) * occ;
-  return static_cast<int>(most < card ? most : card);
+  const long long segs = static_cast<long long>(B) * heads;
+  const long long units = (static_cast<long long>(max_blocks) * page + kUnit - 1) / kUnit;  // of a full table row
+  int c = 1;
+  while (c < kMaxCluster && 2 * c <= units && segs * 2 * c <= card) c *= 2;
+  if (units <= 8 * c && segs * c <= INT32_MAX) return {static_cast<int>(segs * c), c};
+  return {static_cast<int>(segs * units < card ? segs * units : card), 0};
 }
 
-template <int HD, bool FP8>
-int launch(Params& p, cudaStream_t stream) {
-  constexpr int smem = kWarps * kStages * Warp<HD, FP8>::SB;
-  const int grid = grid_of<HD, FP8>(p.B, p.Hk, p.mtiles, p.max_blocks, p.page);
-  if (grid <= 0) return NL_ERR_CUDA;
-  launch_kernel(decode_kernel<HD, FP8>, dim3(grid), dim3(kThreads), smem, stream, 1, p);
+template <int HD, bool FP8, int NH>
+int launch(Params& p, const Plan& plan, cudaStream_t stream) {
+  constexpr int smem = Shape<HD, FP8>::SMEM;
+  if (plan.cluster > 0) {
+    launch_kernel(decode_kernel<HD, FP8, NH, true>, dim3(plan.grid), dim3(kThreads), smem, stream, plan.cluster, p);
+    return launch_status();
+  }
+  launch_kernel(decode_kernel<HD, FP8, NH, false>, dim3(plan.grid), dim3(kThreads), smem, stream, 1, p);
   const int st = launch_status();
-  if (st != NL_OK || static_cast<long long>(p.max_blocks) * p.page <= kUnit) return st;  // one unit each: no partials
+  if (st != NL_OK) return st;
   // few (sequence, head) pairs: many partials each, so their rows are split over blocks too
   const int ysplit = static_cast<long long>(p.B) * p.Hk * p.mtiles <= 16 ? p.rows : 1;
-  launch_kernel(join_kernel<HD, FP8>, dim3(grid, ysplit), dim3(kJoinThreads), 0, stream, 1, p);
+  launch_kernel(join_kernel<HD, FP8>, dim3(plan.grid, ysplit), dim3(kJoinThreads), 0, stream, 1, p);
   return launch_status();
+}
+
+// Calls f<HD, FP8, NH>() of a shape that was checked.
+template <typename F>
+auto dispatch(int d, bool fp8, int rows, F f) {
+  const bool two = rows > kHeads;
+  if (d == 64)
+    return fp8 ? (two ? f.template operator()<64, true, 2>() : f.template operator()<64, true, 1>())
+               : (two ? f.template operator()<64, false, 2>() : f.template operator()<64, false, 1>());
+  return fp8 ? (two ? f.template operator()<128, true, 2>() : f.template operator()<128, true, 1>())
+             : (two ? f.template operator()<128, false, 2>() : f.template operator()<128, false, 1>());
+}
+struct PlanCall {
+  int B, heads, max_blocks, page;
+  template <int HD, bool FP8, int NH>
+  Plan operator()() const { return plan_of<HD, FP8, NH>(B, heads, max_blocks, page); }
+};
+struct LaunchCall {
+  Params& p;
+  const Plan& plan;
+  cudaStream_t stream;
+  template <int HD, bool FP8, int NH>
+  int operator()() const { return launch<HD, FP8, NH>(p, plan, stream); }
+};
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+// Workspace of a flat call: partials and descriptors (a clustered call needs none).
+size_t workspace(const Plan& plan, int rows, int d, size_t* ml, size_t* desc) {
+  if (plan.cluster > 0) return 0;
+  size_t n = align256(static_cast<size_t>(2) * plan.grid * rows * d * sizeof(float));
+  if (ml) *ml = n;
+  n += align256(static_cast<size_t>(2) * plan.grid * rows * sizeof(float2));
+  if (desc) *desc = n;
+  return n + align256(static_cast<size_t>(plan.grid) * sizeof(int4));
+}
+// Query heads of one CTA's product (the group in equal parts of at most 16) and the parts of a group.
+void split_group(int group, int* rows, int* mtiles) {
+  *mtiles = (group + kHeads * kMaxTiles - 1) / (kHeads * kMaxTiles);
+  *rows = (group + *mtiles - 1) / *mtiles;
+}
+bool shape_ok(int B, int Hq, int Hk, int d, int page, int max_blocks) {
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || (d != 64 && d != 128) || page <= 0 || max_blocks <= 0) return false;
+  int rows, mtiles;
+  split_group(Hq / Hk, &rows, &mtiles);
+  const long long cap = static_cast<long long>(max_blocks) * page;
+  // unit counts of a call are 32-bit
+  return cap <= INT32_MAX - kUnit &&
+         static_cast<double>(B) * Hk * mtiles * static_cast<double>((cap + kUnit - 1) / kUnit) <= INT32_MAX;
 }
 
 }  // namespace pa
@@ -692,36 +886,14 @@ int launch(Params& p, cudaStream_t stream) {
 
 using namespace nl;
 
-namespace {
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-// Workspace for the most CTAs a call can use: partials and descriptors.
-size_t paged_ws(int rows, int d, int ctas, size_t* ml, size_t* desc) {
-  size_t n = align256(static_cast<size_t>(2) * ctas * rows * d * sizeof(float));
-  if (ml) *ml = n;
-  n += align256(static_cast<size_t>(2) * ctas * rows * sizeof(float2));
-  if (desc) *desc = n;
-  return n + align256(static_cast<size_t>(ctas) * sizeof(int4));
-}
-int paged_grid(int d, int dtype, int B, int Hk, int mtiles, int max_blocks, int page) {
-  if (d == 64)
-    return dtype == NL_E4M3 ? pa::grid_of<64, true>(B, Hk, mtiles, max_blocks, page)
-                            : pa::grid_of<64, false>(B, Hk, mtiles, max_blocks, page);
-  return dtype == NL_E4M3 ? pa::grid_of<128, true>(B, Hk, mtiles, max_blocks, page)
-                          : pa::grid_of<128, false>(B, Hk, mtiles, max_blocks, page);
-}
-bool paged_shape_ok(int B, int Hq, int Hk, int d, int page, int max_blocks) {
-  return B > 0 && Hq > 0 && Hk > 0 && Hq % Hk == 0 && (d == 64 || d == 128) && page > 0 && max_blocks > 0 &&
-         static_cast<long long>(max_blocks) * page <= INT32_MAX - pa::kUnit &&
-         B * ((static_cast<long long>(max_blocks) * page + pa::kUnit - 1) / pa::kUnit) <= INT32_MAX;
-}
-}  // namespace
-
 extern "C" size_t nl_paged_attention_workspace_bytes(int B, int Hq, int Hk, int d, int page_size, int max_blocks,
                                                      int cache_dtype) {
-  if (!paged_shape_ok(B, Hq, Hk, d, page_size, max_blocks)) return 0;
-  const int group = Hq / Hk, rows = group < pa::kRows ? group : pa::kRows;
-  const int grid = paged_grid(d, cache_dtype, B, Hk, (group + pa::kRows - 1) / pa::kRows, max_blocks, page_size);
-  return grid <= 0 ? 0 : paged_ws(rows, d, grid, nullptr, nullptr);
+  if (!pa::shape_ok(B, Hq, Hk, d, page_size, max_blocks)) return 0;
+  int rows, mtiles;
+  pa::split_group(Hq / Hk, &rows, &mtiles);
+  const pa::Plan plan =
+      pa::dispatch(d, cache_dtype == NL_E4M3, rows, pa::PlanCall{B, Hk * mtiles, max_blocks, page_size});
+  return pa::workspace(plan, rows, d, nullptr, nullptr);
 }
 
 extern "C" int nl_paged_attention(const void* q, long long q_b, long long q_h, void* k_cache, void* v_cache,
@@ -732,7 +904,7 @@ extern "C" int nl_paged_attention(const void* q, long long q_b, long long q_h, v
                                   long long o_h, float* lse, long long lse_b, void* workspace, size_t ws_bytes, int B,
                                   int Hq, int Hk, int d, int page_size, int max_blocks, int n_pages,
                                   cudaStream_t stream) {
-  if (!paged_shape_ok(B, Hq, Hk, d, page_size, max_blocks) || n_pages <= 0 || table_ld < max_blocks)
+  if (!pa::shape_ok(B, Hq, Hk, d, page_size, max_blocks) || n_pages <= 0 || table_ld < max_blocks)
     return NL_ERR_SHAPE;
   if (cache_dtype != NL_BF16 && cache_dtype != NL_E4M3) return NL_ERR_DTYPE;
   if (!q || !k_cache || !v_cache || !block_table || !lens || !o || (k_new != nullptr) != (v_new != nullptr))
@@ -750,14 +922,15 @@ extern "C" int nl_paged_attention(const void* q, long long q_b, long long q_h, v
   const long long extent = (n_pages - 1) * (page_stride * el / 16) + (page_size - 1) * (tok_stride * el / 16);
   if (page_stride * el / 16 > UINT32_MAX || tok_stride * el / 16 > UINT32_MAX || extent >= UINT32_MAX)
     return NL_ERR_TOO_LARGE;
-  const int group = Hq / Hk;
   pa::Params p;
-  p.rows = group < pa::kRows ? group : pa::kRows;
-  p.mtiles = (group + pa::kRows - 1) / pa::kRows;
-  const int grid = paged_grid(d, cache_dtype, B, Hk, p.mtiles, max_blocks, page_size);
-  if (grid <= 0) return NL_ERR_CUDA;
-  size_t ml, desc;
-  if (!workspace || ws_bytes < paged_ws(p.rows, d, grid, &ml, &desc)) return NL_ERR_WORKSPACE;
+  p.group = Hq / Hk;
+  pa::split_group(p.group, &p.rows, &p.mtiles);
+  const pa::Plan plan =
+      pa::dispatch(d, cache_dtype == NL_E4M3, p.rows, pa::PlanCall{B, Hk * p.mtiles, max_blocks, page_size});
+  if (plan.grid <= 0) return NL_ERR_CUDA;
+  size_t ml = 0, desc = 0;
+  const size_t need = pa::workspace(plan, p.rows, d, &ml, &desc);
+  if (need > 0 && (!workspace || ws_bytes < need)) return NL_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = reinterpret_cast<float2*>(ws + ml);
@@ -787,13 +960,11 @@ extern "C" int nl_paged_attention(const void* q, long long q_b, long long q_h, v
   p.B = B;
   p.Hq = Hq;
   p.Hk = Hk;
-  p.group = group;
   p.page = page_size;
   p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   p.max_blocks = max_blocks;
   p.n_pages = n_pages;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = device_error_word();
-  if (d == 64) return cache_dtype == NL_E4M3 ? pa::launch<64, true>(p, stream) : pa::launch<64, false>(p, stream);
-  return cache_dtype == NL_E4M3 ? pa::launch<128, true>(p, stream) : pa::launch<128, false>(p, stream);
+  return pa::dispatch(d, cache_dtype == NL_E4M3, p.rows, pa::LaunchCall{p, plan, stream});
 }
