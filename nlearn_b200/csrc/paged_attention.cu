@@ -60,6 +60,10 @@ constexpr int kHeads = 8;                 // query heads of one product (its col
 constexpr int kMaxTiles = 2;              // products of 8 heads a CTA keeps: groups of up to 16 read the keys once
 constexpr int kMaxCluster = 8;
 constexpr int kJoinThreads = 256;
+// Starting a run and joining its warps costs a CTA about as much as one unit
+// (a fit of CTA times on ragged batches: 1.38 us a unit and 1.60 us a run, bf16,
+// d 128; 1.79 and 2.48 us, e4m3), so it is counted as one.
+constexpr int kOver = 1;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;             // log2 of how far p may grow before the maximum moves
 constexpr uint32_t kNoRow = 0xffffffffu;
@@ -159,6 +163,8 @@ __device__ __forceinline__ int clamp_len(const Params& p, int b) {
   return n < 0 ? 0 : (n > cap ? cap : n);
 }
 __device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
+// Length of one (sequence, head tile) in the flat list: its units, after kOver for its start and its join.
+__device__ __forceinline__ int weight_of(int len) { return len > 0 ? units_of(len) + kOver : 0; }
 
 // First unit of CTA i of n over U units.
 __device__ __forceinline__ int cut(int i, int U, int n) {
@@ -169,29 +175,32 @@ __device__ __forceinline__ int cut(int i, int U, int n) {
 struct Run {
   int b, hm, len, nu, c0, c1;
 };
-// Walks a CTA's range of the flat list, run by run.
+// Walks a CTA's range of the flat list, run by run (a run is not empty).
 struct Walk {
   int u, u1;     // next unit, end of the range
   int b, base;   // sequence of unit u (or an earlier one), units before it
   __device__ __forceinline__ bool next(const Params& p, Run& r) {
-    if (u >= u1) return false;
     const int heads = p.Hk * p.mtiles;
-    int len, nu;
-    for (;; ++b) {
-      len = clamp_len(p, b);
-      nu = units_of(len);
-      if (u - base < nu * heads) break;
-      base += nu * heads;
+    while (u < u1) {
+      int len, w;
+      for (;; ++b) {
+        len = clamp_len(p, b);
+        w = weight_of(len);
+        if (u - base < w * heads) break;
+        base += w * heads;
+      }
+      const int local = u - base;
+      r.b = b;
+      r.len = len;
+      r.nu = w - kOver;
+      r.hm = local / w;
+      const int c = local - r.hm * w, n = min(w - c, u1 - u);
+      r.c0 = max(0, c - kOver);
+      r.c1 = max(0, c + n - kOver);
+      u += n;
+      if (r.c1 > r.c0) return true;
     }
-    const int local = u - base;
-    r.b = b;
-    r.len = len;
-    r.nu = nu;
-    r.hm = local / nu;
-    r.c0 = local - r.hm * nu;
-    r.c1 = min(nu, r.c0 + (u1 - u));
-    u += r.c1 - r.c0;
-    return true;
+    return false;
   }
 };
 
@@ -240,8 +249,8 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   const int heads = p.Hk * p.mtiles;
   int U = 0, ctas = 0, rank = 0, csize = 1;
   const int cta = blockIdx.x;
-  Walk walk;   // of the copies
-  Run first;   // of the products
+  Walk walk;       // of the copies
+  Run first = {};  // of the products
   Walk cwalk;
   bool live;
   if constexpr (CLUSTER) {
@@ -259,14 +268,14 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
       for (int b = tid; b < p.B; b += kThreads)
         if ((p.lens[b] < 0 || p.lens[b] > cap_of(p)) && p.err) atomicExch(p.err, kErrPos);
   } else {
-    // units of all sequences, and where this CTA's range begins
+    // length of the flat list, and where this CTA's range begins
     const int per = (p.B + kThreads - 1) / kThreads;
     const int sb0 = min(tid * per, p.B), sb1 = min(sb0 + per, p.B);
     int mine = 0;
     for (int b = sb0; b < sb1; ++b) {
       const int n = p.lens[b];
       if (cta == 0 && (n < 0 || n > cap_of(p)) && p.err) atomicExch(p.err, kErrPos);
-      mine += units_of(clamp_len(p, b));
+      mine += weight_of(clamp_len(p, b));
     }
     int inc = mine;
 #pragma unroll
@@ -300,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     if (x >= before && x < before + mine) {
       int b = sb0, pre = before;
       for (; b < sb1; ++b) {
-        const int n = units_of(clamp_len(p, b));
+        const int n = weight_of(clamp_len(p, b));
         if (x < pre + n) break;
         pre += n;
       }
@@ -710,62 +719,74 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   if (bad_page && p.err) atomicExch(p.err, kErrPage);
 }
 
-// Joins the partials of each (sequence, head) that more than one CTA worked on:
-// block j does the one that began in CTA j's range and went on past its end,
-// in the order of the cache.  grid.y splits its rows.
+// Joins the partials of each (sequence, head tile) that more than one CTA worked
+// on: block j does the one that began in CTA j's range and went on past its
+// end.  A group of lanes covers one row (query head) with 16 bytes each; the
+// groups of a row take every `per_row`-th partial, with a running maximum of
+// their own, so that a partial's sum and its values are loaded together, and are
+// added up in a fixed order.  grid.y splits the rows.
 template <int HD, bool FP8>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   constexpr int LPR = HD / 4;                     // lanes (of float4) that cover a row
   constexpr int GR = kJoinThreads / LPR;          // groups of lanes
   constexpr float kUp = FP8 ? 7.f : 0.f;
   __shared__ float4 s_o[GR][LPR];
-  __shared__ float s_ml[GR];
+  __shared__ float2 s_ml[GR];
   griddep_sync();
   const int j = blockIdx.x;
   const int4 d = p.desc[j];
   if (d.x < 0) return;
-  const int b = d.x, h = d.y / p.mtiles, mt = d.y % p.mtiles, n = d.z - j + 1;
+  const int b = d.x, h = d.y / p.mtiles, mt = d.y - h * p.mtiles, n = d.z - j + 1;
   const int nrows = min(p.rows, p.group - mt * p.rows);
   const int row0 = h * p.group + mt * p.rows;
   const int li = threadIdx.x % LPR, gi = threadIdx.x / LPR;
-  // partial i of this segment: slot 2 j + 1, then slot 0 of the CTAs that follow
-  auto slot = [&](int i) { return i == 0 ? 2LL * j + 1 : 2LL * (j + i); };
-  for (int r = blockIdx.y; r < nrows; r += gridDim.y) {
-    float M = -INFINITY;
-    for (int i = threadIdx.x % 32; i < n; i += 32) M = fmaxf(M, p.part_ml[slot(i) * p.rows + r].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
+  const int rows = (nrows - blockIdx.y + gridDim.y - 1) / static_cast<int>(gridDim.y);  // of this block
+  if (rows <= 0) return;
+  const int per_row = max(1, GR / rows);
+  for (int i0 = 0; i0 < rows; i0 += GR / per_row) {
+    const int i = i0 + gi / per_row, sub = gi % per_row;
+    const bool on = i < rows && gi / per_row < GR / per_row;
+    const int r = blockIdx.y + i * gridDim.y;
+    float M = -INFINITY, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) {
 #pragma unroll 4
-    for (int i = gi; i < n; i += GR) {
-      const float2 ml = p.part_ml[slot(i) * p.rows + r];
-      const float4 x = reinterpret_cast<const float4*>(p.part_o + (slot(i) * p.rows + r) * HD)[li];
-      const float f = ex2_approx(ml.x - ref);
-      L += f * ml.y;
-      O.x += f * x.x;
-      O.y += f * x.y;
-      O.z += f * x.z;
-      O.w += f * x.w;
+      for (int k = sub; k < n; k += per_row) {
+        // partial k of this segment: slot 2 j + 1, then slot 0 of the CTAs that follow
+        const long long at = (k == 0 ? 2LL * j + 1 : 2LL * (j + k)) * p.rows + r;
+        const float2 ml = p.part_ml[at];
+        const float4 x = reinterpret_cast<const float4*>(p.part_o + at * HD)[li];
+        const float m = fmaxf(M, ml.x), ref = m == -INFINITY ? 0.f : m;
+        const float f = ex2_approx(M - ref), e = ex2_approx(ml.x - ref);
+        M = m;
+        L = f * L + e * ml.y;
+        O.x = f * O.x + e * x.x;
+        O.y = f * O.y + e * x.y;
+        O.z = f * O.z + e * x.z;
+        O.w = f * O.w + e * x.w;
+      }
     }
-    __syncthreads();
     s_o[gi][li] = O;
-    if (li == 0) s_ml[gi] = L;
+    if (li == 0) s_ml[gi] = make_float2(M, L);
     __syncthreads();
-    if (gi == 0) {
-      for (int i = 1; i < GR; ++i) {
-        const float4 x = s_o[i][li];
-        O.x += x.x;
-        O.y += x.y;
-        O.z += x.z;
-        O.w += x.w;
-        L += s_ml[i];
+    if (on && sub == 0) {
+      for (int k = 1; k < per_row; ++k) M = fmaxf(M, s_ml[gi + k].x);
+      const float ref = M == -INFINITY ? 0.f : M;
+      const float f = ex2_approx(s_ml[gi].x - ref);
+      L *= f;
+      O = make_float4(O.x * f, O.y * f, O.z * f, O.w * f);
+      for (int k = 1; k < per_row; ++k) {
+        const float e = ex2_approx(s_ml[gi + k].x - ref);
+        const float4 x = s_o[gi + k][li];
+        L += e * s_ml[gi + k].y;
+        O.x += e * x.x;
+        O.y += e * x.y;
+        O.z += e * x.z;
+        O.w += e * x.w;
       }
       const float vsc = (FP8 && p.v_scale) ? p.v_scale[h] : 1.f;
-      const float inv = L == 0.f ? 0.f : vsc / L;
+      const float inv = L == 0.f ? 0.f : vsc / L;  // (L is 0 only where every key was left out: O is 0 too)
       __nv_bfloat16* out = p.o + b * p.o_b + (row0 + r) * p.o_h + li * 4;
-      // (L is 0 only where every key was left out: o is then 0 as well)
       out[0] = __float2bfloat16_rn(O.x * inv);
       out[1] = __float2bfloat16_rn(O.y * inv);
       out[2] = __float2bfloat16_rn(O.z * inv);
@@ -773,6 +794,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
       if (li == 0 && p.lse)
         p.lse[b * p.lse_b + row0 + r] = L == 0.f ? -INFINITY : (M + log2f(L) - kUp) * kLn2;
     }
+    __syncthreads();
   }
 }
 
@@ -878,7 +900,7 @@ bool shape_ok(int B, int Hq, int Hk, int d, int page, int max_blocks) {
   const long long cap = static_cast<long long>(max_blocks) * page;
   // unit counts of a call are 32-bit
   return cap <= INT32_MAX - kUnit &&
-         static_cast<double>(B) * Hk * mtiles * static_cast<double>((cap + kUnit - 1) / kUnit) <= INT32_MAX;
+         static_cast<double>(B) * Hk * mtiles * static_cast<double>((cap + kUnit - 1) / kUnit + kOver) <= INT32_MAX;
 }
 
 }  // namespace pa
