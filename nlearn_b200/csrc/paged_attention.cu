@@ -12,7 +12,7 @@
 // Bound: HBM.  Every cached element is used once per query head of its group,
 // 2 FLOP per element and head, so the kernel is built to keep loads in flight
 // and to spend few instructions on a byte:
-//   * a warp works on tiles of 16 keys, gathered row by row with 16-byte
+//   * a warp works on tiles of 16 or 32 keys (8 KB, 4 KB for the shortest rows), gathered row by row with 16-byte
 //     cp.async (any page size, any strides) into a ring of tiles of its own: no
 //     block barrier between tiles, and the ring is filled across the ends of
 //     sequences, so a new sequence finds its first tiles on the way;
@@ -32,8 +32,8 @@
 // below 2^15, is rounded to f16's 11 bits, an eighth of the bf16 output's step.
 //
 // Two ways of dividing the work, both with lengths read on the device only:
-//   * flat: the work of all sequences and heads is one list of units of 64 keys
-//     (four warps, one tile each), cut into equal ranges, one per CTA, so any mix of
+//   * flat: the work of all sequences and heads is one list of units of 64 or 128
+//     keys (four warps, one tile each), cut into equal ranges, one per CTA, so any mix of
 //     lengths balances.  The cut ends leave partials (max, sum, o) that
 //     join_kernel merges in the order of the cache;
 //   * clustered, for short caches: a cluster of up to 8 CTAs per (sequence,
@@ -54,8 +54,7 @@ namespace pa {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = 16;                 // keys a warp takes at a time
-constexpr int kUnit = kTile * kWarps;     // keys of one unit of work
+constexpr int kGroup = 16;                // keys of one product (its rows); a page lookup of whole pages
 constexpr int kHeads = 8;                 // query heads of one product (its columns)
 constexpr int kMaxTiles = 2;              // products of 8 heads a CTA keeps: groups of up to 16 read the keys once
 constexpr int kMaxCluster = 8;
@@ -64,6 +63,7 @@ constexpr int kJoinThreads = 256;
 // (a fit of CTA times on ragged batches: 1.38 us a unit and 1.60 us a run, bf16,
 // d 128; 1.79 and 2.48 us, e4m3), so it is counted as one.
 constexpr int kOver = 1;
+constexpr float kNoRef = -3.402823466e38f;  // before the first score: any finite one is above it
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;             // log2 of how far p may grow before the maximum moves
 constexpr uint32_t kNoRow = 0xffffffffu;
@@ -162,39 +162,47 @@ __device__ __forceinline__ int clamp_len(const Params& p, int b) {
   const int n = p.lens[b], cap = cap_of(p);
   return n < 0 ? 0 : (n > cap ? cap : n);
 }
-__device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
+template <int UNIT>
+__device__ __forceinline__ int units_of(int len) {
+  return (len + UNIT - 1) / UNIT;
+}
 // Length of one (sequence, head tile) in the flat list: its units, after kOver for its start and its join.
-__device__ __forceinline__ int weight_of(int len) { return len > 0 ? units_of(len) + kOver : 0; }
+template <int UNIT>
+__device__ __forceinline__ int weight_of(int len) {
+  return len > 0 ? units_of<UNIT>(len) + kOver : 0;
+}
 
 // First unit of CTA i of n over U units.
 __device__ __forceinline__ int cut(int i, int U, int n) {
   return static_cast<int>(static_cast<long long>(i) * U / n);
 }
 
-// A run: consecutive units [c0, c1) of one (sequence, tile of query heads).
+// A run: consecutive units [c0, c1) of one sequence and one segment of its
+// heads (a tile of query heads, or four of them, one per warp).
 struct Run {
-  int b, hm, len, nu, c0, c1;
+  int b, seg, len, nu, c0, c1;
 };
 // Walks a CTA's range of the flat list, run by run (a run is not empty).
+template <int UNIT>
 struct Walk {
+  int segs;      // segments of a sequence
   int u, u1;     // next unit, end of the range
   int b, base;   // sequence of unit u (or an earlier one), units before it
   __device__ __forceinline__ bool next(const Params& p, Run& r) {
-    const int heads = p.Hk * p.mtiles;
     while (u < u1) {
       int len, w;
       for (;; ++b) {
         len = clamp_len(p, b);
-        w = weight_of(len);
-        if (u - base < w * heads) break;
-        base += w * heads;
+        w = weight_of<UNIT>(len);
+        if (u - base < w * segs) break;
+        base += w * segs;
       }
       const int local = u - base;
       r.b = b;
       r.len = len;
       r.nu = w - kOver;
-      r.hm = local / w;
-      const int c = local - r.hm * w, n = min(w - c, u1 - u);
+      r.seg = local / w;
+      const int c = local - r.seg * w, n = min(w - c, u1 - u);
       r.c0 = max(0, c - kOver);
       r.c1 = max(0, c + n - kOver);
       u += n;
@@ -207,14 +215,17 @@ struct Walk {
 template <int HD, bool FP8>
 struct Shape {
   static constexpr int RB = HD * (FP8 ? 1 : 2);  // bytes of a key row
+  static constexpr int NG = RB >= 128 ? 1 : 2;   // groups of 16 keys a warp takes at a time
+  static constexpr int TILE = kGroup * NG;       // keys of a tile
   static constexpr int CPR = RB / 16;            // 16-byte chunks of a row
   static constexpr int RPI = 32 / CPR;           // rows one copy instruction of a warp covers
-  static constexpr int NI = kTile / RPI;         // copy instructions of a tile
-  static constexpr int TB = kTile * RB;          // bytes of a tile
+  static constexpr int NI = kGroup / RPI;        // copy instructions of a group
+  static constexpr int GB = kGroup * RB;         // bytes of a group
+  static constexpr int TB = NG * GB;             // bytes of a tile
   static constexpr int SB = 2 * TB;              // K and V tiles of a stage
   static constexpr int KS = HD / 16;             // k steps of k q^T; row tiles of v^T p^T
-  static constexpr int STAGES = SB <= 2048 ? 4 : 3;
-  static constexpr int MT = SB > 4096 ? 4 : 2;   // row tiles joined at a time (shared memory)
+  static constexpr int STAGES = 3;
+  static constexpr int MT = RB == 256 ? 4 : 2;   // row tiles joined at a time (shared memory)
   static constexpr int RING = kWarps * STAGES * SB;
   static constexpr int SMEM = RING + kWarps * MT * 4 * 32 * 4;
   // Byte offset of chunk c of row r.  Chunks are permuted inside 128 bytes so
@@ -228,17 +239,22 @@ struct Shape {
 // Resident CTAs an SM is meant to hold (shared memory allows them; caps registers).
 template <int HD, bool FP8, int NH>
 constexpr int min_ctas() {
-  if (HD == 128) return FP8 ? (NH == 1 ? 4 : 3) : 2;
-  return FP8 ? (NH == 1 ? 5 : 4) : 4;
+  return Shape<HD, FP8>::SMEM > 64 * 1024 ? 2 : (NH == 2 ? 3 : 4);
 }
 
-template <int HD, bool FP8, int NH, bool CLUSTER>
+// MODE: how the four warps and the CTAs share the work (kClustered: see the top).
+enum : int { kByKeys = 0, kByHeads = 1, kClustered = 2 };
+
+template <int HD, bool FP8, int NH, int MODE>
 __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kernel(const Params p) {
   using S = Shape<HD, FP8>;
-  constexpr float kUp = FP8 ? 7.f : 0.f;  // p is kept as 2^(y - m + kUp): below 2^15 with the slack
+  constexpr bool CLUSTER = MODE == kClustered, HEADS = MODE == kByHeads;
+  constexpr int UNIT = HEADS ? S::TILE : S::TILE * kWarps;  // keys of one unit of work
+  // p = 2^(y - ref) with ref the running maximum less kUp: below 2^15, in f16's range, with the slack
+  constexpr float kUp = FP8 ? 7.f : 0.f;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kWarps][kHeads * NH], s_l[kWarps][kHeads * NH];
-  __shared__ uint32_t s_valid[kWarps][S::STAGES];
+  __shared__ uint32_t s_valid[kWarps][S::STAGES];  // keys of a tile that take part
   __shared__ int s_scan[kWarps];
   __shared__ int s_start[2];
   __shared__ float2 s_ml[kHeads * NH];  // clustered: this CTA's (max, sum)
@@ -246,21 +262,21 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   const int g = lane >> 2, t4 = lane & 3;
   griddep_sync();
 
-  const int heads = p.Hk * p.mtiles;
+  const int segs = p.Hk * p.mtiles / (HEADS ? kWarps : 1);  // of a sequence
   int U = 0, ctas = 0, rank = 0, csize = 1;
   const int cta = blockIdx.x;
-  Walk walk;       // of the copies
-  Run first = {};  // of the products
-  Walk cwalk;
+  Walk<UNIT> walk;  // of the copies
+  Run first = {};      // of the products
+  Walk<UNIT> cwalk;
   bool live;
   if constexpr (CLUSTER) {
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
     rank = cluster_ctarank();
     const int seg = cta / csize;
-    first.b = seg / heads;
-    first.hm = seg - first.b * heads;
+    first.b = seg / segs;
+    first.seg = seg - first.b * segs;
     first.len = clamp_len(p, first.b);
-    first.nu = units_of(first.len);
+    first.nu = units_of<UNIT>(first.len);
     first.c0 = rank * first.nu / csize;
     first.c1 = (rank + 1) * first.nu / csize;
     live = first.c1 > first.c0;
@@ -275,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     for (int b = sb0; b < sb1; ++b) {
       const int n = p.lens[b];
       if (cta == 0 && (n < 0 || n > cap_of(p)) && p.err) atomicExch(p.err, kErrPos);
-      mine += weight_of(clamp_len(p, b));
+      mine += weight_of<UNIT>(clamp_len(p, b));
     }
     int inc = mine;
 #pragma unroll
@@ -291,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
       if (w < warp) before += s_scan[w];
       total += s_scan[w];
     }
-    U = total * heads;
+    U = total * segs;
     ctas = min(U, static_cast<int>(gridDim.x));
     // sequences with no key: zeros (the sum over nothing), lse = -inf
     for (int b = cta; b < p.B; b += gridDim.x) {
@@ -305,11 +321,11 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
       if (tid == 0) p.desc[cta] = make_int4(-1, 0, 0, 0);
       return;
     }
-    const int u0 = cut(cta, U, ctas), x = u0 / heads;
+    const int u0 = cut(cta, U, ctas), x = u0 / segs;
     if (x >= before && x < before + mine) {
       int b = sb0, pre = before;
       for (; b < sb1; ++b) {
-        const int n = weight_of(clamp_len(p, b));
+        const int n = weight_of<UNIT>(clamp_len(p, b));
         if (x < pre + n) break;
         pre += n;
       }
@@ -320,68 +336,95 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     walk.u = u0;
     walk.u1 = cut(cta + 1, U, ctas);
     walk.b = s_start[0];
-    walk.base = s_start[1] * heads;
+    walk.base = s_start[1] * segs;
+    walk.segs = segs;
     live = walk.next(p, first);
     cwalk = walk;
   }
+
+  // tile of query heads (kv head * mtiles + its part of the group) of a segment, for this warp
+  auto tile_of = [&](const Run& r) { return HEADS ? r.seg * kWarps + warp : r.seg; };
+  const int warp_key = HEADS ? 0 : warp * S::TILE;  // where in a unit this warp's tile is
 
   // ---- copies: the ring is filled STAGES - 1 tiles ahead, run after run
   uint8_t* ring = smem + warp * (S::STAGES * S::SB);
   const uint32_t ring_s = smem_u32(ring);
   const int my_row = lane / S::CPR, my_chunk = lane % S::CPR;
-  const bool whole = p.page % kTile == 0;  // a tile lies in one page
+  const uint32_t my_dst = S::at(my_row, my_chunk);
+  const bool whole = p.page % kGroup == 0;  // a group of 16 keys lies in one page
+  const size_t v_minus_k = static_cast<size_t>(p.v - p.k);
+  const size_t step = static_cast<size_t>(p.tok16) * (16 * S::RPI);  // bytes between a lane's rows
   bool bad_page = false;
   bool more = live;         // tiles left to copy
   Run in = first;           // run being copied
   int unit = first.c0;      // its next unit
   int in_stage = 0;
-  int pg = 0;               // page of the next tile (of key lane % 16 of it, if tiles are not whole)
+  int pg[S::NG];            // page of the next tile's groups (of key lane % 16, if groups are not whole)
   auto block_of = [&](int pos) { return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page; };
   auto look_up = [&]() {
-    const int pos = unit * kUnit + warp * kTile + (whole ? 0 : (lane & 15));
-    pg = (more && pos < in.len) ? __ldg(p.table + in.b * p.table_ld + block_of(pos)) : 0;
+    const int pos = unit * UNIT + warp_key + (whole ? 0 : (lane & 15));
+    const int* row = p.table + in.b * p.table_ld;
+#pragma unroll
+    for (int j = 0; j < S::NG; ++j)
+      pg[j] = (more && pos + j * kGroup < in.len) ? __ldg(row + block_of(pos + j * kGroup)) : 0;
+  };
+  // key of this lane in the shared tile: i-th row of a group, relative to my_dst (my_row < RPI)
+  auto row_dst = [&](int i) -> uint32_t {
+    // at(my_row + i RPI, c): the row's part of the permutation splits into my_row's and i's bits
+    if constexpr (S::RB >= 128) return i * S::RPI * S::RB + (my_dst ^ (((i * S::RPI) & 7) << 4));
+    return i * S::RPI * S::RB + my_dst;  // 64-byte rows: 8 rows an instruction, same permutation
   };
   auto copy_tile = [&]() {
     if (more) {
-      const int h = in.hm / p.mtiles;
-      const int k0 = unit * kUnit + warp * kTile;
+      const int hm = tile_of(in), h = hm / p.mtiles;
+      const int k0 = unit * UNIT + warp_key;
       const int left = in.len - k0;  // keys of the tile that exist
-      const bool in_cache = pg >= 0 && pg < p.n_pages;
-      const size_t head_off = h * p.head_bytes + my_chunk * 16;
-      const uint8_t* kb = p.k + head_off;
-      const uint8_t* vb = p.v + head_off;
-      const uint32_t dst = ring_s + in_stage * S::SB;
-      uint32_t mask, off;
-      if (whole) {
-        mask = left >= kTile ? 0xffffu : (left > 0 ? (1u << left) - 1 : 0u);
-        if (mask && !in_cache) {
-          bad_page = true;
-          mask = 0;
+      const uint8_t* kb = p.k + (h * p.head_bytes + my_chunk * 16);
+      uint32_t mask = 0;
+#pragma unroll
+      for (int j = 0; j < S::NG; ++j) {
+        const int pos0 = k0 + j * kGroup;
+        const uint32_t dst = ring_s + in_stage * S::SB + j * S::GB;
+        const int lj = left - j * kGroup;
+        const bool in_cache = pg[j] >= 0 && pg[j] < p.n_pages;
+        const bool append = p.k_new != nullptr && lj > 0 && lj <= kGroup;  // the last key is here
+        if (whole && in_cache && lj >= kGroup && !append) {
+          // sixteen keys of one page: rows at equal steps
+          mask |= 0xffffu << (16 * j);
+          const uint32_t off =
+              static_cast<uint32_t>(pg[j]) * p.page16 +
+              static_cast<uint32_t>(pos0 - block_of(pos0) * p.page + my_row) * p.tok16;
+          const uint8_t* src = kb + static_cast<size_t>(off) * 16;
+#pragma unroll
+          for (int i = 0; i < S::NI; ++i) {
+            cp_async16(dst + row_dst(i), src, 16u);
+            cp_async16(dst + S::TB + row_dst(i), src + v_minus_k, 16u);
+            src += step;
+          }
+          continue;
         }
-        off = static_cast<uint32_t>(pg) * p.page16 + static_cast<uint32_t>(k0 - block_of(k0) * p.page) * p.tok16;
-      } else {
-        const int pos = k0 + (lane & 15);
+        // row by row: the end of a sequence, a group over several pages, a bad page, the new token
+        const int pos = pos0 + (whole ? 0 : (lane & 15));
         const bool here = pos < in.len;
         if (here && !in_cache) bad_page = true;
-        mask = __ballot_sync(0xffffffffu, here && in_cache) & 0xffffu;
-        off = static_cast<uint32_t>(pg) * p.page16 + static_cast<uint32_t>(pos - block_of(pos) * p.page) * p.tok16;
-      }
-      if (lane == 0) s_valid[warp][in_stage] = mask;
-      // row of the new token, if it is in this tile (and has a page)
-      int arow = -1;
-      if (p.k_new != nullptr && left > 0 && left <= kTile && (mask >> (left - 1) & 1) && p.lens[in.b] <= cap_of(p))
-        arow = left - 1;
+        const uint32_t off = static_cast<uint32_t>(pg[j]) * p.page16 +
+                             static_cast<uint32_t>(pos - block_of(pos) * p.page) * p.tok16;
+        uint32_t ok;
+        if (whole) ok = !in_cache || lj <= 0 ? 0u : (lj >= kGroup ? 0xffffu : (1u << lj) - 1);
+        else ok = __ballot_sync(0xffffffffu, here && in_cache) & 0xffffu;
+        mask |= ok << (16 * j);
+        const int arow = append && (ok >> (lj - 1) & 1) && p.lens[in.b] <= cap_of(p) ? lj - 1 : -1;
 #pragma unroll
-      for (int i = 0; i < S::NI; ++i) {
-        const int r = i * S::RPI + my_row;
-        const uint32_t o = whole ? off + r * p.tok16 : __shfl_sync(0xffffffffu, off, r);
-        const bool ok = mask >> r & 1;
-        const size_t src = ok ? static_cast<size_t>(o) * 16 : 0;
-        const uint32_t d = dst + S::at(r, my_chunk);
-        if (r != arow) {
-          cp_async16(d, kb + src, ok ? 16u : 0u);
-          cp_async16(d + S::TB, vb + src, ok ? 16u : 0u);
-        } else {
+        for (int i = 0; i < S::NI; ++i) {
+          const int r = i * S::RPI + my_row;
+          const uint32_t o = whole ? off + r * p.tok16 : __shfl_sync(0xffffffffu, off, r);
+          const bool use = ok >> r & 1;
+          const uint8_t* src = kb + (use ? static_cast<size_t>(o) * 16 : 0);
+          if (r != arow) {
+            cp_async16(dst + row_dst(i), src, use ? 16u : 0u);  // rows that do not exist become zeros
+            cp_async16(dst + S::TB + row_dst(i), src + v_minus_k, use ? 16u : 0u);
+            continue;
+          }
           // the new token: from k_new, v_new into the tile, and into its slot
           const long long nb = in.b * p.n_b + h * p.n_h + my_chunk * (FP8 ? 16 : 8);
 #pragma unroll
@@ -398,12 +441,13 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
               for (int e = 0; e < 16; ++e)
                 ob[e] = __nv_cvt_float_to_fp8(__bfloat162float(x[e]) / sc, __NV_SATFINITE, __NV_E4M3);
             }
-            *reinterpret_cast<uint4*>(ring + in_stage * S::SB + which * S::TB + S::at(r, my_chunk)) = val;
-            if (in.hm % p.mtiles == 0)
-              *reinterpret_cast<uint4*>(const_cast<uint8_t*>(which ? vb : kb) + src) = val;
+            *reinterpret_cast<uint4*>(ring + in_stage * S::SB + which * S::TB + j * S::GB + row_dst(i)) = val;
+            if (hm == h * p.mtiles)
+              *reinterpret_cast<uint4*>(const_cast<uint8_t*>(src) + (which ? v_minus_k : 0)) = val;
           }
         }
       }
+      if (lane == 0) s_valid[warp][in_stage] = mask;
       if (++unit == in.c1) {
         if constexpr (CLUSTER) more = false;
         else more = walk.next(p, in);
@@ -419,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   uint32_t qf[NH][S::KS][2];
   float sl[NH][2];  // factor of the scores of columns 2 t4, 2 t4 + 1
   auto load_q = [&](const Run& r) {
-    const int h = r.hm / p.mtiles, mt = r.hm - h * p.mtiles;
+    const int hm = tile_of(r), h = hm / p.mtiles, mt = hm - h * p.mtiles;
     const int have = min(p.rows, p.group - mt * p.rows);
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
@@ -463,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             qf[n][ks][e] = pack_f16x2(bf16_lo(qf[n][ks][e]) * up, bf16_hi(qf[n][ks][e]) * up);
-        const float ksc = p.k_scale ? p.k_scale[r.hm / p.mtiles] : 1.f;
+        const float ksc = p.k_scale ? p.k_scale[tile_of(r) / p.mtiles] : 1.f;
         const float down = p.scale_log2 * ksc / up;
         sl[n][0] = __shfl_sync(0xffffffffu, down, 8 * t4);      // column 2 t4 is lane 4 (2 t4)'s
         sl[n][1] = __shfl_sync(0xffffffffu, down, 8 * t4 + 4);
@@ -482,10 +526,11 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   while (live || CLUSTER) {
     if (live) scale_q(r);
     float acc[NH][S::KS][4];
-    float m[NH][2], l[NH][2];  // columns 2 t4, 2 t4 + 1: maximum (base 2), this lane's share of the sum
+    // columns 2 t4, 2 t4 + 1: reference of the exponents (base 2; p = 2^(y - ref)), this lane's share of the sum
+    float ref[NH][2], l[NH][2];
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
-      m[n][0] = m[n][1] = -INFINITY;
+      ref[n][0] = ref[n][1] = kNoRef;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < S::KS; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
@@ -500,52 +545,70 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
       stage = stage + 1 == S::STAGES ? 0 : stage + 1;
       if (valid == 0) continue;
 
-      // ---- scores: rows (keys) g, g + 8; columns (heads) 2 t4, 2 t4 + 1
-      float y[NH][4];
+      // ---- scores: rows (keys) g, g + 8 of a group; columns (heads) 2 t4, 2 t4 + 1
+      float y[S::NG][NH][4];
 #pragma unroll
-      for (int n = 0; n < NH; ++n) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.f;
-      if constexpr (!FP8) {
+      for (int j = 0; j < S::NG; ++j) {
 #pragma unroll
-        for (int ks = 0; ks < S::KS; ++ks) {
-          uint32_t a[4];
-          ldsm4(a, kt + S::at(lane & 15, 2 * ks + (lane >> 4)));
+        for (int n = 0; n < NH; ++n) y[j][n][0] = y[j][n][1] = y[j][n][2] = y[j][n][3] = 0.f;
+        if constexpr (!FP8) {
 #pragma unroll
-          for (int n = 0; n < NH; ++n) mma16816<false>(y[n], a, qf[n][ks][0], qf[n][ks][1]);
-        }
-      } else {
+          for (int ks = 0; ks < S::KS; ++ks) {
+            uint32_t a[4];
+            ldsm4(a, kt + j * S::GB + S::at(lane & 15, 2 * ks + (lane >> 4)));
 #pragma unroll
-        for (int kk = 0; kk < S::KS / 2; ++kk) {  // 32 dims
-          uint32_t x[4];
-          ldsm4(x, kt + S::at(lane & 15, 2 * kk + (lane >> 4)));
+            for (int n = 0; n < NH; ++n) mma16816<false>(y[j][n], a, qf[n][ks][0], qf[n][ks][1]);
+          }
+        } else {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t a[4] = {e4m3x2_f16x2(x[2 * e]), e4m3x2_f16x2(x[2 * e + 1]), e4m3x2_f16x2(x[2 * e] >> 16),
-                                   e4m3x2_f16x2(x[2 * e + 1] >> 16)};
+          for (int kk = 0; kk < S::KS / 2; ++kk) {  // 32 dims
+            uint32_t x[4];
+            ldsm4(x, kt + j * S::GB + S::at(lane & 15, 2 * kk + (lane >> 4)));
 #pragma unroll
-            for (int n = 0; n < NH; ++n) mma16816<true>(y[n], a, qf[n][2 * kk + e][0], qf[n][2 * kk + e][1]);
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t a[4] = {e4m3x2_f16x2(x[2 * e]), e4m3x2_f16x2(x[2 * e + 1]),
+                                     e4m3x2_f16x2(x[2 * e] >> 16), e4m3x2_f16x2(x[2 * e + 1] >> 16)};
+#pragma unroll
+              for (int n = 0; n < NH; ++n) mma16816<true>(y[j][n], a, qf[n][2 * kk + e][0], qf[n][2 * kk + e][1]);
+            }
           }
         }
       }
       bool grow = false;
 #pragma unroll
-      for (int n = 0; n < NH; ++n)
+      for (int j = 0; j < S::NG; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[n][e] *= sl[n][e & 1];
-          if (valid != 0xffffu && !(valid >> (g + 8 * (e >> 1)) & 1)) y[n][e] = -INFINITY;
-          grow = grow || y[n][e] > m[n][e & 1] + kSlack;
-        }
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[j][n][e] *= sl[n][e & 1];
+      if (valid != (S::NG == 2 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+        for (int j = 0; j < S::NG; ++j)
+#pragma unroll
+          for (int n = 0; n < NH; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(valid >> (16 * j + g + 8 * (e >> 1)) & 1)) y[j][n][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < S::NG; ++j)
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) grow = grow || y[j][n][e] > ref[n][e & 1] + (kSlack + kUp);
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(y[n][e], y[n][2 + e]);
+            float x = kNoRef;
+#pragma unroll
+            for (int j = 0; j < S::NG; ++j) x = fmaxf(x, fmaxf(y[j][n][e], y[j][n][2 + e]));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-            x = fmaxf(x, m[n][e]);
-            const float f = x == -INFINITY ? 1.f : ex2_approx(m[n][e] - x);
-            m[n][e] = x;
+            x = fmaxf(x - kUp, ref[n][e]);
+            const float f = ex2_approx(ref[n][e] - x);
+            ref[n][e] = x;
             l[n][e] *= f;
 #pragma unroll
             for (int i = 0; i < S::KS; ++i) {
@@ -554,52 +617,55 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
             }
           }
       }
-      uint32_t ph[NH][2], pl[NH][2];  // p^T as the second product's columns; its low part
 #pragma unroll
-      for (int n = 0; n < NH; ++n) {
+      for (int j = 0; j < S::NG; ++j) {
+        uint32_t ph[NH][2], pl[NH][2];  // p^T as the second product's columns; its low part
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float ref = (m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1]) - kUp;
-          y[n][e] = ex2_approx(y[n][e] - ref);
-          l[n][e & 1] += y[n][e];
-        }
+        for (int n = 0; n < NH; ++n) {
+          float pr[4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if constexpr (FP8) {
-            ph[n][e] = transpose8(pack_f16x2(y[n][2 * e], y[n][2 * e + 1]));
-          } else {
-            const uint32_t hi = pack_bf16x2(y[n][2 * e], y[n][2 * e + 1]);
-            ph[n][e] = transpose8(hi);
-            pl[n][e] = transpose8(pack_bf16x2(y[n][2 * e] - bf16_lo(hi), y[n][2 * e + 1] - bf16_hi(hi)));
+          for (int e = 0; e < 4; ++e) {
+            pr[e] = ex2_approx(y[j][n][e] - ref[n][e & 1]);
+            l[n][e & 1] += pr[e];
           }
-        }
-      }
-      // ---- o^T += v^T p^T
-      if constexpr (!FP8) {
-#pragma unroll
-        for (int i = 0; i < S::KS; ++i) {
-          uint32_t a[4];
-          ldsm4_t(a, vt + S::at((lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
-#pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            mma16816<false>(acc[n][i], a, ph[n][0], ph[n][1]);
-            mma16816<false>(acc[n][i], a, pl[n][0], pl[n][1]);
-          }
-        }
-      } else {
-        // a transposed 8x8 of 16-bit units holds, per key, two neighbouring dims:
-        // rows g of a tile are the even dims of 16, rows g + 8 the odd ones
-#pragma unroll
-        for (int ii = 0; ii < S::KS / 2; ++ii) {
-          uint32_t x[4];
-          ldsm4_t(x, vt + S::at(lane & 15, 2 * ii + (lane >> 4)));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t lo = __byte_perm(x[2 * e], 0, 0x3120), hi = __byte_perm(x[2 * e + 1], 0, 0x3120);
-            const uint32_t a[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2(lo >> 16), e4m3x2_f16x2(hi),
-                                   e4m3x2_f16x2(hi >> 16)};
+            if constexpr (FP8) {
+              ph[n][e] = transpose8(pack_f16x2(pr[2 * e], pr[2 * e + 1]));
+            } else {
+              const uint32_t hi = pack_bf16x2(pr[2 * e], pr[2 * e + 1]);
+              ph[n][e] = transpose8(hi);
+              pl[n][e] = transpose8(pack_bf16x2(pr[2 * e] - bf16_lo(hi), pr[2 * e + 1] - bf16_hi(hi)));
+            }
+          }
+        }
+        // ---- o^T += v^T p^T
+        if constexpr (!FP8) {
 #pragma unroll
-            for (int n = 0; n < NH; ++n) mma16816<true>(acc[n][2 * ii + e], a, ph[n][0], ph[n][1]);
+          for (int i = 0; i < S::KS; ++i) {
+            uint32_t a[4];
+            ldsm4_t(a, vt + j * S::GB + S::at((lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+              mma16816<false>(acc[n][i], a, ph[n][0], ph[n][1]);
+              mma16816<false>(acc[n][i], a, pl[n][0], pl[n][1]);
+            }
+          }
+        } else {
+          // a transposed 8x8 of 16-bit units holds, per key, two neighbouring dims:
+          // rows g of a tile are the even dims of 16, rows g + 8 the odd ones
+#pragma unroll
+          for (int ii = 0; ii < S::KS / 2; ++ii) {
+            uint32_t x[4];
+            ldsm4_t(x, vt + j * S::GB + S::at(lane & 15, 2 * ii + (lane >> 4)));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t lo = __byte_perm(x[2 * e], 0, 0x3120), hi = __byte_perm(x[2 * e + 1], 0, 0x3120);
+              const uint32_t a[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2(lo >> 16), e4m3x2_f16x2(hi),
+                                     e4m3x2_f16x2(hi >> 16)};
+#pragma unroll
+              for (int n = 0; n < NH; ++n) mma16816<true>(acc[n][2 * ii + e], a, ph[n][0], ph[n][1]);
+            }
           }
         }
       }
@@ -612,104 +678,138 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
       again = cwalk.next(p, nr);
       if (again) load_q(nr);
     }
-    const int h = r.hm / p.mtiles, mt = r.hm - h * p.mtiles;
+    const int hm = tile_of(r), h = hm / p.mtiles, mt = hm - h * p.mtiles;
     const int row0 = h * p.group + mt * p.rows, nrows = min(p.rows, p.group - mt * p.rows);
     const bool begins = r.c0 == 0, ends = r.c1 == r.nu;
     const int slot = 2 * cta + (begins ? 1 : 0);  // a run that began in an earlier CTA goes to slot 0
     if constexpr (!CLUSTER)
       if (begins && !ends) {
         const int end = cut(cta + 1, U, ctas) - r.c1 + r.nu;  // unit after this segment's last
-        my_desc = make_int4(r.b, r.hm, static_cast<int>((static_cast<long long>(end) * ctas - 1) / U), 0);
+        my_desc = make_int4(r.b, r.seg, static_cast<int>((static_cast<long long>(end) * ctas - 1) / U), 0);
       }
     const float vsc = (FP8 && p.v_scale) ? p.v_scale[h] : 1.f;
 #pragma unroll
     for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
-        if (g == 0) {
-          s_m[warp][n * kHeads + 2 * t4 + e] = m[n][e];
-          s_l[warp][n * kHeads + 2 * t4 + e] = l[n][e];
-        }
-      }
-    float* scratch = reinterpret_cast<float*>(smem + S::RING);
-    float* part = reinterpret_cast<float*>(smem);  // clustered: [rows][HD] over the ring, which is idle by then
-    if constexpr (CLUSTER) {
-      cp_wait<0>();
-      __syncthreads();
-    }
+    if constexpr (HEADS) {
+      // ---- this warp's head is whole in its registers
 #pragma unroll
-    for (int n = 0; n < NH; ++n) {
-      // warp w sums element w of every accumulator: column 2 t4 + (w & 1), row g or g + 8
-      const int col = n * kHeads + 2 * t4 + (warp & 1);
-      float f[kWarps], M = -INFINITY, L = 0.f;
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int i0 = 0; i0 < S::KS; i0 += S::MT) {
+        for (int e = 0; e < 2; ++e) {
+          const int col = n * kHeads + 2 * t4 + e;
+          if (col >= nrows) continue;
+          const float L = l[n][e];
+          if (begins && ends) {
+            const float inv = L == 0.f ? 0.f : vsc / L;  // (L is 0 only where every key was left out: o is 0 too)
+            __nv_bfloat16* out = p.o + r.b * p.o_b + (row0 + col) * p.o_h;
 #pragma unroll
-        for (int i = 0; i < S::MT; ++i)
+            for (int i = 0; i < S::KS; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) scratch[((warp * S::MT + i) * 4 + e) * 32 + lane] = acc[n][i0 + i][e];
-        __syncthreads();
-        if (i0 == 0) {
+              for (int f = 0; f < 2; ++f)
+                out[i * 16 + (FP8 ? 2 * g + f : g + 8 * f)] = __float2bfloat16_rn(acc[n][i][2 * f + e] * inv);
+            if (g == 0 && p.lse)
+              p.lse[r.b * p.lse_b + row0 + col] = L == 0.f ? -INFINITY : (ref[n][e] + log2f(L)) * kLn2;
+          } else {
+            const long long at = (static_cast<long long>(slot) * kWarps + warp) * p.rows + col;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][col]);
-          const float ref = M == -INFINITY ? 0.f : M;
+            for (int i = 0; i < S::KS; ++i)
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            f[w] = ex2_approx(s_m[w][col] - ref);
-            L += f[w] * s_l[w][col];
+              for (int f = 0; f < 2; ++f)
+                p.part_o[at * HD + i * 16 + (FP8 ? 2 * g + f : g + 8 * f)] = acc[n][i][2 * f + e];
+            if (g == 0) p.part_ml[at] = make_float2(ref[n][e], L);
           }
         }
-        if (col < nrows) {
+    } else {
 #pragma unroll
-          for (int i = 0; i < S::MT; ++i) {
-            float O = 0.f;
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) O += f[w] * scratch[((w * S::MT + i) * 4 + warp) * 32 + lane];
-            const int d = (i0 + i) * 16 + (FP8 ? 2 * g + (warp >> 1) : g + 8 * (warp >> 1));
-            if constexpr (CLUSTER) {
-              part[col * HD + d] = O;
-              if (d == 0) s_ml[col] = make_float2(M, L);
-            } else if (begins && ends) {
-              p.o[r.b * p.o_b + (row0 + col) * p.o_h + d] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * vsc);
-              if (d == 0 && p.lse)
-                p.lse[r.b * p.lse_b + row0 + col] = L == 0.f ? -INFINITY : (M + log2f(L) - kUp) * kLn2;
-            } else {
-              p.part_o[(static_cast<long long>(slot) * p.rows + col) * HD + d] = O;
-              if (d == 0) p.part_ml[static_cast<long long>(slot) * p.rows + col] = make_float2(M, L);
+        for (int e = 0; e < 2; ++e)
+          if (g == 0) {
+            s_m[warp][n * kHeads + 2 * t4 + e] = ref[n][e];
+            s_l[warp][n * kHeads + 2 * t4 + e] = l[n][e];
+          }
+      float* scratch = reinterpret_cast<float*>(smem + S::RING);
+      float* part = reinterpret_cast<float*>(smem);  // clustered: [rows][HD] over the ring, which is idle by then
+      if constexpr (CLUSTER) {
+        cp_wait<0>();
+        __syncthreads();
+      }
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        // warp w sums element w of every accumulator: column 2 t4 + (w & 1), row g or g + 8
+        const int col = n * kHeads + 2 * t4 + (warp & 1);
+        float f[kWarps], M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int i0 = 0; i0 < S::KS; i0 += S::MT) {
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) scratch[((warp * S::MT + i) * 4 + e) * 32 + lane] = acc[n][i0 + i][e];
+          __syncthreads();
+          if (i0 == 0) {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][col]);
+            const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              f[w] = ex2_approx(s_m[w][col] - ref);
+              L += f[w] * s_l[w][col];
             }
           }
-        }
-        __syncthreads();  // scratch and s_m are written again
-      }
-    }
-    if constexpr (CLUSTER) {
-      // ---- every CTA of the cluster joins its share of the elements
-      cluster_sync();
-      for (int i = rank * kThreads + tid; i < nrows * HD; i += csize * kThreads) {
-        const int col = i / HD, d = i - col * HD;
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        float cm[kMaxCluster];
+          if (col < nrows) {
 #pragma unroll
-        for (int k = 0; k < kMaxCluster; ++k) {
-          cm[k] = k < csize ? ld_cluster(mapa_shared(smem_u32(&s_ml[col]), k)) : -INFINITY;
-          M = fmaxf(M, cm[k]);
-        }
-        const float ref = M == -INFINITY ? 0.f : M;
+            for (int i = 0; i < S::MT; ++i) {
+              float O = 0.f;
 #pragma unroll
-        for (int k = 0; k < kMaxCluster; ++k)
-          if (k < csize) {
-            const float f = ex2_approx(cm[k] - ref);
-            L += f * ld_cluster(mapa_shared(smem_u32(&s_ml[col].y), k));
-            O += f * ld_cluster(mapa_shared(smem_u32(part + i), k));
+              for (int w = 0; w < kWarps; ++w) O += f[w] * scratch[((w * S::MT + i) * 4 + warp) * 32 + lane];
+              const int d = (i0 + i) * 16 + (FP8 ? 2 * g + (warp >> 1) : g + 8 * (warp >> 1));
+              if constexpr (CLUSTER) {
+                part[col * HD + d] = O;
+                if (d == 0) s_ml[col] = make_float2(M, L);
+              } else if (begins && ends) {
+                p.o[r.b * p.o_b + (row0 + col) * p.o_h + d] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * vsc);
+                if (d == 0 && p.lse)
+                  p.lse[r.b * p.lse_b + row0 + col] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+              } else {
+                p.part_o[(static_cast<long long>(slot) * p.rows + col) * HD + d] = O;
+                if (d == 0) p.part_ml[static_cast<long long>(slot) * p.rows + col] = make_float2(M, L);
+              }
+            }
           }
-        p.o[r.b * p.o_b + (row0 + col) * p.o_h + d] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * vsc);
-        if (d == 0 && p.lse)
-          p.lse[r.b * p.lse_b + row0 + col] = L == 0.f ? -INFINITY : (M + log2f(L) - kUp) * kLn2;
+          __syncthreads();  // scratch and s_m are written again
+        }
       }
-      cluster_sync();  // no CTA leaves while another reads its shared memory
-      break;
+      if constexpr (CLUSTER) {
+        // ---- every CTA of the cluster joins its share of the elements
+        cluster_sync();
+        for (int i = rank * kThreads + tid; i < nrows * HD; i += csize * kThreads) {
+          const int col = i / HD, d = i - col * HD;
+          float M = -INFINITY, L = 0.f, O = 0.f;
+          float cm[kMaxCluster];
+#pragma unroll
+          for (int k = 0; k < kMaxCluster; ++k) {
+            cm[k] = k < csize ? ld_cluster(mapa_shared(smem_u32(&s_ml[col]), k)) : -INFINITY;
+            M = fmaxf(M, cm[k]);
+          }
+          const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+          for (int k = 0; k < kMaxCluster; ++k)
+            if (k < csize) {
+              const float f = ex2_approx(cm[k] - ref);
+              L += f * ld_cluster(mapa_shared(smem_u32(&s_ml[col].y), k));
+              O += f * ld_cluster(mapa_shared(smem_u32(part + i), k));
+            }
+          p.o[r.b * p.o_b + (row0 + col) * p.o_h + d] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * vsc);
+          if (d == 0 && p.lse)
+            p.lse[r.b * p.lse_b + row0 + col] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+        }
+        cluster_sync();  // no CTA leaves while another reads its shared memory
+        break;
+      }
     }
     r = nr;
     live = again;
@@ -719,41 +819,41 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   if (bad_page && p.err) atomicExch(p.err, kErrPage);
 }
 
-// Joins the partials of each (sequence, head tile) that more than one CTA worked
-// on: block j does the one that began in CTA j's range and went on past its
-// end.  A group of lanes covers one row (query head) with 16 bytes each; the
-// groups of a row take every `per_row`-th partial, with a running maximum of
-// their own, so that a partial's sum and its values are loaded together, and are
-// added up in a fixed order.  grid.y splits the rows.
+// Joins the partials of each segment that more than one CTA worked on: block j
+// does the one that began in CTA j's range and went on past its end.  A group of
+// lanes covers one row (query head) with 16 bytes each; the groups of a row take
+// every `per_row`-th partial, with a running maximum of their own, so that a
+// partial's sum and its values are loaded together, and are added up in a
+// fixed order.  grid.y splits the rows.
 template <int HD, bool FP8>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, const int tiles) {
   constexpr int LPR = HD / 4;                     // lanes (of float4) that cover a row
   constexpr int GR = kJoinThreads / LPR;          // groups of lanes
-  constexpr float kUp = FP8 ? 7.f : 0.f;
   __shared__ float4 s_o[GR][LPR];
   __shared__ float2 s_ml[GR];
   griddep_sync();
   const int j = blockIdx.x;
   const int4 d = p.desc[j];
   if (d.x < 0) return;
-  const int b = d.x, h = d.y / p.mtiles, mt = d.y - h * p.mtiles, n = d.z - j + 1;
-  const int nrows = min(p.rows, p.group - mt * p.rows);
-  const int row0 = h * p.group + mt * p.rows;
+  const int b = d.x, n = d.z - j + 1;
+  const int seg_rows = tiles * p.rows;            // `tiles` tiles of query heads lie in a segment
   const int li = threadIdx.x % LPR, gi = threadIdx.x / LPR;
-  const int rows = (nrows - blockIdx.y + gridDim.y - 1) / static_cast<int>(gridDim.y);  // of this block
+  const int rows = (seg_rows - blockIdx.y + gridDim.y - 1) / static_cast<int>(gridDim.y);  // of this block
   if (rows <= 0) return;
   const int per_row = max(1, GR / rows);
   for (int i0 = 0; i0 < rows; i0 += GR / per_row) {
     const int i = i0 + gi / per_row, sub = gi % per_row;
-    const bool on = i < rows && gi / per_row < GR / per_row;
     const int r = blockIdx.y + i * gridDim.y;
+    const int hm = d.y * tiles + r / p.rows, h = hm / p.mtiles, mt = hm - h * p.mtiles;
+    const int row = mt * p.rows + r % p.rows;  // in the group of kv head h (the last tile may be short)
+    const bool on = i < rows && gi / per_row < GR / per_row && row < p.group;
     float M = -INFINITY, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
     if (on) {
 #pragma unroll 4
       for (int k = sub; k < n; k += per_row) {
         // partial k of this segment: slot 2 j + 1, then slot 0 of the CTAs that follow
-        const long long at = (k == 0 ? 2LL * j + 1 : 2LL * (j + k)) * p.rows + r;
+        const long long at = (k == 0 ? 2LL * j + 1 : 2LL * (j + k)) * seg_rows + r;
         const float2 ml = p.part_ml[at];
         const float4 x = reinterpret_cast<const float4*>(p.part_o + at * HD)[li];
         const float m = fmaxf(M, ml.x), ref = m == -INFINITY ? 0.f : m;
@@ -786,13 +886,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
       }
       const float vsc = (FP8 && p.v_scale) ? p.v_scale[h] : 1.f;
       const float inv = L == 0.f ? 0.f : vsc / L;  // (L is 0 only where every key was left out: O is 0 too)
-      __nv_bfloat16* out = p.o + b * p.o_b + (row0 + r) * p.o_h + li * 4;
+      __nv_bfloat16* out = p.o + b * p.o_b + (h * p.group + row) * p.o_h + li * 4;
       out[0] = __float2bfloat16_rn(O.x * inv);
       out[1] = __float2bfloat16_rn(O.y * inv);
       out[2] = __float2bfloat16_rn(O.z * inv);
       out[3] = __float2bfloat16_rn(O.w * inv);
       if (li == 0 && p.lse)
-        p.lse[b * p.lse_b + row0 + r] = L == 0.f ? -INFINITY : (M + log2f(L) - kUp) * kLn2;
+        p.lse[b * p.lse_b + h * p.group + row] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
     }
     __syncthreads();
   }
@@ -807,51 +907,67 @@ int ctas_per_sm() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return 0;
   if (known[dev] == 0) {
-    int k = 0;
-    if (cudaFuncSetAttribute(decode_kernel<HD, FP8, NH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(decode_kernel<HD, FP8, NH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-            cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&k, decode_kernel<HD, FP8, NH, false>, kThreads, smem) !=
-            cudaSuccess)
-      return 0;
-    known[dev] = k;
+    int least = INT32_MAX;
+    void (*const kerns[3])(const Params) = {decode_kernel<HD, FP8, NH, 0>, decode_kernel<HD, FP8, NH, 1>,
+                                            decode_kernel<HD, FP8, NH, 2>};
+    for (auto kern : kerns) {
+      int k = 0;
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&k, kern, kThreads, smem) != cudaSuccess)
+        return 0;
+      if (k < least) least = k;
+    }
+    known[dev] = least;
   }
   return known[dev];
 }
 
-// How a call is launched: clustered with `cluster` CTAs per (sequence, head
-// tile), or (cluster 0) flat with `grid` CTAs.
+// How a call is launched.
 struct Plan {
-  int grid, cluster;
+  int mode, grid, cluster;
+  int tiles() const { return mode == kByHeads ? kWarps : 1; }  // tiles of query heads in a segment
 };
 
 template <int HD, bool FP8, int NH>
 Plan plan_of(int B, int heads, int max_blocks, int page) {
   const int occ = ctas_per_sm<HD, FP8, NH>();
-  if (occ <= 0) return {0, 0};
+  if (occ <= 0) return {0, 0, 0};
   const long long card = static_cast<long long>(sm_count()) * occ;
   const long long segs = static_cast<long long>(B) * heads;
-  const long long units = (static_cast<long long>(max_blocks) * page + kUnit - 1) / kUnit;  // of a full table row
+  const long long cap = static_cast<long long>(max_blocks) * page;
+  constexpr int unit = Shape<HD, FP8>::TILE * kWarps;
+  const long long units = (cap + unit - 1) / unit;  // of a full table row
   int c = 1;
   while (c < kMaxCluster && 2 * c <= units && segs * 2 * c <= card) c *= 2;
-  if (units <= 8 * c && segs * c <= INT32_MAX) return {static_cast<int>(segs * c), c};
-  return {static_cast<int>(segs * units < card ? segs * units : card), 0};
+  if (cap <= 512 * c && segs * c <= INT32_MAX) return {kClustered, static_cast<int>(segs * c), c};
+  // The four warps of a CTA on four heads (no join of the warps at a run's end, four
+  // times the partials at a CTA's) or on one: by heads where sequences end often,
+  // that is where there are at least half as many (sequence, head) pairs as
+  // CTAs, and the partials are small (groups of up to 8).  By heads / by keys: 64
+  // sequences of up to 2048, 16 heads of 64, token-major: 58.8 / 73.8 us; e4m3,
+  // 64 of up to 4097, 32/8 heads of 128: 59.1 / 62.0; but 1 of 131072: 94.4 / 86.1;
+  // 32 of up to 8192, 64/4 heads of 128: 84.6 / 59.4.
+  // (A unit is as many bytes either way, so there are as many of them.)
+  const int mode = heads % kWarps == 0 && NH == 1 && 2 * segs >= card ? kByHeads : kByKeys;
+  return {mode, static_cast<int>(segs * units < card ? segs * units : card), 0};
 }
 
 template <int HD, bool FP8, int NH>
 int launch(Params& p, const Plan& plan, cudaStream_t stream) {
   constexpr int smem = Shape<HD, FP8>::SMEM;
-  if (plan.cluster > 0) {
-    launch_kernel(decode_kernel<HD, FP8, NH, true>, dim3(plan.grid), dim3(kThreads), smem, stream, plan.cluster, p);
+  const dim3 grid(plan.grid), block(kThreads);
+  if (plan.mode == kClustered) {
+    launch_kernel(decode_kernel<HD, FP8, NH, kClustered>, grid, block, smem, stream, plan.cluster, p);
     return launch_status();
   }
-  launch_kernel(decode_kernel<HD, FP8, NH, false>, dim3(plan.grid), dim3(kThreads), smem, stream, 1, p);
+  if (plan.mode == kByHeads) launch_kernel(decode_kernel<HD, FP8, NH, kByHeads>, grid, block, smem, stream, 1, p);
+  else launch_kernel(decode_kernel<HD, FP8, NH, kByKeys>, grid, block, smem, stream, 1, p);
   const int st = launch_status();
   if (st != NL_OK) return st;
-  // few (sequence, head) pairs: many partials each, so their rows are split over blocks too
-  const int ysplit = static_cast<long long>(p.B) * p.Hk * p.mtiles <= 16 ? p.rows : 1;
-  launch_kernel(join_kernel<HD, FP8>, dim3(plan.grid, ysplit), dim3(kJoinThreads), 0, stream, 1, p);
+  // few segments: many partials each, so their rows are split over blocks too
+  const int rows = plan.tiles() * p.rows;
+  const int ysplit = static_cast<long long>(p.B) * p.Hk * p.mtiles <= 16 * plan.tiles() ? rows : 1;
+  launch_kernel(join_kernel<HD, FP8>, dim3(plan.grid, ysplit), dim3(kJoinThreads), 0, stream, 1, p, plan.tiles());
   return launch_status();
 }
 
@@ -881,7 +997,8 @@ struct LaunchCall {
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // Workspace of a flat call: partials and descriptors (a clustered call needs none).
 size_t workspace(const Plan& plan, int rows, int d, size_t* ml, size_t* desc) {
-  if (plan.cluster > 0) return 0;
+  if (plan.mode == kClustered) return 0;
+  rows *= plan.tiles();
   size_t n = align256(static_cast<size_t>(2) * plan.grid * rows * d * sizeof(float));
   if (ml) *ml = n;
   n += align256(static_cast<size_t>(2) * plan.grid * rows * sizeof(float2));
@@ -899,8 +1016,8 @@ bool shape_ok(int B, int Hq, int Hk, int d, int page, int max_blocks) {
   split_group(Hq / Hk, &rows, &mtiles);
   const long long cap = static_cast<long long>(max_blocks) * page;
   // unit counts of a call are 32-bit
-  return cap <= INT32_MAX - kUnit &&
-         static_cast<double>(B) * Hk * mtiles * static_cast<double>((cap + kUnit - 1) / kUnit + kOver) <= INT32_MAX;
+  return cap <= INT32_MAX - 256 &&
+         static_cast<double>(B) * Hk * mtiles * static_cast<double>((cap + 63) / 64 + kOver) <= INT32_MAX;
 }
 
 }  // namespace pa
