@@ -9,10 +9,16 @@
 // No reference counterpart (nlearn/model.py:440-444 samples the raw logits).
 //
 // Bound: HBM, one read and one write of the logits.  A CTA owns a chunk of one
-// row's columns: it counts the row's tokens that fall into the chunk in shared
-// memory (integer atomics: the order does not matter), sums the biases the
-// same way, and then streams the chunk once.  The row's history is read once
-// per chunk, from L2 after the first time.
+// row's columns.  The chunk comes into shared memory by asynchronous copies;
+// meanwhile the row's tokens that fall into it are counted there (integer
+// atomics: the order does not matter), and the first that comes to a column puts
+// the column on a list.  The list is then worked off with all lanes busy, on the
+// copy in shared memory, and the chunk is written once, with the mask.  (With the
+// rules inside a pass over all columns nearly every warp held a named one and
+// took the long way; with the list worked off in global memory its scattered
+// 2-byte accesses were the longest part: 36 and 27 us for 256 rows of 50257 in
+// bf16 with 2048 tokens each.)  In place and without a mask the chunk is not
+// copied: only the columns on the list are read and written.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <math.h>
@@ -24,8 +30,21 @@
 namespace nl {
 namespace lg {
 
-constexpr int kThreads = 256;
-constexpr uint32_t kSeen = 0x80000000u;  // a token's count word: occurs in the prompt
+constexpr int kThreads = 768;
+constexpr int kCtas = 2;              // resident CTAs of an SM: registers and shared memory are kept for them
+constexpr int kList = 128;            // biases of a row that are kept in shared memory
+constexpr int kSmem = 108 * 1024;     // dynamic shared memory of a CTA: kCtas of them fit an SM
+
+
+// A column's word: how often it was generated, and two flags.
+template <typename C>
+struct Word {
+  static constexpr int BITS = 8 * sizeof(C);
+  static constexpr uint32_t kSeen = 1u << (BITS - 1);   // occurs in the prompt
+  static constexpr uint32_t kNamed = 1u << (BITS - 2);  // a bias names it
+  static constexpr uint32_t kCount = kNamed - 1;
+  static constexpr uint32_t kField = kSeen | kNamed | kCount;
+};
 
 struct Params {
   const void* x;
@@ -45,7 +64,7 @@ struct Params {
   const uint32_t* mask;  // [R, words]
   long long ldm;
   const int* mask_rows;  // null: row b uses mask row b; < 0: row b has no mask
-  int V, L, n_bias, n_masks, chunk;
+  int V, L, n_bias, n_masks, chunk, staged;  // staged: the chunk goes through shared memory
 };
 
 template <typename T>
@@ -61,77 +80,291 @@ __device__ __forceinline__ float put<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 put<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// 16 bytes of a row's columns: x[i .. i + VEC) of n columns that exist.  Rows that
+// are not 16-byte aligned are read by 32-bit words, shifted together.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) process_kernel(const Params p) {
-  extern __shared__ uint32_t s_count[];  // [chunk], then (with biases) float [chunk]
-  float* s_bias = reinterpret_cast<float*>(s_count + p.chunk);
-  const int tid = threadIdx.x;
-  const int b = blockIdx.y, c0 = blockIdx.x * p.chunk, n = min(p.chunk, p.V - c0);
-  griddep_sync();
-  const bool counts = p.tokens != nullptr, biases = p.n_bias > 0;
-  float rep = 1.f, freq = 0.f, pres = 0.f;
-  if (counts) {
-    rep = p.repetition ? p.repetition[b] : 1.f;
-    freq = p.frequency ? p.frequency[b] : 0.f;
-    pres = p.presence ? p.presence[b] : 0.f;
+struct Piece {
+  static constexpr int VEC = 16 / sizeof(T);
+  uint4 w;
+  __device__ __forceinline__ void load(const T* x, int i, int n, bool aligned) {
+    if (aligned && i + VEC <= n) {
+      w = *reinterpret_cast<const uint4*>(x + i);
+      return;
+    }
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x + i);
+    if (i > 0 && i + VEC < n) {  // the words around the piece lie in the row too
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+      if (sizeof(T) == 4 || (a & 3) == 0) {
+        w = make_uint4(p[0], p[1], p[2], p[3]);
+      } else {
+        const uint32_t w0 = p[0], w1 = p[1], w2 = p[2], w3 = p[3], w4 = p[4];
+        w = make_uint4(__funnelshift_r(w0, w1, 16), __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
+                       __funnelshift_r(w3, w4, 16));
+      }
+      return;
+    }
+    T e[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) e[k] = i + k < n ? x[i + k] : put<T>(0.f);
+    w = *reinterpret_cast<const uint4*>(e);
   }
-  if (counts)
-    for (int i = tid; i < n; i += kThreads) s_count[i] = 0;
-  if (biases)
-    for (int i = tid; i < n; i += kThreads) s_bias[i] = 0.f;
-  __syncthreads();
-  if (counts) {
-    const int len = max(0, min(p.lens[b], p.L));
-    const int prompt = p.prompt_lens ? max(0, min(p.prompt_lens[b], len)) : 0;
-    const int* t = p.tokens + b * p.ldt;
-    for (int i = tid; i < len; i += kThreads) {
-      const unsigned j = static_cast<unsigned>(t[i]) - static_cast<unsigned>(c0);
-      if (j < static_cast<unsigned>(n)) {
-        if (i < prompt) atomicOr(s_count + j, kSeen);
-        else atomicAdd(s_count + j, 1u);
+  // from shared memory, where the words around the piece can always be read
+  __device__ __forceinline__ void load_shared(const T* x, bool aligned) {
+    if (aligned) {
+      w = *reinterpret_cast<const uint4*>(x);
+      return;
+    }
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x);
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+    w = make_uint4(p[0], p[1], p[2], p[3]);
+    if (sizeof(T) == 2 && (a & 2)) {
+      const uint32_t w4 = p[4];
+      w = make_uint4(__funnelshift_r(w.x, w.y, 16), __funnelshift_r(w.y, w.z, 16), __funnelshift_r(w.z, w.w, 16),
+                     __funnelshift_r(w.w, w4, 16));
+    }
+  }
+  // columns whose bit is 0 become -inf
+  __device__ __forceinline__ void mask(uint32_t bits) {
+    uint32_t* u = &w.x;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (!(bits >> k & 1)) u[k] = 0xff800000u;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // bits 2 k and 2 k + 1 to the tops of the two halves, spread over them
+        const uint32_t lo = bits << (15 - 2 * k), hi = bits << (30 - 2 * k);
+        uint32_t keep;
+        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(keep) : "r"((lo & 0xffffu) | (hi & 0xffff0000u)));
+        u[k] = (u[k] & keep) | (0xff80ff80u & ~keep);
       }
     }
   }
-  if (biases) {
-    const int* ids = p.bias_ids + b * p.ldb;
-    const float* val = p.bias + b * p.ldb;
-    for (int i = tid; i < p.n_bias; i += kThreads) {
-      const int id = ids[i];
-      const unsigned j = static_cast<unsigned>(id) - static_cast<unsigned>(c0);
-      if (j >= static_cast<unsigned>(n)) continue;
-      // the first entry of an id sums the later ones, in list order
-      bool first = true;
-      for (int k = 0; k < i; ++k) first = first && ids[k] != id;
-      if (!first) continue;
-      float sum = val[i];
-      for (int k = i + 1; k < p.n_bias; ++k)
-        if (ids[k] == id) sum += val[k];
-      s_bias[j] = sum;
+  __device__ __forceinline__ void store(T* y, int i, int n, bool aligned) const {
+    if (aligned && i + VEC <= n) {
+      *reinterpret_cast<uint4*>(y + i) = w;
+      return;
     }
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (i + k < n) y[i + k] = e[k];
   }
-  __syncthreads();
+};
+
+// Four of a row's tokens, -1 past the last.
+__device__ __forceinline__ int4 four_tokens(const int* t, int i, int len, bool vec) {
+  if (vec && i + 4 <= len) return *reinterpret_cast<const int4*>(t + i);
+  return make_int4(i < len ? t[i] : -1, i + 1 < len ? t[i + 1] : -1, i + 2 < len ? t[i + 2] : -1,
+                   i + 3 < len ? t[i + 3] : -1);
+}
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p) {
+  using W = Word<C>;
+  constexpr int VEC = Piece<T>::VEC;
+  constexpr uint32_t kAll = (1u << VEC) - 1;
+  constexpr int HEADS = 2;  // groups of four tokens a thread asks for at the start
+  extern __shared__ __align__(16) uint8_t smem[];  // words C [chunk], logits T [chunk + VEC] if staged, the list
+  uint8_t* s_chunk = smem + p.chunk * sizeof(C);
+  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_chunk + (p.staged ? (p.chunk + VEC) * sizeof(T) : 0));
+  __shared__ int s_ids[kList];
+  __shared__ float s_add[kList];
+  __shared__ int s_n;
+  const int tid = threadIdx.x;
+  const int b = blockIdx.y, c0 = blockIdx.x * p.chunk, n = min(p.chunk, p.V - c0);
+  const bool counts = p.tokens != nullptr, biases = p.n_bias > 0, sparse = counts || biases;
+  if (sparse)
+    for (int i = tid; i < static_cast<int>(p.chunk * sizeof(C) / 16); i += kThreads)
+      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) s_n = 0;
+  griddep_sync();
+  // ---- what depends on no other load is asked for first
+  const T* x = static_cast<const T*>(p.x) + b * p.ldx + c0;
+  T* y = static_cast<T*>(p.y) + b * p.ldy + c0;
+  const bool in_place = p.x == p.y;
+  const bool vec_in = (reinterpret_cast<uintptr_t>(x) & 15) == 0, vec_out = (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+  const int* t = counts ? p.tokens + b * p.ldt : nullptr;
+  const bool vec_t = (reinterpret_cast<uintptr_t>(t) & 15) == 0;
+  int4 head[HEADS];
+#pragma unroll
+  for (int k = 0; k < HEADS; ++k) head[k] = four_tokens(t, 4 * (k * kThreads + tid), counts ? p.L : 0, vec_t);
+  const int* ids = p.bias_ids + b * p.ldb;
+  const float* add = p.bias + b * p.ldb;
+  int my_id = -1, len = 0, prompt = 0;
+  float my_add = 0.f, rep = 1.f, freq = 0.f, pres = 0.f;
+  if (tid < min(p.n_bias, kList)) my_id = ids[tid], my_add = add[tid];
+  if (counts) {
+    len = p.lens[b];
+    if (p.prompt_lens) prompt = p.prompt_lens[b];
+    if (p.repetition) rep = p.repetition[b];
+    if (p.frequency) freq = p.frequency[b];
+    if (p.presence) pres = p.presence[b];
+  }
   const uint32_t* mask = nullptr;
   if (p.mask) {
     const int r = p.mask_rows ? p.mask_rows[b] : b;
-    if (r >= 0 && r < p.n_masks) mask = p.mask + r * p.ldm;
+    if (r >= 0 && r < p.n_masks) mask = p.mask + r * p.ldm + (c0 >> 5);
   }
-  const T* x = static_cast<const T*>(p.x) + b * p.ldx;
-  T* y = static_cast<T*>(p.y) + b * p.ldy;
-  for (int i = tid; i < n; i += kThreads) {
-    const int v = c0 + i;
-    float f = get<T>(x[v]);
-    if (counts) {
-      const uint32_t c = s_count[i];
-      if (c) {
-        f = f > 0.f ? f / rep : f * rep;
-        const uint32_t made = c & ~kSeen;
-        if (made) f = f - freq * static_cast<float>(made) - pres;
-      }
+  constexpr int STEP = kThreads * VEC;
+  // (chunks are multiples of 32 columns: the bits of a piece lie in one word)
+  auto bits_of = [&](int i) { return mask && i < n ? mask[i >> 5] >> (i & 31) & kAll : kAll; };
+  auto masked = [&](Piece<T>& piece, uint32_t bits) { if (bits != kAll) piece.mask(bits); };
+  if (!sparse) {  // no rule but the mask: straight through, two pieces ahead
+    if (in_place && !mask) return;
+    Piece<T> next[2];
+    uint32_t next_bits[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = tid * VEC + k * STEP;
+      if (i < n) next[k].load(x, i, n, vec_in);
+      next_bits[k] = bits_of(i);
     }
-    if (biases) f += s_bias[i];
-    if (mask && !(mask[v >> 5] >> (v & 31) & 1)) f = -INFINITY;
-    y[v] = put<T>(f);
+    for (int i = tid * VEC; i < n; i += STEP) {
+      Piece<T> cur = next[0];
+      const uint32_t bits = next_bits[0];
+      next[0] = next[1];
+      next_bits[0] = next_bits[1];
+      if (i + 2 * STEP < n) {
+        next[1].load(x, i + 2 * STEP, n, vec_in);
+        next_bits[1] = bits_of(i + 2 * STEP);
+      }
+      masked(cur, bits);
+      if (!in_place || bits != kAll) cur.store(y, i, n, vec_out);
+    }
+    return;
   }
+  // the chunk into shared memory, at the same place in a 16-byte unit as it has in memory
+  const int phase = p.staged ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
+  T* s_x = reinterpret_cast<T*>(s_chunk) + phase;
+  if (p.staged) {
+    const int lead = min(n, (VEC - phase) % VEC), units = (n - lead) / VEC, done = lead + units * VEC;
+    for (int i = tid; i < units; i += kThreads)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s_x + lead + i * VEC)),
+                   "l"(x + lead + i * VEC)
+                   : "memory");
+    if (tid < lead) s_x[tid] = x[tid];
+    if (tid < n - done) s_x[done + tid] = x[done + tid];
+  }
+
+  // ---- the columns that tokens and biases name
+  auto word_of = [&](unsigned j) { return reinterpret_cast<uint32_t*>(smem) + (sizeof(C) == 2 ? j >> 1 : j); };
+  auto shift_of = [&](unsigned j) { return sizeof(C) == 2 ? (j & 1) * 16 : 0; };
+  if (tid < kList) s_ids[tid] = my_id, s_add[tid] = my_add;
+  __syncthreads();
+  if (biases) {
+    for (int i = tid; i < p.n_bias; i += kThreads) {
+      const unsigned j = static_cast<unsigned>(i < kList ? my_id : ids[i]) - static_cast<unsigned>(c0);
+      if (j >= static_cast<unsigned>(n)) continue;
+      if ((atomicOr(word_of(j), W::kNamed << shift_of(j)) >> shift_of(j) & W::kField) == 0)
+        s_list[atomicAdd(&s_n, 1)] = static_cast<uint16_t>(j);
+    }
+    __syncthreads();  // a column with a bias is on the list before a token comes to it
+  }
+  if (counts) {
+    len = max(0, min(len, p.L));
+    prompt = min(prompt, len);
+    // whole warps: the new columns of its 128 tokens get their places on the list with one addition
+    auto count4 = [&](const int4& u, int i) {
+      const int token[4] = {u.x, u.y, u.z, u.w};
+      uint32_t fresh[4];
+      int total = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned j = static_cast<unsigned>(token[k]) - static_cast<unsigned>(c0);
+        bool is_new = false;
+        if (j < static_cast<unsigned>(n) && i + k < len) {
+          const uint32_t old = i + k < prompt ? atomicOr(word_of(j), W::kSeen << shift_of(j))
+                                              : atomicAdd(word_of(j), 1u << shift_of(j));
+          is_new = (old >> shift_of(j) & W::kField) == 0;
+        }
+        fresh[k] = __ballot_sync(0xffffffffu, is_new);
+        total += __popc(fresh[k]);
+      }
+      if (total == 0) return;
+      const int lane = tid & 31;
+      int at = lane == 0 ? atomicAdd(&s_n, total) : 0;
+      at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int mine = at + __popc(fresh[k] & ((1u << lane) - 1));
+        if (fresh[k] >> lane & 1) s_list[mine] = static_cast<uint16_t>(token[k] - c0);
+        at += __popc(fresh[k]);
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k)
+      if (4 * (k * kThreads + (tid & ~31)) < len) count4(head[k], 4 * (k * kThreads + tid));
+    for (int i0 = 4 * HEADS * kThreads + 4 * (tid & ~31); i0 < len; i0 += 4 * kThreads) {
+      const int i = i0 + 4 * (tid & 31);
+      count4(four_tokens(t, i, len, vec_t), i);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();  // counts, list and chunk
+  const T* from = p.staged ? s_x : x;
+  T* to = p.staged ? s_x : y;
+  const int on_list = s_n;
+  for (int i = tid; i < on_list; i += kThreads) {
+    const unsigned j = s_list[i];
+    const uint32_t w = *word_of(j) >> shift_of(j);
+    float f = get<T>(from[j]);
+    if (w & (W::kSeen | W::kCount)) {
+      f = f > 0.f ? f / rep : f * rep;
+      const uint32_t made = w & W::kCount;
+      if (made) f = f - freq * static_cast<float>(made) - pres;
+    }
+    if (w & W::kNamed) {  // its entries of the list, in order
+      const int id = c0 + static_cast<int>(j), kept = min(p.n_bias, kList);
+#pragma unroll 4
+      for (int m = 0; m < kept; ++m)
+        if (s_ids[m] == id) f += s_add[m];
+      for (int m = kept; m < p.n_bias; ++m)
+        if (ids[m] == id) f += add[m];
+    }
+    to[j] = put<T>(f);  // (rounded once: a masked column is overwritten below)
+  }
+  if (!p.staged) return;
+  __syncthreads();
+  const bool vec_s = phase == 0;
+  for (int i = tid * VEC; i < n; i += STEP) {
+    Piece<T> cur;
+    cur.load_shared(s_x + i, vec_s);
+    masked(cur, bits_of(i));
+    cur.store(y, i, n, vec_out);
+  }
+}
+
+// Columns of a CTA: a row in as many equal chunks as fill one wave of CTAs, of at most `most` columns.
+int chunk_of(int B, int V, int most) {
+  int parts = sm_count() * kCtas / B;
+  const int least = (V + most - 1) / most, limit = (V + 2047) / 2048;
+  if (parts > limit) parts = limit;
+  if (parts < least) parts = least;
+  return ((V + parts - 1) / parts + 63) / 64 * 64;
+}
+
+template <typename T, typename C>
+int launch(Params& p, int B, cudaStream_t stream) {
+  const bool sparse = p.tokens || p.n_bias > 0;
+  p.staged = sparse && !(p.x == p.y && !p.mask);
+  // a list holds each column once, and no more than there are tokens and biases
+  const int bytes = sizeof(C) + (p.staged ? sizeof(T) : 0), tail = 64;
+  const long long list = static_cast<long long>(p.tokens ? p.L : 0) + p.n_bias;
+  long long most = 65536;
+  if (sparse) {
+    most = (kSmem - tail) / (bytes + 2);
+    if (list < most) most = (kSmem - tail - 2 * list) / bytes;
+  }
+  p.chunk = chunk_of(B, p.V, static_cast<int>(most / 64 * 64));
+  const size_t smem =
+      sparse ? tail + static_cast<size_t>(p.chunk) * bytes + 2 * static_cast<size_t>(list < p.chunk ? list : p.chunk)
+             : 0;
+  if (cudaFuncSetAttribute(process_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    return NL_ERR_LAUNCH;
+  launch_kernel(process_kernel<T, C>, dim3((p.V + p.chunk - 1) / p.chunk, B), dim3(kThreads), smem, stream, 1, p);
+  return launch_status();
 }
 
 }  // namespace lg
@@ -151,11 +384,9 @@ extern "C" int nl_process_logits(const void* logits, long long ldx, int dtype, v
   if (n_bias < 0 || (n_bias > 0 && (!bias_ids || !bias || ldb < n_bias))) return NL_ERR_SHAPE;
   if (mask && (ldm < (V + 31) / 32 || n_masks <= 0 || (!mask_rows && n_masks < B))) return NL_ERR_SHAPE;
   lg::Params p{logits, ldx,  out,  ldy, tokens, ldt, lens, prompt_lens, repetition, frequency, presence, bias_ids,
-               bias,   ldb, static_cast<const uint32_t*>(mask), ldm, mask_rows, V, tokens ? L : 0, n_bias, n_masks, 0};
-  p.chunk = 4096;
-  const size_t smem = static_cast<size_t>(p.chunk) * (4 + (n_bias > 0 ? 4 : 0));
-  const dim3 grid((V + p.chunk - 1) / p.chunk, B);
-  if (dtype == NL_F32) launch_kernel(lg::process_kernel<float>, grid, dim3(lg::kThreads), smem, stream, 1, p);
-  else launch_kernel(lg::process_kernel<__nv_bfloat16>, grid, dim3(lg::kThreads), smem, stream, 1, p);
-  return launch_status();
+               bias,   ldb, static_cast<const uint32_t*>(mask), ldm, mask_rows, V, tokens ? L : 0, n_bias, n_masks, 0, 0};
+  const bool small = p.L <= static_cast<int>(lg::Word<uint16_t>::kCount);  // no count can overflow
+  if (dtype == NL_F32)
+    return small ? lg::launch<float, uint16_t>(p, B, stream) : lg::launch<float, uint32_t>(p, B, stream);
+  return small ? lg::launch<__nv_bfloat16, uint16_t>(p, B, stream) : lg::launch<__nv_bfloat16, uint32_t>(p, B, stream);
 }
