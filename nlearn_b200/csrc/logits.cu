@@ -361,8 +361,15 @@ int launch(Params& p, int B, cudaStream_t stream) {
   const size_t smem =
       sparse ? tail + static_cast<size_t>(p.chunk) * bytes + 2 * static_cast<size_t>(list < p.chunk ? list : p.chunk)
              : 0;
-  if (cudaFuncSetAttribute(process_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-    return NL_ERR_LAUNCH;
+  constexpr int kMaxDev = 64;
+  static bool ready[kMaxDev] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return NL_ERR_CUDA;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(process_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+      return NL_ERR_LAUNCH;
+    ready[dev] = true;
+  }
   launch_kernel(process_kernel<T, C>, dim3((p.V + p.chunk - 1) / p.chunk, B), dim3(kThreads), smem, stream, 1, p);
   return launch_status();
 }
@@ -372,19 +379,22 @@ int launch(Params& p, int B, cudaStream_t stream) {
 
 using namespace nl;
 
-extern "C" int nl_process_logits(const void* logits, long long ldx, int dtype, void* out, long long ldy,
-                                 const int* tokens, long long ldt, const int* lens, const int* prompt_lens, int L,
-                                 const float* repetition, const float* frequency, const float* presence,
-                                 const int* bias_ids, const float* bias, long long ldb, int n_bias,
-                                 const void* mask, long long ldm, int n_masks, const int* mask_rows, int B, int V,
-                                 cudaStream_t stream) {
-  if (B <= 0 || B > 65535 || V <= 0 || ldx < V || ldy < V || !logits || !out) return NL_ERR_SHAPE;
+static_assert(sizeof(nl_process_logits_args) == 160, "packed by _lib.py");
+
+extern "C" int nl_process_logits(const nl_process_logits_args* args, cudaStream_t stream) {
+  if (!args) return NL_ERR_SHAPE;
+  const nl_process_logits_args& a = *args;
+  const int B = a.B, V = a.V, dtype = a.dtype;
+  if (B <= 0 || B > 65535 || V <= 0 || a.ldx < V || a.ldy < V || !a.logits || !a.out) return NL_ERR_SHAPE;
   if (dtype != NL_F32 && dtype != NL_BF16) return NL_ERR_DTYPE;
-  if (tokens && (L <= 0 || ldt < L || !lens)) return NL_ERR_SHAPE;
-  if (n_bias < 0 || (n_bias > 0 && (!bias_ids || !bias || ldb < n_bias))) return NL_ERR_SHAPE;
-  if (mask && (ldm < (V + 31) / 32 || n_masks <= 0 || (!mask_rows && n_masks < B))) return NL_ERR_SHAPE;
-  lg::Params p{logits, ldx,  out,  ldy, tokens, ldt, lens, prompt_lens, repetition, frequency, presence, bias_ids,
-               bias,   ldb, static_cast<const uint32_t*>(mask), ldm, mask_rows, V, tokens ? L : 0, n_bias, n_masks, 0, 0};
+  if (a.tokens && (a.L <= 0 || a.ldt < a.L || !a.lens)) return NL_ERR_SHAPE;
+  if (a.n_bias < 0 || (a.n_bias > 0 && (!a.bias_ids || !a.bias || a.ldb < a.n_bias))) return NL_ERR_SHAPE;
+  if (a.mask && (a.ldm < (V + 31) / 32 || a.n_masks <= 0 || (!a.mask_rows && a.n_masks < B))) return NL_ERR_SHAPE;
+  const size_t align = dtype == NL_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.out)) % align) return NL_ERR_ALIGN;
+  lg::Params p{a.logits, a.ldx, a.out, a.ldy, a.tokens, a.ldt, a.lens, a.prompt_lens, a.repetition, a.frequency,
+               a.presence, a.bias_ids, a.bias, a.ldb, static_cast<const uint32_t*>(a.mask), a.ldm, a.mask_rows, V,
+               a.tokens ? a.L : 0, a.n_bias, a.n_masks, 0, 0};
   const bool small = p.L <= static_cast<int>(lg::Word<uint16_t>::kCount);  // no count can overflow
   if (dtype == NL_F32)
     return small ? lg::launch<float, uint16_t>(p, B, stream) : lg::launch<float, uint32_t>(p, B, stream);

@@ -1025,6 +1025,8 @@ bool shape_ok(int B, int Hq, int Hk, int d, int page, int max_blocks) {
 
 using namespace nl;
 
+static_assert(sizeof(nl_paged_attention_args) == 232, "packed by _lib.py");
+
 extern "C" size_t nl_paged_attention_workspace_bytes(int B, int Hq, int Hk, int d, int page_size, int max_blocks,
                                                      int cache_dtype) {
   if (!pa::shape_ok(B, Hq, Hk, d, page_size, max_blocks)) return 0;
@@ -1035,32 +1037,31 @@ extern "C" size_t nl_paged_attention_workspace_bytes(int B, int Hq, int Hk, int 
   return pa::workspace(plan, rows, d, nullptr, nullptr);
 }
 
-extern "C" int nl_paged_attention(const void* q, long long q_b, long long q_h, void* k_cache, void* v_cache,
-                                  int cache_dtype, long long page_stride, long long head_stride,
-                                  long long tok_stride, const int* block_table, long long table_ld, const int* lens,
-                                  const void* k_new, const void* v_new, long long n_b, long long n_h,
-                                  const float* k_scale, const float* v_scale, float scale, void* o, long long o_b,
-                                  long long o_h, float* lse, long long lse_b, void* workspace, size_t ws_bytes, int B,
-                                  int Hq, int Hk, int d, int page_size, int max_blocks, int n_pages,
-                                  cudaStream_t stream) {
-  if (!pa::shape_ok(B, Hq, Hk, d, page_size, max_blocks) || n_pages <= 0 || table_ld < max_blocks)
+extern "C" int nl_paged_attention(const nl_paged_attention_args* args, cudaStream_t stream) {
+  if (!args) return NL_ERR_SHAPE;
+  const nl_paged_attention_args& a = *args;
+  const int B = a.B, Hq = a.Hq, Hk = a.Hk, d = a.d, page_size = a.page_size, max_blocks = a.max_blocks;
+  const int n_pages = a.n_pages, cache_dtype = a.cache_dtype;
+  const long long page_stride = a.page_stride, head_stride = a.head_stride, tok_stride = a.tok_stride;
+  if (!pa::shape_ok(B, Hq, Hk, d, page_size, max_blocks) || n_pages <= 0 || a.table_ld < max_blocks)
     return NL_ERR_SHAPE;
   if (cache_dtype != NL_BF16 && cache_dtype != NL_E4M3) return NL_ERR_DTYPE;
-  if (!q || !k_cache || !v_cache || !block_table || !lens || !o || (k_new != nullptr) != (v_new != nullptr))
+  if (!a.q || !a.k_cache || !a.v_cache || !a.block_table || !a.lens || !a.o ||
+      (a.k_new != nullptr) != (a.v_new != nullptr))
     return NL_ERR_SHAPE;
-  if (page_stride <= 0 || tok_stride <= 0 || head_stride < 0 || q_b < 0 || q_h < 0 || n_b < 0 || n_h < 0)
+  if (page_stride <= 0 || tok_stride <= 0 || head_stride < 0 || a.q_b < 0 || a.q_h < 0 || a.n_b < 0 || a.n_h < 0)
     return NL_ERR_SHAPE;
   const int el = cache_dtype == NL_E4M3 ? 1 : 2;
-  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
-                         reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(k_new) |
-                         reinterpret_cast<uintptr_t>(v_new);
-  if ((ptrs & 15) || ((q_b | q_h | n_b | n_h) & 7) || ((page_stride | head_stride | tok_stride) * el & 15) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 255))
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_cache) |
+                         reinterpret_cast<uintptr_t>(a.v_cache) | reinterpret_cast<uintptr_t>(a.k_new) |
+                         reinterpret_cast<uintptr_t>(a.v_new);
+  if ((ptrs & 15) || ((a.q_b | a.q_h | a.n_b | a.n_h) & 7) || ((page_stride | head_stride | tok_stride) * el & 15) ||
+      (reinterpret_cast<uintptr_t>(a.workspace) & 255))
     return NL_ERR_ALIGN;
   // rows are addressed inside one head by 32-bit offsets of 16 bytes: 64 GB of each cache
-  const long long extent = (n_pages - 1) * (page_stride * el / 16) + (page_size - 1) * (tok_stride * el / 16);
-  if (page_stride * el / 16 > UINT32_MAX || tok_stride * el / 16 > UINT32_MAX || extent >= UINT32_MAX)
-    return NL_ERR_TOO_LARGE;
+  if (page_stride > (1LL << 36) || tok_stride > (1LL << 36)) return NL_ERR_TOO_LARGE;
+  const double extent = (n_pages - 1.) * (page_stride * el / 16) + (page_size - 1.) * (tok_stride * el / 16);
+  if (extent >= UINT32_MAX) return NL_ERR_TOO_LARGE;
   pa::Params p;
   p.group = Hq / Hk;
   pa::split_group(p.group, &p.rows, &p.mtiles);
@@ -1069,33 +1070,33 @@ extern "C" int nl_paged_attention(const void* q, long long q_b, long long q_h, v
   if (plan.grid <= 0) return NL_ERR_CUDA;
   size_t ml = 0, desc = 0;
   const size_t need = pa::workspace(plan, p.rows, d, &ml, &desc);
-  if (need > 0 && (!workspace || ws_bytes < need)) return NL_ERR_WORKSPACE;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (need > 0 && (!a.workspace || a.ws_bytes < need)) return NL_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = reinterpret_cast<float2*>(ws + ml);
   p.desc = reinterpret_cast<int4*>(ws + desc);
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.q_b = q_b;
-  p.q_h = q_h;
-  p.k = static_cast<uint8_t*>(k_cache);
-  p.v = static_cast<uint8_t*>(v_cache);
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.q_b = a.q_b;
+  p.q_h = a.q_h;
+  p.k = static_cast<uint8_t*>(a.k_cache);
+  p.v = static_cast<uint8_t*>(a.v_cache);
   p.page16 = static_cast<uint32_t>(page_stride * el / 16);
   p.tok16 = static_cast<uint32_t>(tok_stride * el / 16);
   p.head_bytes = head_stride * el;
-  p.table = block_table;
-  p.table_ld = table_ld;
-  p.lens = lens;
-  p.k_new = static_cast<const __nv_bfloat16*>(k_new);
-  p.v_new = static_cast<const __nv_bfloat16*>(v_new);
-  p.n_b = n_b;
-  p.n_h = n_h;
-  p.k_scale = cache_dtype == NL_E4M3 ? k_scale : nullptr;
-  p.v_scale = cache_dtype == NL_E4M3 ? v_scale : nullptr;
-  p.o = static_cast<__nv_bfloat16*>(o);
-  p.o_b = o_b;
-  p.o_h = o_h;
-  p.lse = lse;
-  p.lse_b = lse_b;
+  p.table = a.block_table;
+  p.table_ld = a.table_ld;
+  p.lens = a.lens;
+  p.k_new = static_cast<const __nv_bfloat16*>(a.k_new);
+  p.v_new = static_cast<const __nv_bfloat16*>(a.v_new);
+  p.n_b = a.n_b;
+  p.n_h = a.n_h;
+  p.k_scale = cache_dtype == NL_E4M3 ? a.k_scale : nullptr;
+  p.v_scale = cache_dtype == NL_E4M3 ? a.v_scale : nullptr;
+  p.o = static_cast<__nv_bfloat16*>(a.o);
+  p.o_b = a.o_b;
+  p.o_h = a.o_h;
+  p.lse = a.lse;
+  p.lse_b = a.lse_b;
   p.B = B;
   p.Hq = Hq;
   p.Hk = Hk;
@@ -1103,7 +1104,7 @@ extern "C" int nl_paged_attention(const void* q, long long q_b, long long q_h, v
   p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   p.max_blocks = max_blocks;
   p.n_pages = n_pages;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
   p.err = device_error_word();
   return pa::dispatch(d, cache_dtype == NL_E4M3, p.rows, pa::LaunchCall{p, plan, stream});
 }

@@ -265,19 +265,23 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const WriteParams p) {
 
 using namespace nl;
 
-extern "C" int nl_update_block_tables(int* block_table, long long table_ld, const int* lens, const int* new_lens,
-                                      const int* done, int* free_pages, const int* n_free, int* lens_out,
-                                      int* n_free_out, int* slots, int* positions, int* cu, int* status, int B,
-                                      int max_blocks, int page_size, int n_pages, int n_tokens, cudaStream_t stream) {
-  if (B <= 0 || B > pc::kMaxRows || max_blocks <= 0 || page_size <= 0 || n_pages <= 0 || n_tokens < 0 ||
-      table_ld < max_blocks || static_cast<long long>(max_blocks) * page_size > INT32_MAX ||
-      static_cast<long long>(n_pages) * page_size > INT32_MAX)
+static_assert(sizeof(nl_update_block_tables_args) == 128 && sizeof(nl_paged_kv_write_args) == 120,
+              "packed by _lib.py");
+
+extern "C" int nl_update_block_tables(const nl_update_block_tables_args* args, cudaStream_t stream) {
+  if (!args) return NL_ERR_SHAPE;
+  const nl_update_block_tables_args& a = *args;
+  const int B = a.B, n_tokens = a.n_tokens;
+  if (B <= 0 || B > pc::kMaxRows || a.max_blocks <= 0 || a.page_size <= 0 || a.n_pages <= 0 || n_tokens < 0 ||
+      a.table_ld < a.max_blocks || static_cast<long long>(a.max_blocks) * a.page_size > INT32_MAX ||
+      static_cast<long long>(a.n_pages) * a.page_size > INT32_MAX)
     return NL_ERR_SHAPE;
-  if (!block_table || !lens || !new_lens || !free_pages || !n_free || !lens_out || !n_free_out || !cu || !status ||
-      (n_tokens > 0 && (!slots || !positions)))
+  if (!a.block_table || !a.lens || !a.new_lens || !a.free_pages || !a.n_free || !a.lens_out || !a.n_free_out ||
+      !a.cu || !a.status || (n_tokens > 0 && (!a.slots || !a.positions)))
     return NL_ERR_SHAPE;
-  pc::TableParams p{block_table, table_ld, lens, new_lens, done, free_pages, n_free, lens_out, n_free_out, slots,
-                    positions,   cu,       status, B,      max_blocks, page_size, n_pages, n_tokens};
+  pc::TableParams p{a.block_table, a.table_ld, a.lens, a.new_lens, a.done, a.free_pages, a.n_free, a.lens_out,
+                    a.n_free_out, a.slots, a.positions, a.cu, a.status, B, a.max_blocks, a.page_size, a.n_pages,
+                    n_tokens};
   const size_t smem = static_cast<size_t>(B) * sizeof(int4);
   const bool wide = n_tokens > 4 * pc::kThreads;
   auto kern = wide ? pc::update_tables_kernel<true> : pc::update_tables_kernel<false>;
@@ -289,23 +293,25 @@ extern "C" int nl_update_block_tables(int* block_table, long long table_ld, cons
   return launch_status();
 }
 
-extern "C" int nl_paged_kv_write(const void* k, const void* v, long long n_t, long long n_h, void* k_cache,
-                                 void* v_cache, int cache_dtype, long long page_stride, long long head_stride,
-                                 long long tok_stride, const int* slots, const float* k_scale, const float* v_scale,
-                                 int T, int Hk, int d, int page_size, int n_pages, cudaStream_t stream) {
-  if (T <= 0 || Hk <= 0 || d <= 0 || page_size <= 0 || n_pages <= 0 || !k || !v || !k_cache || !v_cache || !slots ||
-      n_t < 0 || n_h < 0 || page_stride <= 0 || head_stride < 0 || tok_stride <= 0)
+extern "C" int nl_paged_kv_write(const nl_paged_kv_write_args* args, cudaStream_t stream) {
+  if (!args) return NL_ERR_SHAPE;
+  const nl_paged_kv_write_args& a = *args;
+  const int T = a.T, Hk = a.Hk, d = a.d, page_size = a.page_size, n_pages = a.n_pages, cache_dtype = a.cache_dtype;
+  const long long n_t = a.n_t, n_h = a.n_h;
+  const long long page_stride = a.page_stride, head_stride = a.head_stride, tok_stride = a.tok_stride;
+  if (T <= 0 || Hk <= 0 || d <= 0 || page_size <= 0 || n_pages <= 0 || !a.k || !a.v || !a.k_cache || !a.v_cache ||
+      !a.slots || n_t < 0 || n_h < 0 || page_stride <= 0 || head_stride < 0 || tok_stride <= 0)
     return NL_ERR_SHAPE;
   if (cache_dtype != NL_BF16 && cache_dtype != NL_E4M3) return NL_ERR_DTYPE;
   const bool fp8 = cache_dtype == NL_E4M3;
   const int el = fp8 ? 1 : 2, per = fp8 ? 16 : 8;  // elements of a 16-byte store
   if (d % per || static_cast<long long>(Hk) * (d / per) > INT32_MAX) return NL_ERR_SHAPE;
-  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-                         reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache);
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                         reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache);
   if ((ptrs & 15) || ((n_t | n_h) & 7) || ((page_stride | head_stride | tok_stride) * el & 15)) return NL_ERR_ALIGN;
-  pc::WriteParams p{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), n_t, n_h,
-                    static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), page_stride * el,
-                    head_stride * el, tok_stride * el, slots, k_scale, v_scale, T, Hk, d / per, page_size,
+  pc::WriteParams p{static_cast<const __nv_bfloat16*>(a.k), static_cast<const __nv_bfloat16*>(a.v), n_t, n_h,
+                    static_cast<uint8_t*>(a.k_cache), static_cast<uint8_t*>(a.v_cache), page_stride * el,
+                    head_stride * el, tok_stride * el, a.slots, a.k_scale, a.v_scale, T, Hk, d / per, page_size,
                     static_cast<long long>(n_pages) * page_size, device_error_word()};
   const long long n = static_cast<long long>(T) * Hk * (d / per);
   long long blocks = (n + 255) / 256;

@@ -6,18 +6,23 @@ import numpy as np
 import pytest
 import torch
 
-from nlearn_b200._lib import STATUS, lib
+from nlearn_b200._lib import ARGS, STATUS, lib
 from oracle import paged as OP
 
 P = 1 << 20  # an aligned non-null address that no refused call reads
 
 
+def call(name, defaults, kw):
+    """The status of a C entry point whose argument struct holds `defaults` changed by `kw`."""
+    assert set(kw) <= set(defaults)
+    return STATUS[getattr(lib, name)(ARGS[name].pack(*{**defaults, **kw}.values()), None)]
+
+
 def attention(**kw):
-    a = dict(q=P, q_b=512, q_h=64, k=P, v=P, dt=1, page_s=1024, head_s=8192, tok_s=64, table=P, table_ld=4, lens=P,
-             kn=0, vn=0, n_b=0, n_h=0, ks=0, vs=0, scale=1.0, o=P, o_b=512, o_h=64, lse=0, lse_b=0, ws=P, nb=0, B=2,
-             Hq=8, Hk=8, d=64, page=16, blocks=4, n_pages=10)
-    a.update(kw)
-    return STATUS[lib.nl_paged_attention(*a.values(), None)]
+    return call("nl_paged_attention",
+                dict(q=P, k=P, v=P, table=P, lens=P, kn=0, vn=0, ks=0, vs=0, o=P, lse=0, ws=P, q_b=512, q_h=64,
+                     page_s=1024, head_s=8192, tok_s=64, table_ld=4, n_b=0, n_h=0, o_b=512, o_h=64, lse_b=0, nb=0,
+                     B=2, Hq=8, Hk=8, d=64, page=16, blocks=4, n_pages=10, dt=1, scale=1.0), kw)
 
 
 @pytest.mark.parametrize("kw", [dict(B=0), dict(Hq=7), dict(Hk=0), dict(d=80), dict(page=0), dict(blocks=0),
@@ -44,10 +49,9 @@ def test_attention_workspace_of_refused_shapes():
 
 
 def write(**kw):
-    a = dict(k=P, v=P, n_t=512, n_h=64, kc=P, vc=P, dt=1, page_s=1024, head_s=8192, tok_s=64, slots=P, ks=0, vs=0,
-             T=3, Hk=8, d=64, page=16, n_pages=10)
-    a.update(kw)
-    return STATUS[lib.nl_paged_kv_write(*a.values(), None)]
+    return call("nl_paged_kv_write",
+                dict(k=P, v=P, kc=P, vc=P, slots=P, ks=0, vs=0, n_t=512, n_h=64, page_s=1024, head_s=8192, tok_s=64,
+                     T=3, Hk=8, d=64, page=16, n_pages=10, dt=1), kw)
 
 
 @pytest.mark.parametrize("kw,code", [(dict(T=0), "NL_ERR_SHAPE"), (dict(d=60), "NL_ERR_SHAPE"),
@@ -59,10 +63,9 @@ def test_write_refusals(kw, code):
 
 
 def tables(**kw):
-    a = dict(table=P, ld=4, lens=P, new=P, done=0, free=P, n_free=P, lens_out=P, n_free_out=P, slots=P, pos=P, cu=P,
-             status=P, B=2, blocks=4, page=16, n_pages=10, n_tokens=5)
-    a.update(kw)
-    return STATUS[lib.nl_update_block_tables(*a.values(), None)]
+    return call("nl_update_block_tables",
+                dict(table=P, lens=P, new=P, done=0, free=P, n_free=P, lens_out=P, n_free_out=P, slots=P, pos=P,
+                     cu=P, status=P, ld=4, B=2, blocks=4, page=16, n_pages=10, n_tokens=5), kw)
 
 
 @pytest.mark.parametrize("kw", [dict(B=0), dict(B=8193), dict(blocks=0), dict(page=0), dict(n_pages=0),
@@ -73,10 +76,9 @@ def test_table_refusals(kw):
 
 
 def logits(**kw):
-    a = dict(x=P, ldx=100, dt=0, y=P, ldy=100, tok=0, ldt=0, lens=0, pl=0, L=0, rep=0, fr=0, pr=0, ids=0, bias=0,
-             ldb=0, n_bias=0, mask=0, ldm=0, n_masks=0, mrows=0, B=2, V=100)
-    a.update(kw)
-    return STATUS[lib.nl_process_logits(*a.values(), None)]
+    return call("nl_process_logits",
+                dict(x=P, y=P, tok=0, lens=0, pl=0, rep=0, fr=0, pr=0, ids=0, bias=0, mask=0, mrows=0, ldx=100,
+                     ldy=100, ldt=0, ldb=0, ldm=0, dt=0, L=0, n_bias=0, n_masks=0, B=2, V=100), kw)
 
 
 @pytest.mark.parametrize("kw,code", [(dict(B=0), "NL_ERR_SHAPE"), (dict(B=65536), "NL_ERR_SHAPE"),
@@ -88,6 +90,11 @@ def logits(**kw):
                                      (dict(mask=P, ldm=4, n_masks=1), "NL_ERR_SHAPE")])
 def test_logits_refusals(kw, code):
     assert logits(**kw) == code
+
+
+@pytest.mark.parametrize("name", sorted(ARGS))
+def test_no_arguments(name):
+    assert STATUS[getattr(lib, name)(None, None)] == "NL_ERR_SHAPE"
 
 
 def test_cpu_tensors_raise():
