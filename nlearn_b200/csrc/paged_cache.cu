@@ -15,7 +15,11 @@
 // All of it is prefix sums over the rows, which every CTA of the one cluster
 // makes for itself, so the CTAs share no state but the two sides of the
 // cluster barrier: lengths, stack and tables are read before it and rewritten
-// after it (the outputs may then be the inputs).  Latency-bound: one launch.
+// after it (the outputs may then be the inputs).
+// Bound by latency: one launch, and a chain of five loads (lengths, freed pages, taken
+// pages, the slots' pages; each with all of a thread's loads in flight) and
+// two prefix sums.  256 rows of one token: 6.0 us; 96 prompts, 109000 slots: 10.1 us
+// (8 CTAs; up to 4096 slots one CTA does them without a cluster barrier).
 //
 // kv_write_kernel: a thread per 16 bytes of a key row and of its value row.
 // Bound by HBM: each element is read and written once.
@@ -31,7 +35,7 @@ namespace nl {
 namespace pc {
 
 constexpr int kThreads = 1024;
-constexpr int kMaxRows = 8192;  // rows of a block table: 16 bytes of shared memory each
+constexpr int kMaxRows = 8192;  // rows of a block table: 20 bytes of shared memory each
 
 enum : int { kOk = 0, kNoPages = 1, kTooLong = 2, kNoSlots = 3, kInvalid = 4 };  // status of a row
 enum : int { kErrPage = 4 };                                                      // device error word
@@ -50,30 +54,49 @@ struct TableParams {
   int* positions;
   int* cu;
   int* status;
-  int B, max_blocks, page, n_pages, tokens;
+  int B, max_blocks, page, page_shift, n_pages, tokens;
 };
 
-// Exclusive prefix sums of one value per thread over the block; total of all.
-__device__ __forceinline__ long long block_scan(long long v, long long* warp_sum, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long inc = v;
+// Exclusive prefix sums of two values per thread over the block, and their
+// totals.  Every warp sums the warps' totals for itself: one barrier, and one
+// before s_sum may be written again.
+struct Two {
+  long long a, b;
+};
+__device__ __forceinline__ Two warp_scan(Two v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += y;
+    const long long x = __shfl_up_sync(0xffffffffu, v.a, o), y = __shfl_up_sync(0xffffffffu, v.b, o);
+    if (lane >= o) {
+      v.a += x;
+      v.b += y;
+    }
   }
-  if (lane == 31) warp_sum[warp] = inc;
+  return v;
+}
+__device__ __forceinline__ Two block_scan(Two v, Two* s_sum, Two& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const Two inc = warp_scan(v);
+  if (lane == 31) s_sum[warp] = inc;
   __syncthreads();
-  long long s = warp_sum[lane];
+  const Two w = warp_scan(lane < warps ? s_sum[lane] : Two{0, 0});
+  total = {__shfl_sync(0xffffffffu, w.a, 31), __shfl_sync(0xffffffffu, w.b, 31)};
+  const int prev = warp > 0 ? warp - 1 : 0;
+  const long long pa = __shfl_sync(0xffffffffu, w.a, prev), pb = __shfl_sync(0xffffffffu, w.b, prev);
+  return {inc.a - v.a + (warp > 0 ? pa : 0), inc.b - v.b + (warp > 0 ? pb : 0)};
+}
+
+// A warp copies n entries, dst[i] = src[step i], with four loads of a lane in flight.
+__device__ __forceinline__ void move_pages(int* dst, const int* src, int n, int step) {
+  for (int i0 = threadIdx.x & 31; i0 < n; i0 += 128) {
+    int x[4];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += y;
+    for (int k = 0; k < 4; ++k) x[k] = i0 + 32 * k < n ? __ldcg(src + step * (i0 + 32 * k)) : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i0 + 32 * k < n) dst[i0 + 32 * k] = x[k];
   }
-  total = __shfl_sync(0xffffffffu, s, 31);
-  const long long before = warp == 0 ? 0 : __shfl_sync(0xffffffffu, s, warp == 0 ? 0 : warp - 1);
-  __syncthreads();
-  return before + inc - v;
 }
 
 __device__ __forceinline__ int sat(long long x) { return x > INT32_MAX ? INT32_MAX : static_cast<int>(x); }
@@ -81,127 +104,183 @@ __device__ __forceinline__ int sat(long long x) { return x > INT32_MAX ? INT32_M
 template <bool CLUSTER>
 __global__ void __launch_bounds__(kThreads) update_tables_kernel(const TableParams p) {
   extern __shared__ int4 s_row[];  // {first token, len0 or -1 if refused, first page from the top, pages held}
-  __shared__ long long s_sum[32];
-  const int tid = threadIdx.x, lane = tid & 31;
+  int* s_new = reinterpret_cast<int*>(s_row + p.B);  // tokens a row grows by
+  __shared__ Two s_sum[3][32];
+  __shared__ int s_used;
+  const int tid = threadIdx.x, lane = tid & 31, threads = blockDim.x;
   const int rank = blockIdx.x, nctas = gridDim.x;
+  if (tid == 0) s_used = 0;
   griddep_sync();
 
   const int P = p.page;
   const long long cap = static_cast<long long>(p.max_blocks) * P;
-  auto up = [P](int x) { return static_cast<int>((static_cast<long long>(x) + P - 1) / P); };
+  // pages of x tokens, page of position x (x >= 0; sums stay below 2^32)
+  auto block_of = [&](unsigned x) {
+    return static_cast<int>(p.page_shift >= 0 ? x >> p.page_shift : x / static_cast<unsigned>(P));
+  };
+  auto up = [&](int x) { return block_of(static_cast<unsigned>(x) + static_cast<unsigned>(P - 1)); };
   const int stack0 = max(0, min(*p.n_free, p.n_pages));
-  const int warps = nctas * (kThreads / 32), gw = rank * (kThreads / 32) + (tid >> 5);
+  const int warps = nctas * (threads / 32), gw = rank * (threads / 32) + (tid >> 5);
 
   // ---- first tokens, and the pages of rows that ended
   long long tok = 0, freed = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+  int turn = 0;  // consecutive scans use different sums: one barrier each
+  for (int b0 = 0; b0 < p.B; b0 += threads) {
     const int b = b0 + tid;
     int n = 0, back = 0, len = 0;
     if (b < p.B) {
       len = p.lens[b];
-      n = max(0, p.new_lens[b]);
+      n = p.new_lens[b];
       if (p.done && p.done[b] && len > 0 && len <= cap) back = up(len);
+      s_new[b] = n;
+      n = max(0, n);
     }
-    long long t, f;
-    const long long at = tok + block_scan(n, s_sum, t);
-    const long long top = freed + block_scan(back, s_sum, f);
+    Two t;
+    const Two at = block_scan({n, back}, s_sum[turn], t);
+    turn = turn == 2 ? 0 : turn + 1;
     if (b < p.B) {
-      s_row[b] = make_int4(sat(at), len, sat(top), back);
-      if (rank == 0) p.cu[b] = sat(at);
+      s_row[b] = make_int4(sat(tok + at.a), len, sat(freed + at.b), back);
+      if (rank == 0) p.cu[b] = sat(tok + at.a);
     }
-    tok += t;
-    freed += f;
+    tok += t.a;
+    freed += t.b;
   }
   if (rank == 0 && tid == 0) p.cu[p.B] = sat(tok);
-  __syncthreads();
-  if (freed > 0)
-    for (int b = gw; b < p.B; b += warps) {
-      const int4 r = s_row[b];
-      for (int i = lane; i < r.w; i += 32) {
-        const long long at = static_cast<long long>(stack0) + r.z + i;
-        if (at < p.n_pages) p.free_pages[at] = p.table[b * p.ld + i];
+  if (freed > 0) {  // (the same in every thread)
+    __syncthreads();
+    // a lane looks at a row, the warp moves its pages; neighbouring rows belong to different warps
+    for (int b0 = gw; b0 < p.B; b0 += warps * 32) {
+      const int mine = b0 + lane * warps;
+      uint32_t m = __ballot_sync(0xffffffffu, mine < p.B && s_row[mine].w > 0);
+      for (; m; m &= m - 1) {
+        const int b = b0 + (__ffs(m) - 1) * warps;
+        const int4 r = s_row[b];
+        // (entries past the stack's capacity, which only pages freed twice can make, are dropped)
+        const long long at = static_cast<long long>(stack0) + r.z;
+        if (at < p.n_pages)
+          move_pages(p.free_pages + at, p.table + b * p.ld,
+                     static_cast<int>(min(static_cast<long long>(r.w), p.n_pages - at)), 1);
       }
     }
-  __syncthreads();
+    __syncthreads();
+  }
   const int avail = static_cast<int>(min(static_cast<long long>(p.n_pages), stack0 + freed));
 
   // ---- refusals and the pages each row takes (from the top of the stack)
   long long taken = 0;
-  int used = 0;  // pages taken by rows that were not refused: this thread's rows
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+  int used = 0;  // pages taken by this thread's rows that were not refused
+  for (int b0 = 0; b0 < p.B; b0 += threads) {
     const int b = b0 + tid;
-    int st = kOk, len0 = 0, n = 0, take = 0, first = 0, len = 0;
+    int st = kOk, len0 = 0, n = 0, take = 0, first = 0;
     if (b < p.B) {
-      len = s_row[b].y;
-      first = s_row[b].x;
-      n = p.new_lens[b];
-      const bool ended = p.done && p.done[b];
+      const int4 r = s_row[b];
+      const int len = r.y;
+      first = r.x;
+      n = s_new[b];
       const bool bad = len < 0 || len > cap;
-      len0 = ended && !bad ? 0 : len;
+      len0 = r.w > 0 ? 0 : len;  // (a row that ended with no page had no token)
       if (bad || n < 0) st = kInvalid;
       else if (static_cast<long long>(len0) + n > cap) st = kTooLong;
       else if (n > 0 && static_cast<long long>(first) + n > p.tokens) st = kNoSlots;
       if (st == kOk) take = up(len0 + n) - up(len0);
     }
-    long long t;
-    const long long off = taken + block_scan(take, s_sum, t);
-    taken += t;
+    Two t;
+    const Two off = block_scan({take, 0}, s_sum[turn], t);
+    turn = turn == 2 ? 0 : turn + 1;
     if (b < p.B) {
-      if (take > 0 && off + take > avail) st = kNoPages;
+      const long long at = taken + off.a;
+      if (take > 0 && at + take > avail) st = kNoPages;
       if (st != kOk) take = 0;
       used += take;
-      s_row[b] = make_int4(first, st == kOk ? len0 : -1, sat(off), st == kOk ? up(len0) : 0);
+      s_row[b] = make_int4(first, st == kOk ? len0 : -1, sat(at), st == kOk ? up(len0) : 0);
       if (rank == 0) p.status[b] = st;
     }
+    taken += t.a;
   }
-  long long total_used;
-  block_scan(used, s_sum, total_used);
+  if (used) atomicAdd(&s_used, used);
   if constexpr (CLUSTER) cluster_sync();  // stack written, lengths and stack size read by every CTA
   else __syncthreads();
 
   // ---- the taken pages into the tables, new lengths
-  for (int b = gw; b < p.B; b += warps) {
-    const int4 r = s_row[b];
-    if (r.y < 0) continue;
-    const int n = p.new_lens[b];
-    const int take = up(r.y + n) - r.w;
-    for (int i = lane; i < take; i += 32) p.table[b * p.ld + r.w + i] = __ldcg(p.free_pages + avail - 1 - r.z - i);
+  const int* top = p.free_pages + avail - 1;
+  for (int b0 = gw; b0 < p.B; b0 += warps * 32) {
+    // rows that take one page, as most do in a decode step: a lane each; the others one after the other
+    const int mine = b0 + lane * warps;
+    int take = 0;
+    if (mine < p.B) {
+      const int4 r = s_row[mine];
+      if (r.y >= 0) take = up(r.y + s_new[mine]) - r.w;
+      if (take == 1) p.table[mine * p.ld + r.w] = __ldcg(top - r.z);
+    }
+    uint32_t m = __ballot_sync(0xffffffffu, take > 1);
+    for (; m; m &= m - 1) {
+      const int src = __ffs(m) - 1, b = b0 + src * warps, n = __shfl_sync(0xffffffffu, take, src);
+      const int4 r = s_row[b];
+      move_pages(p.table + b * p.ld + r.w, top - r.z, n, -1);
+    }
   }
   if (rank == 0) {
-    for (int b = tid; b < p.B; b += kThreads) {
+    for (int b = tid; b < p.B; b += threads) {
       const int4 r = s_row[b];
-      const int len = r.y >= 0 ? r.y + p.new_lens[b] : 0;
-      if (r.y >= 0) p.lens_out[b] = len;
-      else {  // refused: a row that ended still gave its pages back
+      if (r.y >= 0) {
+        p.lens_out[b] = r.y + s_new[b];
+      } else {  // refused: a row that ended still gave its pages back
         const int old = p.lens[b];
         p.lens_out[b] = (p.done && p.done[b] && old >= 0 && old <= cap) ? 0 : old;
       }
     }
-    if (tid == 0) *p.n_free_out = avail - static_cast<int>(total_used);
+    if (tid == 0) *p.n_free_out = avail - s_used;
   }
 
-  // ---- slots
-  for (int t = rank * kThreads + tid; t < p.tokens; t += nctas * kThreads) {
-    int slot = -1, pos = -1;
+  // ---- slots, four tokens a thread
+  const bool vec = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15) == 0;
+  for (int t = 4 * (rank * threads + tid); t < p.tokens; t += 4 * nctas * threads) {
+    int slot[4], pos[4];
+    int lo = 0;
     if (t < tok) {
-      int lo = 0, hi = p.B - 1;  // last row whose first token is not after t
+      int hi = p.B - 1;  // last row whose first token is not after t
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (s_row[mid].x <= t) lo = mid;
         else hi = mid - 1;
       }
-      const int4 r = s_row[lo];
-      if (r.y >= 0) {
-        pos = r.y + t - r.x;
-        const int blk = pos / P;
-        // (pages already held are not rewritten by this call; the others come off the stack)
-        const int page = blk < r.w ? __ldcg(p.table + lo * p.ld + blk)
-                                   : __ldcg(p.free_pages + avail - 1 - r.z - (blk - r.w));
-        slot = (page >= 0 && page < p.n_pages) ? page * P + (pos - blk * P) : -1;
-      }
     }
-    p.slots[t] = slot;
-    p.positions[t] = pos;
+    int4 r = s_row[lo];
+    int next = lo + 1 < p.B ? s_row[lo + 1].x : INT32_MAX;
+    const int* entry[4];  // where a token's page stands: all four before the first is read
+    int off[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      pos[k] = -1;
+      off[k] = 0;
+      entry[k] = nullptr;
+      if (t + k >= tok || t + k >= p.tokens) continue;
+      while (t + k >= next) {
+        r = s_row[++lo];
+        next = lo + 1 < p.B ? s_row[lo + 1].x : INT32_MAX;
+      }
+      if (r.y < 0) continue;
+      pos[k] = r.y + t + k - r.x;
+      const int blk = block_of(pos[k]);
+      off[k] = pos[k] - blk * P;
+      // (pages already held are not rewritten by this call; the others come off the stack)
+      entry[k] = blk < r.w ? p.table + lo * p.ld + blk : top - r.z - (blk - r.w);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) slot[k] = entry[k] ? __ldcg(entry[k]) : -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) slot[k] = slot[k] >= 0 && slot[k] < p.n_pages ? slot[k] * P + off[k] : -1;
+    if (vec && t + 4 <= p.tokens) {
+      *reinterpret_cast<int4*>(p.slots + t) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(p.positions + t) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (t + k < p.tokens) {
+          p.slots[t + k] = slot[k];
+          p.positions[t + k] = pos[k];
+        }
+    }
   }
 }
 
@@ -280,16 +359,19 @@ extern "C" int nl_update_block_tables(const nl_update_block_tables_args* args, c
       !a.cu || !a.status || (n_tokens > 0 && (!a.slots || !a.positions)))
     return NL_ERR_SHAPE;
   pc::TableParams p{a.block_table, a.table_ld, a.lens, a.new_lens, a.done, a.free_pages, a.n_free, a.lens_out,
-                    a.n_free_out, a.slots, a.positions, a.cu, a.status, B, a.max_blocks, a.page_size, a.n_pages,
-                    n_tokens};
-  const size_t smem = static_cast<size_t>(B) * sizeof(int4);
+                    a.n_free_out, a.slots, a.positions, a.cu, a.status, B, a.max_blocks, a.page_size,
+                    (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctz(a.page_size) : -1, a.n_pages, n_tokens};
+  const size_t smem = static_cast<size_t>(B) * (sizeof(int4) + sizeof(int));
+  // one CTA of as many threads as rows or fours of tokens need; a cluster of 8 for long lists
   const bool wide = n_tokens > 4 * pc::kThreads;
+  const int need = B > n_tokens / 4 ? B : n_tokens / 4;
+  const int threads = wide ? pc::kThreads : need >= pc::kThreads ? pc::kThreads : need <= 128 ? 128 : (need + 31) / 32 * 32;
   auto kern = wide ? pc::update_tables_kernel<true> : pc::update_tables_kernel<false>;
   if (smem > 40 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return NL_ERR_LAUNCH;
   const int ctas = wide ? 8 : 1;
-  launch_kernel(kern, dim3(ctas), dim3(pc::kThreads), smem, stream, ctas, p);
+  launch_kernel(kern, dim3(ctas), dim3(threads), smem, stream, ctas, p);
   return launch_status();
 }
 

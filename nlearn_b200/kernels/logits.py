@@ -8,8 +8,8 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import ARGS, BF16, F32, check, lib, raw_stream
-from ..paged import _ints1, _ints2, _no_grad, _on, _refuse_place
+from .._lib import BF16, F32
+from ..paged import _ints1, _ints2, _launch, _no_grad, _refuse_place
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
 
@@ -113,11 +113,8 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
         raise ValueError("mask_rows come with mask")
     if B == 0:
         return out
-    with _on(index):
-        check(lib.nl_process_logits(
-            ARGS["nl_process_logits"].pack(logits.data_ptr(), out.data_ptr(), tp, lp, pp, rp, fp, ap, ip, bp, mp, mr,
-                                           max(ldx, V), max(ldy, V), tl, ldb, ldm, dt, L, n_bias, n_masks, B, V),
-            raw_stream(index)), "nl_process_logits")
+    _launch("nl_process_logits", index, logits.data_ptr(), out.data_ptr(), tp, lp, pp, rp, fp, ap, ip, bp, mp, mr,
+            max(ldx, V), max(ldy, V), tl, ldb, ldm, dt, L, n_bias, n_masks, B, V)
     return out
 
 

@@ -23,7 +23,6 @@ and have no backward.  The reference has no counterpart (nlearn/model.py:
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -46,9 +45,17 @@ def _refuse_place(name: str, t: torch.Tensor, index: int) -> None:
     raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
 
 
-def _on(index: int):
-    """Context in which device `index` is current (entry points launch on the current device)."""
-    return nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+def _launch(name: str, index: int, *fields) -> None:
+    """Calls a C entry point with its packed arguments on the current stream of
+    device `index`, which entry points take to be the current device."""
+    args = ARGS[name].pack(*fields)
+    if index == torch._C._cuda_getDevice():
+        status = getattr(lib, name)(args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = getattr(lib, name)(args, raw_stream(index))
+    if status:
+        check(status, name)
 
 
 def _ints1(name: str, t: torch.Tensor, n: int, index: int) -> int:
@@ -138,8 +145,9 @@ def _scale(name: str, t, heads: int, dt: int, index: int) -> int:
 
 @lru_cache(maxsize=256)
 def _workspace_bytes(index: int, *shape) -> int:
-    """nl_paged_attention_workspace_bytes of a shape on the (current) device `index`."""
-    return lib.nl_paged_attention_workspace_bytes(*shape)
+    """nl_paged_attention_workspace_bytes of a shape on device `index`."""
+    with torch.cuda.device(index):
+        return lib.nl_paged_attention_workspace_bytes(*shape)
 
 
 def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -207,15 +215,12 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         return out
     if blocks == 0 or n_pages == 0 or page == 0:
         raise ValueError("block_table and caches must hold at least one page")
-    with _on(index):
-        nb = _workspace_bytes(index, B, Hq, Hk, d, page, blocks, dt)
-        ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
-        check(lib.nl_paged_attention(
-            ARGS["nl_paged_attention"].pack(
-                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lens_p, kn, vn, ks, vs,
-                out.data_ptr(), lp, ws.data_ptr() if nb else 0, q_b, q_h, page_s, head_s, tok_s, table_ld, n_b, n_h,
-                o_b, o_h, ls, nb, B, Hq, Hk, d, page, blocks, n_pages, dt, d ** -0.5 if scale is None else scale),
-            raw_stream(index)), "nl_paged_attention")
+    nb = _workspace_bytes(index, B, Hq, Hk, d, page, blocks, dt)
+    ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
+    _launch("nl_paged_attention", index, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+            lens_p, kn, vn, ks, vs, out.data_ptr(), lp, ws.data_ptr() if nb else 0, q_b, q_h, page_s, head_s, tok_s,
+            table_ld, n_b, n_h, o_b, o_h, ls, nb, B, Hq, Hk, d, page, blocks, n_pages, dt,
+            d ** -0.5 if scale is None else scale)
     return out
 
 
@@ -246,11 +251,8 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     vs = _scale("v_scale", v_scale, Hk, dt, index)
     if T == 0 or k_cache.numel() == 0:
         return
-    with _on(index):
-        check(lib.nl_paged_kv_write(
-            ARGS["nl_paged_kv_write"].pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), sp, ks,
-                                           vs, kst[0], kst[1], page_s, head_s, tok_s, T, Hk, d, page, n_pages, dt),
-            raw_stream(index)), "nl_paged_kv_write")
+    _launch("nl_paged_kv_write", index, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), sp, ks, vs,
+            kst[0], kst[1], page_s, head_s, tok_s, T, Hk, d, page, n_pages, dt)
 
 
 class BlockPlan(NamedTuple):
@@ -300,17 +302,19 @@ def update_block_tables(block_table: torch.Tensor, lens: torch.Tensor, new_lens:
     free_p, nf_p = _ints1("free_pages", free_pages, n_pages, index), _ints1("n_free", n_free, 1, index)
     if lens_out is None:
         lens_out = torch.empty_like(lens)
+        lo_p = lens_out.data_ptr()
+    else:
+        lo_p = _ints1("lens_out", lens_out, B, index)
     if n_free_out is None:
         n_free_out = torch.empty_like(n_free)
-    lo_p, nfo_p = _ints1("lens_out", lens_out, B, index), _ints1("n_free_out", n_free_out, 1, index)
+        nfo_p = n_free_out.data_ptr()
+    else:
+        nfo_p = _ints1("n_free_out", n_free_out, 1, index)
     status = torch.empty_like(lens)
     slots, positions, cu = lens.new_empty(n_tokens), lens.new_empty(n_tokens), lens.new_empty(B + 1)
-    with _on(index):
-        check(lib.nl_update_block_tables(
-            ARGS["nl_update_block_tables"].pack(block_table.data_ptr(), lens_p, new_p, done_p, free_p, nf_p, lo_p,
-                                                nfo_p, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
-                                                status.data_ptr(), table_ld, B, blocks, page_size, n_pages, n_tokens),
-            raw_stream(index)), "nl_update_block_tables")
+    _launch("nl_update_block_tables", index, block_table.data_ptr(), lens_p, new_p, done_p, free_p, nf_p, lo_p, nfo_p,
+            slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), status.data_ptr(), table_ld, B, blocks, page_size,
+            n_pages, n_tokens)
     return BlockPlan(slots, positions, cu, lens_out, n_free_out, status)
 
 
