@@ -304,6 +304,17 @@ NL_API int nl_decode_attention(const void* qkv_new, void* cache, void* o, const 
 NL_API int nl_sample_tokens(const float* logits, long long ldl, int V, float temperature, unsigned long long seed,
                             const int* pos, int* tok, int* out, long long ldo, int B, cudaStream_t stream);
 NL_API int nl_decode_advance(int* pos, cudaStream_t stream);
+/* The embedding and the sampler for rows that are at positions of their own:
+ * lens[b] (int32) counts row b's tokens, tok[b] the last of them, so its position is
+ * lens[b] - 1.  A row with lens 0 is idle: x[b] = 0, and no token is drawn or
+ * written.  A position outside wpe's max_pos rows or a token outside [0, V) gives
+ * a zero row and sets device error 3.  The sampler's random bits are those
+ * of nl_sample_tokens at (seed, lens[b] - 1, b); out[b, lens[b]] = tok[b]. */
+NL_API int nl_decode_embed_rows(const int* tok, const int* lens, const void* wte, const void* wpe, void* x, int B,
+                                int D, int max_pos, int V, cudaStream_t stream);
+NL_API int nl_sample_tokens_rows(const float* logits, long long ldl, int V, float temperature,
+                                 unsigned long long seed, const int* lens, int* tok, int* out, long long ldo, int B,
+                                 cudaStream_t stream);
 /* C[M, N] = LayerNorm(x)[M, K] . W[K, N] with the nl_gemm_ex epilogues
  * (STORE / ACCUM / BIAS / BIAS_GELU / RESID), the LayerNorm (gamma, beta over
  * K, eps) applied while the small-M kernel stages x; M <= 8, x and W

@@ -65,6 +65,9 @@ SIGNATURES: dict[str, list] = {
     "nl_sample_tokens": [c_void_p, c_longlong, c_int, c_float, c_ulonglong, c_void_p, c_void_p, c_void_p,
                          c_longlong, c_int, c_void_p],
     "nl_decode_advance": [c_void_p, c_void_p],
+    "nl_decode_embed_rows": [c_void_p] * 5 + [c_int] * 4 + [c_void_p],
+    "nl_sample_tokens_rows": [c_void_p, c_longlong, c_int, c_float, c_ulonglong, c_void_p, c_void_p, c_void_p,
+                              c_longlong, c_int, c_void_p],
     "nl_linear_ln_small": [c_void_p, c_longlong, c_void_p, c_void_p, c_float, c_void_p, c_longlong, c_void_p,
                            c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "nl_paged_attention_workspace_bytes": [c_int] * 7,

@@ -40,13 +40,22 @@ constexpr int HD = 64;
 constexpr int kChunk = 256;   // positions per split
 constexpr int kThreads = 128;
 
+// ROWS: each row has a position of its own, pos[b] - 1 (pos counts the row's
+// tokens, 0: the row is idle and gets zeros); otherwise all rows share *pos.
+template <bool ROWS>
 __global__ void decode_embed_kernel(const int* __restrict__ tok, const int* __restrict__ pos,
                                     const __nv_bfloat16* __restrict__ wte, const __nv_bfloat16* __restrict__ wpe,
-                                    __nv_bfloat16* __restrict__ x, int B, int D) {
+                                    __nv_bfloat16* __restrict__ x, int B, int D, int max_pos, int V, int* err) {
   griddep_sync();
   const int b = blockIdx.x;
   if (b >= B) return;
-  const int t = *pos;
+  const int t = ROWS ? pos[b] - 1 : *pos;
+  if (ROWS && (t < 0 || t >= max_pos || tok[b] < 0 || tok[b] >= V)) {
+    if (t >= 0 && threadIdx.x == 0 && err) atomicExch(err, 3);
+    for (int i = threadIdx.x; i < D; i += blockDim.x)
+      x[static_cast<long long>(b) * D + i] = __float2bfloat16_rn(0.f);
+    return;
+  }
   const __nv_bfloat16* e = wte + static_cast<long long>(tok[b]) * D;
   const __nv_bfloat16* p = wpe + static_cast<long long>(t) * D;
   for (int i = threadIdx.x; i < D; i += blockDim.x)
@@ -201,7 +210,9 @@ __host__ __device__ __forceinline__ uint64_t mix64(uint64_t z) {
   return z ^ (z >> 31);
 }
 
-// One CTA per row: argmax over the vocabulary of logit/T + Gumbel noise.
+// One CTA per row: argmax over the vocabulary of logit/T + Gumbel noise.  ROWS as
+// in decode_embed_kernel: row b is at position pos[b] - 1, idle rows keep their token.
+template <bool ROWS>
 __global__ void __launch_bounds__(1024) sample_kernel(const float* __restrict__ logits, long long ldl, int V,
                                                      float inv_temp, int greedy, unsigned long long seed,
                                                      const int* __restrict__ pos, int* __restrict__ tok,
@@ -210,7 +221,8 @@ __global__ void __launch_bounds__(1024) sample_kernel(const float* __restrict__ 
   __shared__ float bv[32];
   __shared__ int bi[32];
   const int b = blockIdx.x;
-  const int t = *pos;
+  const int t = ROWS ? pos[b] - 1 : *pos;
+  if (ROWS && t < 0) return;
   const float* row = logits + b * ldl;
   const uint64_t key = mix64(seed ^ mix64((static_cast<uint64_t>(t) << 32) ^ static_cast<uint64_t>(b)));
   float best = -INFINITY;
@@ -278,9 +290,18 @@ using namespace nl;
 extern "C" int nl_decode_embed(const int* tok, const int* pos, const void* wte, const void* wpe, void* x, int B,
                                int D, cudaStream_t stream) {
   if (B <= 0 || D <= 0 || !tok || !pos) return NL_ERR_SHAPE;
-  launch_kernel(dec::decode_embed_kernel, dim3(B), dim3(256), 0, stream, 1, tok, pos,
+  launch_kernel(dec::decode_embed_kernel<false>, dim3(B), dim3(256), 0, stream, 1, tok, pos,
                 static_cast<const __nv_bfloat16*>(wte), static_cast<const __nv_bfloat16*>(wpe),
-                static_cast<__nv_bfloat16*>(x), B, D);
+                static_cast<__nv_bfloat16*>(x), B, D, 0, 0, device_error_word());
+  return launch_status();
+}
+
+extern "C" int nl_decode_embed_rows(const int* tok, const int* lens, const void* wte, const void* wpe, void* x,
+                                    int B, int D, int max_pos, int V, cudaStream_t stream) {
+  if (B <= 0 || D <= 0 || max_pos <= 0 || V <= 0 || !tok || !lens || !wte || !wpe || !x) return NL_ERR_SHAPE;
+  launch_kernel(dec::decode_embed_kernel<true>, dim3(B), dim3(256), 0, stream, 1, tok, lens,
+                static_cast<const __nv_bfloat16*>(wte), static_cast<const __nv_bfloat16*>(wpe),
+                static_cast<__nv_bfloat16*>(x), B, D, max_pos, V, device_error_word());
   return launch_status();
 }
 
@@ -322,8 +343,18 @@ extern "C" int nl_sample_tokens(const float* logits, long long ldl, int V, float
                                 cudaStream_t stream) {
   if (B <= 0 || V <= 0 || ldl < V || !pos || !tok) return NL_ERR_SHAPE;
   const int greedy = temperature <= 0.f;
-  launch_kernel(dec::sample_kernel, dim3(B), dim3(1024), 0, stream, 1, logits, ldl, V,
+  launch_kernel(dec::sample_kernel<false>, dim3(B), dim3(1024), 0, stream, 1, logits, ldl, V,
                 greedy ? 1.f : 1.f / temperature, greedy, seed, pos, tok, out, ldo, device_error_word());
+  return launch_status();
+}
+
+extern "C" int nl_sample_tokens_rows(const float* logits, long long ldl, int V, float temperature,
+                                     unsigned long long seed, const int* lens, int* tok, int* out, long long ldo,
+                                     int B, cudaStream_t stream) {
+  if (B <= 0 || V <= 0 || ldl < V || !logits || !lens || !tok) return NL_ERR_SHAPE;
+  const int greedy = temperature <= 0.f;
+  launch_kernel(dec::sample_kernel<true>, dim3(B), dim3(1024), 0, stream, 1, logits, ldl, V,
+                greedy ? 1.f : 1.f / temperature, greedy, seed, lens, tok, out, ldo, device_error_word());
   return launch_status();
 }
 

@@ -18,7 +18,10 @@ rows are kept as the KV cache, and each further token is one decode step:
 LayerNorm while staging its A operand).
 
 The position lives in device memory, so one decode step is captured into a
-CUDA graph once and replayed per token.  The random stream (seed, position,
+CUDA graph once and replayed per token.  ``Decoder`` does this for a batch of
+prompts of one length; ``PagedDecoder`` for rows that come and go with prompts
+of any lengths, over a paged cache (``nlearn_b200.paged``), with penalties,
+biases and masks on the logits (``nlearn_b200.kernels.logits``).  The random stream (seed, position,
 row) is this library's own counter-based one (the reference's JAX PRNG key is
 replaced by an integer seed).
 """
@@ -30,14 +33,15 @@ import torch
 from . import _lib
 from ._lib import check, lib, ptr, stream_handle
 from .kernels.gemm import gemm_ex
+from .kernels.logits import process_logits
 from .model import FlatParams, GPTConfig
+from .paged import paged_decode_attention, paged_kv_write, update_block_tables
 
 
-class Decoder:
-    """Static buffers, KV caches and the captured decode step for one batch
-    size; ``generate`` may be called repeatedly."""
+class _DecodeStep:
+    """Static buffers of one decode step of `batch` rows and its layers around the attention."""
 
-    def __init__(self, params: FlatParams, cfg: GPTConfig, batch: int = 1, max_len: int | None = None):
+    def __init__(self, params: FlatParams, cfg: GPTConfig, batch: int, max_len: int | None):
         self.P, self.cfg, self.B = params, cfg, batch
         self.S = max_len or cfg.max_seq
         if self.S > cfg.max_seq:
@@ -45,9 +49,7 @@ class Decoder:
         B, D, F, Vp = batch, cfg.d_model, cfg.d_ff, cfg.vocab_padded
         dev = params.device
         bf = dict(device=dev, dtype=torch.bfloat16)
-        self.cache = [torch.zeros(B, self.S, 3 * D, **bf) for _ in range(cfg.n_layers)]
         self.tok = torch.zeros(B, device=dev, dtype=torch.int32)
-        self.pos = torch.zeros(1, device=dev, dtype=torch.int32)
         self.out = torch.zeros(B, self.S + 1, device=dev, dtype=torch.int32)
         self.x, self.x2, self.x3, self.h, self.o = (torch.empty(B, D, **bf) for _ in range(5))
         self.qkv = torch.empty(B, 3 * D, **bf)
@@ -55,19 +57,65 @@ class Decoder:
         self.mean = torch.empty(B, device=dev, dtype=torch.float32)
         self.rstd = torch.empty_like(self.mean)
         self.logits = torch.empty(B, Vp, device=dev, dtype=torch.float32)
-        nbytes = lib.nl_decode_workspace_bytes(B, cfg.n_heads, self.S)
-        self.ws = torch.zeros(nbytes, device=dev, dtype=torch.uint8)
-        self._graph = None
-        self._graph_key = None
         self._fuse_ln = True  # LayerNorm folded into the small-M GEMM (batch <= 8)
 
-    # ------------------------------------------------------------------ pieces
+    def _layers(self, attention):
+        """From the embedded rows in ``x`` to the logits; ``attention(layer)``
+        turns ``qkv`` into ``o``."""
+        cfg, P = self.cfg, self.P
+        x = self.x
+        for layer in range(cfg.n_layers):
+            pre = f"blocks.{layer}."
+            self._ln_linear(x, P.f(pre + "ln1.g"), P.f(pre + "ln1.b"), P.p(pre + "wqkv"), self.qkv)
+            attention(layer)
+            gemm_ex(self.o, P.p(pre + "wo"), out=self.x2, epilogue=_lib.EPI_RESID, resid=x)
+            self._ln_linear(self.x2, P.f(pre + "ln2.g"), P.f(pre + "ln2.b"), P.p(pre + "w1"), self.u,
+                            epilogue=_lib.EPI_BIAS_GELU, bias=P.f(pre + "b1"), aux=self.a)
+            gemm_ex(self.u, P.p(pre + "w2"), out=self.x3, epilogue=_lib.EPI_RESID, bias=P.f(pre + "b2"),
+                    resid=self.x2)
+            x = self.x3
+        V = cfg.vocab
+        self._ln_linear(x, P.f("lnf.g"), P.f("lnf.b"), P.p("head.w")[:, :V], self.logits[:, :V])
+
     def _ln(self, x, y, g, b, M):
         check(lib.nl_layernorm_fwd(ptr(x), ptr(g), ptr(b), ptr(y), ptr(self.mean if M == self.B else
                                                                           torch.empty(M, device=x.device)),
                                    ptr(self.rstd if M == self.B else torch.empty(M, device=x.device)), M,
                                    self.cfg.d_model, self.cfg.ln_eps, stream_handle()), "nl_layernorm_fwd")
 
+    def _ln_linear(self, x, g, b, W, out, epilogue=_lib.EPI_STORE, bias=None, aux=None):
+        """out = LayerNorm(x) . W (+ epilogue): one fused small-M kernel when the
+        shape allows (batch <= 8), else LayerNorm then the GEMM."""
+        if self._fuse_ln:
+            dt = _lib.F32 if out.dtype == torch.float32 else _lib.BF16
+            st = lib.nl_linear_ln_small(ptr(x), x.stride(0), ptr(g), ptr(b), self.cfg.ln_eps, ptr(W), W.stride(0),
+                                        ptr(out), out.stride(0), dt, out.shape[0], out.shape[1], W.shape[0],
+                                        epilogue, ptr(bias), ptr(aux), None, stream_handle())
+            if st == 0:
+                return
+            if st != -1:  # anything but NL_ERR_SHAPE ("not a shape the fused kernel takes") is an error
+                check(st, "nl_linear_ln_small")
+            self._fuse_ln = False
+        self._ln(x, self.h, g, b, self.B)
+        gemm_ex(self.h, W, out=out, epilogue=epilogue, bias=bias, aux=aux)
+
+
+class Decoder(_DecodeStep):
+    """KV caches and the captured decode step for one batch size, all rows at
+    one position; ``generate`` may be called repeatedly."""
+
+    def __init__(self, params: FlatParams, cfg: GPTConfig, batch: int = 1, max_len: int | None = None):
+        super().__init__(params, cfg, batch, max_len)
+        dev = params.device
+        self.cache = [torch.zeros(batch, self.S, 3 * cfg.d_model, device=dev, dtype=torch.bfloat16)
+                      for _ in range(cfg.n_layers)]
+        self.pos = torch.zeros(1, device=dev, dtype=torch.int32)
+        nbytes = lib.nl_decode_workspace_bytes(batch, cfg.n_heads, self.S)
+        self.ws = torch.zeros(nbytes, device=dev, dtype=torch.uint8)
+        self._graph = None
+        self._graph_key = None
+
+    # ------------------------------------------------------------------ pieces
     def _head_and_sample(self, hf_rows, seed: int, temperature: float):
         V = self.cfg.vocab
         gemm_ex(hf_rows, self.P.p("head.w")[:, :V], out=self.logits[:, :V])
@@ -116,42 +164,17 @@ class Decoder:
         self.pos.fill_(Pl - 1)
         self._head_and_sample(h.view(B, Pl, D)[:, -1], seed, temperature)
 
-    def _ln_linear(self, x, g, b, W, out, epilogue=_lib.EPI_STORE, bias=None, aux=None):
-        """out = LayerNorm(x) . W (+ epilogue): one fused small-M kernel when the
-        shape allows (batch <= 8), else LayerNorm then the GEMM."""
-        if self._fuse_ln:
-            dt = _lib.F32 if out.dtype == torch.float32 else _lib.BF16
-            st = lib.nl_linear_ln_small(ptr(x), x.stride(0), ptr(g), ptr(b), self.cfg.ln_eps, ptr(W), W.stride(0),
-                                        ptr(out), out.stride(0), dt, out.shape[0], out.shape[1], W.shape[0],
-                                        epilogue, ptr(bias), ptr(aux), None, stream_handle())
-            if st == 0:
-                return
-            if st != -1:  # anything but NL_ERR_SHAPE ("not a shape the fused kernel takes") is an error
-                check(st, "nl_linear_ln_small")
-            self._fuse_ln = False
-        self._ln(x, self.h, g, b, self.B)
-        gemm_ex(self.h, W, out=out, epilogue=epilogue, bias=bias, aux=aux)
+    def _attention(self, layer: int):
+        check(lib.nl_decode_attention(ptr(self.qkv), ptr(self.cache[layer]), ptr(self.o), ptr(self.pos), ptr(self.ws),
+                                      self.ws.numel(), self.B, self.cfg.n_heads, self.S, 64, stream_handle()),
+              "nl_decode_attention")
 
     def step(self, seed: int, temperature: float):
         """One decode step: the token in ``tok`` at position ``pos``."""
-        cfg, P = self.cfg, self.P
-        D, H, V = cfg.d_model, cfg.n_heads, cfg.vocab
+        P = self.P
         check(lib.nl_decode_embed(ptr(self.tok), ptr(self.pos), ptr(P.p("wte")), ptr(P.p("wpe")), ptr(self.x),
-                                  self.B, D, stream_handle()), "nl_decode_embed")
-        x = self.x
-        for layer in range(cfg.n_layers):
-            pre = f"blocks.{layer}."
-            self._ln_linear(x, P.f(pre + "ln1.g"), P.f(pre + "ln1.b"), P.p(pre + "wqkv"), self.qkv)
-            check(lib.nl_decode_attention(ptr(self.qkv), ptr(self.cache[layer]), ptr(self.o), ptr(self.pos),
-                                          ptr(self.ws), self.ws.numel(), self.B, H, self.S, 64, stream_handle()),
-                  "nl_decode_attention")
-            gemm_ex(self.o, P.p(pre + "wo"), out=self.x2, epilogue=_lib.EPI_RESID, resid=x)
-            self._ln_linear(self.x2, P.f(pre + "ln2.g"), P.f(pre + "ln2.b"), P.p(pre + "w1"), self.u,
-                            epilogue=_lib.EPI_BIAS_GELU, bias=P.f(pre + "b1"), aux=self.a)
-            gemm_ex(self.u, P.p(pre + "w2"), out=self.x3, epilogue=_lib.EPI_RESID, bias=P.f(pre + "b2"),
-                    resid=self.x2)
-            x = self.x3
-        self._ln_linear(x, P.f("lnf.g"), P.f("lnf.b"), P.p("head.w")[:, :V], self.logits[:, :V])
+                                  self.B, self.cfg.d_model, stream_handle()), "nl_decode_embed")
+        self._layers(self._attention)
         self._sample(seed, temperature)
 
     def capture(self, seed: int, temperature: float):
@@ -187,12 +210,299 @@ class Decoder:
         return self.out[:, :Pl + n_tokens].cpu().numpy()
 
 
-def generate(trainer_or_params, prompt_ids, n_tokens: int, seed: int = 0, temperature: float = 1.0,
-             cfg: GPTConfig | None = None) -> np.ndarray:
+class PagedDecoder(_DecodeStep):
+    """Generation for rows that come and go, each with a prompt, a length and
+    rules of its own, over a paged KV cache.
+
+    ``add`` admits a prompt to a free row, ``step`` draws a token for every row
+    in use (one captured CUDA graph), ``tokens`` reads a row, ``release`` gives its
+    pages back; ``generate`` runs any number of prompts through the rows.  A
+    step whose rows all fit is never refused: the host keeps count of the pages.
+
+    cache_dtype bfloat16, or float8_e4m3fn (half the bytes; keys and values
+    are stored as they are, scale 1).
+    """
+
+    def __init__(self, params: FlatParams, cfg: GPTConfig, max_batch: int = 8, n_pages: int | None = None,
+                 page_size: int = 16, max_len: int | None = None, max_bias: int = 32, seed: int = 0,
+                 temperature: float = 1.0, cache_dtype=torch.bfloat16):
+        super().__init__(params, cfg, max_batch, max_len)
+        R, H, dev = max_batch, cfg.n_heads, params.device
+        if page_size < 1 or max_bias < 0 or max_batch < 1:
+            raise ValueError(f"page_size {page_size}, max_bias {max_bias}, max_batch {max_batch}: out of range")
+        self.page_size, self.seed, self.temperature = page_size, int(seed), float(temperature)
+        self.blocks = -(-self.S // page_size)
+        self.n_pages = n_pages or R * self.blocks
+        i32, f32 = dict(device=dev, dtype=torch.int32), dict(device=dev, dtype=torch.float32)
+        shape = (self.n_pages, H, page_size, 64)
+        self.k_cache, self.v_cache = ([torch.zeros(shape, device=dev, dtype=torch.bfloat16).to(cache_dtype)
+                                       for _ in range(cfg.n_layers)] for _ in range(2))
+        self.block_table = torch.full((R, self.blocks), -1, **i32)
+        self.lens = torch.zeros(R, **i32)          # tokens of a row; its cache holds their keys after a step
+        self.free_pages = torch.arange(self.n_pages, **i32)
+        self.n_free = torch.full((1,), self.n_pages, **i32)
+        self.new = torch.zeros(R, **i32)           # 1: the row is in use
+        self.now = torch.zeros(R, **i32)           # lengths of the rows that draw a token
+        self.prompt_lens = torch.zeros(R, **i32)
+        self.repetition, self.frequency, self.presence = torch.ones(R, **f32), torch.zeros(R, **f32), torch.zeros(R,
+                                                                                                                 **f32)
+        self.bias_ids, self.bias = torch.full((R, max_bias), -1, **i32), torch.zeros(R, max_bias, **f32)
+        self.mask = torch.zeros(R, (cfg.vocab + 31) // 32, **i32)
+        self.mask_rows = torch.full((R,), -1, **i32)
+        self._len = [0] * R                        # host's copy of the lengths
+        self._rules = [frozenset()] * R
+        self._graphs = {}
+
+    # ------------------------------------------------------------------ pieces
+    def _pages(self, n: int) -> int:
+        return -(-n // self.page_size)
+
+    def free_rows(self) -> list[int]:
+        return [r for r in range(self.B) if self._len[r] == 0]
+
+    def free_page_count(self) -> int:
+        # (a row's last token has no key in the cache until the next step)
+        return self.n_pages - sum(self._pages(n - 1) for n in self._len if n)
+
+    def _attention(self, layer: int):
+        D, H = self.cfg.d_model, self.cfg.n_heads
+        q, k, v = (self.qkv[:, i * D:(i + 1) * D].view(self.B, H, 64) for i in range(3))
+        paged_decode_attention(q, self.k_cache[layer], self.v_cache[layer], self.block_table, self.lens, k, v,
+                               out=self.o.view(self.B, H, 64))
+
+    def _draw(self, lens, rules):
+        """Rules, then a token for every row with lens > 0 (its tokens so far)."""
+        V = self.cfg.vocab
+        kw = {}
+        if "penalties" in rules:
+            kw.update(tokens=self.out, lens=lens, prompt_lens=self.prompt_lens, repetition=self.repetition,
+                      frequency=self.frequency, presence=self.presence)
+        if "bias" in rules:
+            kw.update(bias_ids=self.bias_ids, bias=self.bias)
+        if "mask" in rules:
+            kw.update(mask=self.mask, mask_rows=self.mask_rows)
+        if kw:
+            process_logits(self.logits[:, :V], out=self.logits[:, :V], **kw)
+        check(lib.nl_sample_tokens_rows(ptr(self.logits), self.logits.stride(0), V, self.temperature, self.seed,
+                                        ptr(lens), ptr(self.tok), ptr(self.out), self.out.stride(0), self.B,
+                                        stream_handle()), "nl_sample_tokens_rows")
+
+    def _embed(self, tok, lens, x):
+        P, cfg = self.P, self.cfg
+        check(lib.nl_decode_embed_rows(ptr(tok), ptr(lens), ptr(P.p("wte")), ptr(P.p("wpe")), ptr(x), tok.numel(),
+                                       cfg.d_model, self.S, cfg.vocab, stream_handle()), "nl_decode_embed_rows")
+
+    def _step(self, rules):
+        update_block_tables(self.block_table, self.lens, self.new, self.free_pages, self.n_free, self.page_size,
+                            self.B, lens_out=self.lens, n_free_out=self.n_free)
+        self._embed(self.tok, self.lens, self.x)
+        self._layers(self._attention)
+        self._draw(self.lens, rules)
+
+    def _set_rules(self, row, repetition, frequency, presence, bias, allowed):
+        rules = set()
+        if repetition != 1.0 or frequency != 0.0 or presence != 0.0:
+            rules.add("penalties")
+        self.repetition[row], self.frequency[row], self.presence[row] = repetition, frequency, presence
+        self.bias_ids[row] = -1
+        if bias:
+            ids = list(bias)
+            if len(ids) > self.bias_ids.shape[1]:
+                raise ValueError(f"{len(ids)} biases, over max_bias {self.bias_ids.shape[1]}")
+            self.bias_ids[row, :len(ids)] = torch.tensor(ids, dtype=torch.int32)
+            self.bias[row, :len(ids)] = torch.tensor([float(bias[i]) for i in ids])
+            rules.add("bias")
+        self.set_allowed(row, allowed)
+        if allowed is not None:
+            rules.add("mask")
+        self._rules[row] = frozenset(rules)
+
+    # ------------------------------------------------------------------ API
+    def set_allowed(self, row: int, allowed) -> None:
+        """Token ids that row may draw from now on (None: all; a grammar calls this between steps)."""
+        if allowed is None:
+            self.mask_rows[row] = -1
+            self._rules[row] = self._rules[row] - {"mask"}
+            return
+        ids = np.asarray(list(allowed), np.int64)
+        if ids.size and (ids.min() < 0 or ids.max() >= self.cfg.vocab):
+            raise ValueError("allowed token ids outside the vocabulary")
+        words = np.zeros(self.mask.shape[1], np.uint32)
+        np.bitwise_or.at(words, ids // 32, np.uint32(1) << (ids % 32).astype(np.uint32))
+        self.mask[row] = torch.from_numpy(words.view(np.int32)).to(self.mask.device)
+        self.mask_rows[row] = row
+        self._rules[row] = self._rules[row] | {"mask"}
+
+    def add(self, prompts, *, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
+            bias: dict | None = None, allowed=None) -> list[int]:
+        """Admit prompts (a list of 1-D id arrays) to free rows, run them and
+        draw the first token of each; -> the rows.  The rules (see
+        ``process_logits``) hold for all of them; ``allowed`` is a set of token ids."""
+        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        rows = self.free_rows()[:len(prompts)]
+        if len(rows) < len(prompts):
+            raise RuntimeError(f"{len(prompts)} prompts, {len(rows)} free rows")
+        sizes = [p.size for p in prompts]
+        if any(n < 1 or n >= self.S for n in sizes):
+            raise ValueError(f"prompt lengths {sizes}: must be 1 to {self.S - 1}")
+        if sum(self._pages(n) for n in sizes) > self.free_page_count():
+            raise RuntimeError(f"prompts need {sum(self._pages(n) for n in sizes)} pages, {self.free_page_count()} free")
+        if not rows:
+            return rows
+        cfg, P, D, H, F = self.cfg, self.P, self.cfg.d_model, self.cfg.n_heads, self.cfg.d_ff
+        dev, T = self.P.device, sum(sizes)
+        # the flat list holds the prompts in the order of their rows, which is ascending
+        flat = torch.from_numpy(np.concatenate(prompts)).to(dev)
+        for row in rows:
+            self._set_rules(row, repetition, frequency, presence, bias, allowed)
+        grow = torch.zeros(self.B, dtype=torch.int32)
+        grow[rows] = torch.tensor(sizes, dtype=torch.int32)
+        grow = grow.to(dev)
+        plan = update_block_tables(self.block_table, self.lens, grow, self.free_pages, self.n_free, self.page_size, T,
+                                   lens_out=self.lens, n_free_out=self.n_free)
+        at = [sum(sizes[:i]) for i in range(len(sizes))]
+        for row, a, n in zip(rows, at, sizes):
+            self.out[row, :n] = flat[a:a + n]
+            self.prompt_lens[row] = n
+            self._len[row] = n
+        x = torch.empty(T, D, device=dev, dtype=torch.bfloat16)
+        self._embed(flat, plan.positions + 1, x)
+        h, o = torch.empty_like(x), torch.empty_like(x)
+        L = torch.empty(H, max(sizes), device=dev, dtype=torch.float32)
+        for layer in range(cfg.n_layers):
+            pre = f"blocks.{layer}."
+            self._ln(x, h, P.f(pre + "ln1.g"), P.f(pre + "ln1.b"), T)
+            qkv = gemm_ex(h, P.p(pre + "wqkv"), out_dtype=torch.bfloat16)
+            q, k, v = (qkv[:, i * D:(i + 1) * D] for i in range(3))
+            paged_kv_write(k.view(T, H, 64), v.view(T, H, 64), self.k_cache[layer], self.v_cache[layer], plan.slots)
+            for a, n in zip(at, sizes):  # (kernels on one stream: L may serve all)
+                check(lib.nl_flash_attention_fwd_strided(ptr(q[a:]), ptr(k[a:]), ptr(v[a:]), 3 * D, 64, n * 3 * D,
+                                                         ptr(o[a:]), D, 64, n * D, ptr(L), 1, H, n, 64,
+                                                         stream_handle()), "attn fwd")
+            x2 = gemm_ex(o, P.p(pre + "wo"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_RESID, resid=x)
+            self._ln(x2, h, P.f(pre + "ln2.g"), P.f(pre + "ln2.b"), T)
+            a_ = torch.empty(T, F, device=dev, dtype=torch.bfloat16)
+            u = gemm_ex(h, P.p(pre + "w1"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_BIAS_GELU,
+                        bias=P.f(pre + "b1"), aux=a_)
+            x = gemm_ex(u, P.p(pre + "w2"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_RESID,
+                        bias=P.f(pre + "b2"), resid=x2)
+        last = torch.tensor([a + n - 1 for a, n in zip(at, sizes)], device=dev)
+        where = torch.tensor(rows, device=dev)
+        self.x3.zero_()
+        self.x3[where] = x[last]
+        V = cfg.vocab
+        self._ln_linear(self.x3, P.f("lnf.g"), P.f("lnf.b"), P.p("head.w")[:, :V], self.logits[:, :V])
+        self.now.zero_()
+        self.now[where] = self.lens[where]
+        self._draw(self.now, frozenset().union(*(self._rules[r] for r in rows)))
+        for row in rows:
+            self._len[row] += 1
+            self.new[row] = 1
+        return rows
+
+    def step(self, n: int = 1, use_graph: bool = True) -> None:
+        """Draw n tokens for every row in use."""
+        for _ in range(n):
+            used = [r for r in range(self.B) if self._len[r]]
+            if not used:
+                return
+            if any(self._len[r] > self.S for r in used):
+                raise RuntimeError(f"a row is at its full length of {self.S} tokens: release it")
+            grow = sum(self._pages(self._len[r]) - self._pages(self._len[r] - 1) for r in used)
+            if grow > self.free_page_count():
+                raise RuntimeError(f"the step needs {grow} pages, {self.free_page_count()} free: release a row")
+            rules = frozenset().union(*(self._rules[r] for r in used))
+            if not use_graph:
+                self._step(rules)
+            else:
+                graph = self._graphs.get(rules)
+                if graph is None:
+                    self._step(rules)  # (the first step of a kind runs eagerly: it sets the kernels up)
+                    self._graphs[rules] = False
+                else:
+                    if graph is False:
+                        graph = self._graphs[rules] = torch.cuda.CUDAGraph()
+                        with torch.cuda.graph(graph):
+                            self._step(rules)
+                    graph.replay()
+            for r in used:
+                self._len[r] += 1
+
+    def tokens(self, row: int) -> np.ndarray:
+        """The row's prompt and the tokens drawn so far."""
+        return self.out[row, :self._len[row]].cpu().numpy()
+
+    def release(self, rows) -> None:
+        """End rows: their pages are free, the rows may be admitted anew."""
+        done = torch.zeros(self.B, dtype=torch.int32)
+        for r in rows:
+            if not self._len[r]:
+                raise ValueError(f"row {r} is not in use")
+            done[r] = 1
+        done = done.to(self.P.device)
+        update_block_tables(self.block_table, self.lens, torch.zeros_like(self.new), self.free_pages, self.n_free,
+                            self.page_size, 0, done=done, lens_out=self.lens, n_free_out=self.n_free)
+        for r in rows:
+            self._len[r] = 0
+            self._rules[r] = frozenset()
+            self.new[r] = 0
+            self.mask_rows[r] = -1
+            self.bias_ids[r] = -1
+            self.repetition[r], self.frequency[r], self.presence[r] = 1.0, 0.0, 0.0
+
+    def generate(self, prompts, n_tokens, use_graph: bool = True, **rules) -> list[np.ndarray]:
+        """Prompts of any lengths and number, n_tokens (one number, or one per prompt)
+        drawn for each: as rows and pages come free the next prompts are admitted.
+        Long prompts keep their last ids, as in ``Decoder``."""
+        if any(self._len):
+            raise RuntimeError("generate needs all rows free")
+        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        counts = [int(n) for n in np.broadcast_to(n_tokens, (len(prompts),))]
+        if any(n >= self.S for n in counts):
+            raise ValueError(f"n_tokens {max(counts)} must be below max_len {self.S}")
+        prompts = [p[-(self.S - n):] if n > 0 else p for p, n in zip(prompts, counts)]
+        done: list = [p.copy() if n <= 0 else None for p, n in zip(prompts, counts)]
+        queue = [i for i in range(len(prompts)) if done[i] is None]
+        running: dict[int, int] = {}
+        need = lambda i: self._pages(prompts[i].size + counts[i] - 1)  # noqa: E731  (the last token's key is never kept)
+        for i in queue:
+            if need(i) > self.n_pages:
+                raise ValueError(f"prompt {i} needs {need(i)} pages, the cache has {self.n_pages}")
+        while queue or running:
+            take, held = [], sum(need(i) for i in running.values())
+            for i in queue[:len(self.free_rows())]:
+                if held + need(i) > self.n_pages:
+                    break
+                held += need(i)
+                take.append(i)
+            if take:
+                del queue[:len(take)]
+                running.update(zip(self.add([prompts[i] for i in take], **rules), take))
+            left = {r: prompts[i].size + counts[i] - self._len[r] for r, i in running.items()}
+            if min(left.values()) > 0:
+                self.step(min(left.values()), use_graph)
+            ended = [r for r, n in left.items() if n == min(left.values())]
+            for r in ended:
+                done[running.pop(r)] = self.tokens(r)
+            self.release(ended)
+        return done
+
+
+def generate(trainer_or_params, prompt_ids, n_tokens, seed: int = 0, temperature: float = 1.0,
+             cfg: GPTConfig | None = None, **rules):
     """Reference-shaped entry point: a Trainer (or FlatParams + cfg), a 1-D or
-    [B, P] prompt -> tokens (1-D for a 1-D prompt)."""
+    [B, P] prompt -> tokens (1-D for a 1-D prompt).  A list of prompts of
+    different lengths, an n_tokens per prompt, or any of the rules of
+    ``PagedDecoder.add`` (repetition, frequency, presence, bias, allowed) run on the
+    paged cache; a list of prompts then gives a list of arrays."""
     P = getattr(trainer_or_params, "P", trainer_or_params)
     cfg = cfg or getattr(trainer_or_params, "cfg", None) or P.cfg
+    several = isinstance(prompt_ids, (list, tuple)) and any(np.ndim(p) == 1 for p in prompt_ids)
+    if rules or np.ndim(n_tokens) or (several and len({len(p) for p in prompt_ids}) > 1):
+        prompts = prompt_ids if several or np.ndim(prompt_ids) == 2 else [prompt_ids]
+        dec = PagedDecoder(P, cfg, max_batch=max(1, min(len(prompts), 32)), seed=seed, temperature=temperature)
+        out = dec.generate(prompts, n_tokens, **rules)
+        return out if several or np.ndim(prompt_ids) == 2 else out[0]
     p = np.asarray(prompt_ids, np.int32)
     dec = Decoder(P, cfg, batch=1 if p.ndim == 1 else p.shape[0])
     out = dec.generate(p, n_tokens, seed, temperature)
