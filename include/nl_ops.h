@@ -355,8 +355,7 @@ NL_API int nl_linear_ln_small(const void* x, long long ldx, const float* gamma, 
 NL_API size_t nl_paged_attention_workspace_bytes(int B, int Hq, int Hk, int d, int page_size, int max_blocks,
                                                  int cache_dtype);
 /* The entry points of this and the next section take their arguments in a
- * struct, read before the call returns (a Python caller packs one in a tenth of the time that
- * forty separate arguments take). */
+ * struct, which is read before the call returns. */
 typedef struct {
   const void* q;
   void* k_cache;

@@ -12,7 +12,6 @@ needs it raises, naming the build command.
 from __future__ import annotations
 
 import ctypes
-import struct
 from ctypes import c_float, c_int, c_longlong, c_size_t, c_ulonglong, c_void_p
 from pathlib import Path
 
@@ -94,12 +93,6 @@ _RESTYPE = {"nl_version": ctypes.c_char_p, "nl_launch_count": c_longlong,
             "nl_flash_attention_bwd_noalloc_max_rows": c_longlong, "nl_flash_attention_workspace_bytes": c_size_t, "nl_lce_workspace_bytes": ctypes.c_size_t,
             "nl_decode_workspace_bytes": ctypes.c_size_t, "nl_paged_attention_workspace_bytes": ctypes.c_size_t}
 
-# Argument structs of include/nl_ops.h, packed field by field in their order
-# (P pointer, q long long, N size_t, i int, f float) and passed as bytes.
-ARGS = {"nl_paged_attention": struct.Struct("@12P11qN8if4x"), "nl_paged_kv_write": struct.Struct("@7P5q6i"),
-        "nl_update_block_tables": struct.Struct("@12Pq5i4x"), "nl_process_logits": struct.Struct("@12P5q6i")}
-
-
 class NlError(RuntimeError):
     """A kernel entry point returned a non-zero nl_status."""
 
@@ -123,9 +116,7 @@ class _Lib:
 
     def __getattr__(self, name):
         if name.startswith("nl_"):
-            fn = getattr(self._load(), name)
-            setattr(self, name, fn)  # found at once from now on
-            return fn
+            return getattr(self._load(), name)
         raise AttributeError(name)
 
 
@@ -142,12 +133,6 @@ def stream_handle():
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def raw_stream(device_index: int) -> int:
-    """Handle of the current stream of a device, without a Stream object."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device_index)
-
-
 def ptr(t) -> c_void_p:
     return c_void_p(0 if t is None else t.data_ptr())
 
@@ -162,6 +147,6 @@ def device_error() -> int:
     return lib.nl_get_device_error(stream_handle())
 
 
-__all__ = ["lib", "check", "ptr", "stream_handle", "raw_stream", "ARGS", "device_error", "NlError", "LIB_PATH", "SIGNATURES",
+__all__ = ["lib", "check", "ptr", "stream_handle", "device_error", "NlError", "LIB_PATH", "SIGNATURES",
            "F32", "BF16", "E4M3", "EPI_STORE", "EPI_ACCUM", "EPI_BIAS", "EPI_BIAS_GELU", "EPI_RESID", "EPI_DGELU",
            "c_longlong"]

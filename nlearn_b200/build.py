@@ -3,6 +3,9 @@
 Each ``csrc/*.cu`` is compiled to an object under ``_build/`` (in parallel,
 skipped when up to date) and linked into ``nlearn_b200/libnl_ops.so`` with the
 static CUDA runtime, so the library depends only on the driver at run time.
+``csrc/host/ops_py.cpp``, the host side of the serving operators, is compiled
+with g++ against torch's headers into the extension module
+``nlearn_b200/_ops.so``, which calls the library.
 
     python -m nlearn_b200.build          # or __graft_entry__.build()
 """
@@ -13,12 +16,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 OUT = PKG / "libnl_ops.so"
+EXT_SRC = CSRC / "host" / "ops_py.cpp"
+EXT = PKG / "_ops.so"
 BUILD_DIR = PKG.parent / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -48,6 +54,25 @@ def _compile(nvcc: str, src: Path, obj: Path, dep_mtime: float, verbose: bool) -
     return f"compiled: {src.name}" + (f"\n{r.stderr}" if verbose and r.stderr else "")
 
 
+def _build_ext() -> str:
+    """The extension module (linked against libnl_ops.so, which lies beside it)."""
+    newest = max(EXT_SRC.stat().st_mtime, (INCLUDE / "nl_ops.h").stat().st_mtime)
+    if EXT.exists() and EXT.stat().st_mtime >= newest:
+        return f"up to date: {EXT_SRC.name}"
+    import torch
+    tdir = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parents[1] / "include"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{tdir / 'include'}", f"-I{tdir / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{cuda}",
+           str(EXT_SRC), "-o", str(EXT), f"-L{PKG}", "-lnl_ops", f"-L{tdir / 'lib'}", "-ltorch_python", "-ltorch_cpu",
+           "-ltorch", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {EXT_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    return f"compiled: {EXT_SRC.name}"
+
+
 def build(verbose: bool = False) -> Path:
     nvcc = _nvcc()
     BUILD_DIR.mkdir(exist_ok=True)
@@ -64,6 +89,9 @@ def build(verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    msg = _build_ext()
+    if verbose:
+        print(msg)
     return OUT
 
 

@@ -379,8 +379,6 @@ int launch(Params& p, int B, cudaStream_t stream) {
 
 using namespace nl;
 
-static_assert(sizeof(nl_process_logits_args) == 160, "packed by _lib.py");
-
 extern "C" int nl_process_logits(const nl_process_logits_args* args, cudaStream_t stream) {
   if (!args) return NL_ERR_SHAPE;
   const nl_process_logits_args& a = *args;

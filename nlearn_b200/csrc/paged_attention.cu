@@ -1025,8 +1025,6 @@ bool shape_ok(int B, int Hq, int Hk, int d, int page, int max_blocks) {
 
 using namespace nl;
 
-static_assert(sizeof(nl_paged_attention_args) == 232, "packed by _lib.py");
-
 extern "C" size_t nl_paged_attention_workspace_bytes(int B, int Hq, int Hk, int d, int page_size, int max_blocks,
                                                      int cache_dtype) {
   if (!pa::shape_ok(B, Hq, Hk, d, page_size, max_blocks)) return 0;

@@ -344,9 +344,6 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const WriteParams p) {
 
 using namespace nl;
 
-static_assert(sizeof(nl_update_block_tables_args) == 128 && sizeof(nl_paged_kv_write_args) == 120,
-              "packed by _lib.py");
-
 extern "C" int nl_update_block_tables(const nl_update_block_tables_args* args, cudaStream_t stream) {
   if (!args) return NL_ERR_SHAPE;
   const nl_update_block_tables_args& a = *args;

@@ -2,13 +2,18 @@
 the C entries' status codes on arguments they must not take (no GPU needed;
 the pointers are never read), CPU tensors at the Python entries, and the
 NumPy restatements against hand-made cases."""
+import struct
+
 import numpy as np
 import pytest
 import torch
 
-from nlearn_b200._lib import ARGS, STATUS, lib
+from nlearn_b200._lib import STATUS, lib
 from oracle import paged as OP
 
+# the argument structs of include/nl_ops.h (P pointer, q long long, N size_t, i int, f float)
+ARGS = {"nl_paged_attention": struct.Struct("@12P11qN8if4x"), "nl_paged_kv_write": struct.Struct("@7P5q6i"),
+        "nl_update_block_tables": struct.Struct("@12Pq5i4x"), "nl_process_logits": struct.Struct("@12P5q6i")}
 P = 1 << 20  # an aligned non-null address that no refused call reads
 
 
