@@ -30,7 +30,7 @@
 namespace nl {
 namespace lg {
 
-constexpr int kThreads = 768;
+constexpr int kThreads = 512;
 constexpr int kCtas = 2;              // resident CTAs of an SM: registers and shared memory are kept for them
 constexpr int kList = 128;            // biases of a row that are kept in shared memory
 constexpr int kSmem = 108 * 1024;     // dynamic shared memory of a CTA: kCtas of them fit an SM
@@ -108,29 +108,36 @@ struct Piece {
     for (int k = 0; k < VEC; ++k) e[k] = i + k < n ? x[i + k] : put<T>(0.f);
     w = *reinterpret_cast<const uint4*>(e);
   }
-  // from shared memory, where the words around the piece can always be read
-  __device__ __forceinline__ void load_shared(const T* x, bool aligned) {
-    if (aligned) {
-      w = *reinterpret_cast<const uint4*>(x);
+  // From shared memory: the piece that begins `bytes` into the 16-byte unit at u
+  // (the same for all lanes; the unit after it can be read too).
+  __device__ __forceinline__ void load_shared(const uint4* u, int bytes) {
+    const uint4 lo = u[0];
+    if (bytes == 0) {
+      w = lo;
       return;
     }
-    const uintptr_t a = reinterpret_cast<uintptr_t>(x);
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
-    w = make_uint4(p[0], p[1], p[2], p[3]);
-    if (sizeof(T) == 2 && (a & 2)) {
-      const uint32_t w4 = p[4];
-      w = make_uint4(__funnelshift_r(w.x, w.y, 16), __funnelshift_r(w.y, w.z, 16), __funnelshift_r(w.z, w.w, 16),
-                     __funnelshift_r(w.w, w4, 16));
+    const uint4 hi = u[1];
+    uint4 v;
+    uint32_t v4;  // the words from `bytes` on
+    switch (bytes >> 2) {
+      case 0: v = lo, v4 = hi.x; break;
+      case 1: v = make_uint4(lo.y, lo.z, lo.w, hi.x), v4 = hi.y; break;
+      case 2: v = make_uint4(lo.z, lo.w, hi.x, hi.y), v4 = hi.z; break;
+      default: v = make_uint4(lo.w, hi.x, hi.y, hi.z), v4 = hi.w; break;
     }
+    const int half = (bytes & 2) * 8;
+    w = make_uint4(__funnelshift_r(v.x, v.y, half), __funnelshift_r(v.y, v.z, half),
+                   __funnelshift_r(v.z, v.w, half), __funnelshift_r(v.w, v4, half));
   }
   // columns whose bit is 0 become -inf
   __device__ __forceinline__ void mask(uint32_t bits) {
-    uint32_t* u = &w.x;
     if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (!(bits >> k & 1)) u[k] = 0xff800000u;
+      if (!(bits & 1)) w.x = 0xff800000u;
+      if (!(bits & 2)) w.y = 0xff800000u;
+      if (!(bits & 4)) w.z = 0xff800000u;
+      if (!(bits & 8)) w.w = 0xff800000u;
     } else {
+      uint32_t* u = &w.x;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         // bits 2 k and 2 k + 1 to the tops of the two halves, spread over them
@@ -166,9 +173,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   constexpr int VEC = Piece<T>::VEC;
   constexpr uint32_t kAll = (1u << VEC) - 1;
   constexpr int HEADS = 2;  // groups of four tokens a thread asks for at the start
-  extern __shared__ __align__(16) uint8_t smem[];  // words C [chunk], logits T [chunk + VEC] if staged, the list
+  extern __shared__ __align__(16) uint8_t smem[];  // words C [chunk], if staged: logits T [chunk + 2 VEC], mask [chunk / 32]; the list
   uint8_t* s_chunk = smem + p.chunk * sizeof(C);
-  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_chunk + (p.staged ? (p.chunk + VEC) * sizeof(T) : 0));
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_chunk + (p.staged ? (p.chunk + 2 * VEC) * sizeof(T) : 0));
+  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_mask + (p.staged && p.mask ? p.chunk / 32 : 0));
   __shared__ int s_ids[kList];
   __shared__ float s_add[kList];
   __shared__ int s_n;
@@ -202,17 +210,37 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
     if (p.frequency) freq = p.frequency[b];
     if (p.presence) pres = p.presence[b];
   }
-  const uint32_t* mask = nullptr;
+  const uint8_t* mask = nullptr;  // bit v of the row, as bytes from the chunk's first column on
   if (p.mask) {
     const int r = p.mask_rows ? p.mask_rows[b] : b;
-    if (r >= 0 && r < p.n_masks) mask = p.mask + r * p.ldm + (c0 >> 5);
+    if (r >= 0 && r < p.n_masks) mask = reinterpret_cast<const uint8_t*>(p.mask + r * p.ldm) + (c0 >> 3);
   }
   constexpr int STEP = kThreads * VEC;
-  // (chunks are multiples of 32 columns: the bits of a piece lie in one word)
-  auto bits_of = [&](int i) { return mask && i < n ? mask[i >> 5] >> (i & 31) & kAll : kAll; };
+  // (chunks and steps are multiples of 64 columns: the bits of a piece lie in one byte)
+  auto bits_of = [&](int i) { return mask && i < n ? mask[i >> 3] >> (i & 7) & kAll : kAll; };
   auto masked = [&](Piece<T>& piece, uint32_t bits) { if (bits != kAll) piece.mask(bits); };
   if (!sparse) {  // no rule but the mask: straight through, two pieces ahead
     if (in_place && !mask) return;
+    if (vec_in && vec_out && !in_place) {
+      const uint4* src = reinterpret_cast<const uint4*>(x) + tid;
+      uint4* dst = reinterpret_cast<uint4*>(y) + tid;
+      const uint8_t* bits = mask ? mask + (tid * VEC >> 3) : nullptr;
+      const int whole = n / VEC;
+#pragma unroll 4
+      for (int i = tid; i < whole; i += kThreads) {
+        Piece<T> cur{*src};
+        if (bits) {
+          masked(cur, *bits >> (tid * VEC & 7) & kAll);
+          bits += STEP >> 3;
+        }
+        *dst = cur.w;
+        src += kThreads;
+        dst += kThreads;
+      }
+      const int i = whole * VEC + tid;
+      if (i < n) y[i] = mask && !(mask[i >> 3] >> (i & 7) & 1) ? put<T>(-INFINITY) : x[i];
+      return;
+    }
     Piece<T> next[2];
     uint32_t next_bits[2];
 #pragma unroll
@@ -240,10 +268,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   T* s_x = reinterpret_cast<T*>(s_chunk) + phase;
   if (p.staged) {
     const int lead = min(n, (VEC - phase) % VEC), units = (n - lead) / VEC, done = lead + units * VEC;
-    for (int i = tid; i < units; i += kThreads)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s_x + lead + i * VEC)),
-                   "l"(x + lead + i * VEC)
-                   : "memory");
+    const T* src = x + lead + tid * VEC;
+    uint32_t dst = smem_u32(s_x + lead + tid * VEC);
+    for (int i = tid; i < units; i += kThreads) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+      src += STEP;
+      dst += STEP * sizeof(T);
+    }
+    if (mask)
+      for (int i = tid; i < (n + 31) / 32; i += kThreads)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(s_mask + i)), "l"(mask + 4 * i)
+                     : "memory");
     if (tid < lead) s_x[tid] = x[tid];
     if (tid < n - done) s_x[done + tid] = x[done + tid];
   }
@@ -303,13 +338,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();  // counts, list and chunk
-  const T* from = p.staged ? s_x : x;
   T* to = p.staged ? s_x : y;
   const int on_list = s_n;
-  for (int i = tid; i < on_list; i += kThreads) {
-    const unsigned j = s_list[i];
+  auto rewrite = [&](unsigned j, float f) {
     const uint32_t w = *word_of(j) >> shift_of(j);
-    float f = get<T>(from[j]);
     if (w & (W::kSeen | W::kCount)) {
       f = f > 0.f ? f / rep : f * rep;
       const uint32_t made = w & W::kCount;
@@ -324,16 +356,49 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
         if (ids[m] == id) f += add[m];
     }
     to[j] = put<T>(f);  // (rounded once: a masked column is overwritten below)
+  };
+  if (p.staged) {
+    for (int i = tid; i < on_list; i += kThreads) rewrite(s_list[i], get<T>(s_x[s_list[i]]));
+  } else {
+    // in place the columns come from HBM: four are asked for before the first is worked on
+    for (int i0 = tid; i0 < on_list; i0 += 4 * kThreads) {
+      float f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = get<T>(x[s_list[min(i0 + k * kThreads, on_list - 1)]]);
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        if (i0 + k * kThreads < on_list) rewrite(s_list[i0 + k * kThreads], f[0]);
+        f[0] = f[1], f[1] = f[2], f[2] = f[3];
+      }
+    }
   }
   if (!p.staged) return;
   __syncthreads();
-  const bool vec_s = phase == 0;
-  for (int i = tid * VEC; i < n; i += STEP) {
+  const int whole = n / VEC, shift = phase * static_cast<int>(sizeof(T));
+  const uint4* src = reinterpret_cast<const uint4*>(s_chunk) + tid;
+  T* dst = y + tid * VEC;
+  const uint8_t* row_bits = reinterpret_cast<const uint8_t*>(s_mask);
+  const uint8_t* bits = mask ? row_bits + (tid * VEC >> 3) : nullptr;
+#pragma unroll 2
+  for (int i = tid; i < whole; i += kThreads) {
     Piece<T> cur;
-    cur.load_shared(s_x + i, vec_s);
-    masked(cur, bits_of(i));
-    cur.store(y, i, n, vec_out);
+    cur.load_shared(src, shift);
+    if (bits) {
+      masked(cur, *bits >> (tid * VEC & 7) & kAll);
+      bits += STEP >> 3;
+    }
+    if (vec_out) {
+      *reinterpret_cast<uint4*>(dst) = cur.w;
+    } else {
+      const T* e = reinterpret_cast<const T*>(&cur.w);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) dst[k] = e[k];
+    }
+    src += kThreads;
+    dst += STEP;
   }
+  const int i = whole * VEC + tid;
+  if (i < n) y[i] = mask && !(row_bits[i >> 3] >> (i & 7) & 1) ? put<T>(-INFINITY) : s_x[i];
 }
 
 // Columns of a CTA: a row in as many equal chunks as fill one wave of CTAs, of at most `most` columns.
@@ -350,16 +415,17 @@ int launch(Params& p, int B, cudaStream_t stream) {
   const bool sparse = p.tokens || p.n_bias > 0;
   p.staged = sparse && !(p.x == p.y && !p.mask);
   // a list holds each column once, and no more than there are tokens and biases
-  const int bytes = sizeof(C) + (p.staged ? sizeof(T) : 0), tail = 64;
+  const double bytes = sizeof(C) + (p.staged ? sizeof(T) + (p.mask ? 0.125 : 0.) : 0.);
+  constexpr int tail = 64;
   const long long list = static_cast<long long>(p.tokens ? p.L : 0) + p.n_bias;
   long long most = 65536;
   if (sparse) {
-    most = (kSmem - tail) / (bytes + 2);
-    if (list < most) most = (kSmem - tail - 2 * list) / bytes;
+    most = static_cast<long long>((kSmem - tail) / (bytes + 2));
+    if (list < most) most = static_cast<long long>((kSmem - tail - 2 * list) / bytes);
   }
   p.chunk = chunk_of(B, p.V, static_cast<int>(most / 64 * 64));
   const size_t smem =
-      sparse ? tail + static_cast<size_t>(p.chunk) * bytes + 2 * static_cast<size_t>(list < p.chunk ? list : p.chunk)
+      sparse ? tail + static_cast<size_t>(p.chunk * bytes) + 2 * static_cast<size_t>(list < p.chunk ? list : p.chunk)
              : 0;
   constexpr int kMaxDev = 64;
   static bool ready[kMaxDev] = {false};
@@ -385,6 +451,7 @@ extern "C" int nl_process_logits(const nl_process_logits_args* args, cudaStream_
   const int B = a.B, V = a.V, dtype = a.dtype;
   if (B <= 0 || B > 65535 || V <= 0 || a.ldx < V || a.ldy < V || !a.logits || !a.out) return NL_ERR_SHAPE;
   if (dtype != NL_F32 && dtype != NL_BF16) return NL_ERR_DTYPE;
+  if (a.logits == a.out && B > 1 && a.ldx != a.ldy) return NL_ERR_SHAPE;
   if (a.tokens && (a.L <= 0 || a.ldt < a.L || !a.lens)) return NL_ERR_SHAPE;
   if (a.n_bias < 0 || (a.n_bias > 0 && (!a.bias_ids || !a.bias || a.ldb < a.n_bias))) return NL_ERR_SHAPE;
   if (a.mask && (a.ldm < (V + 31) / 32 || a.n_masks <= 0 || (!a.mask_rows && a.n_masks < B))) return NL_ERR_SHAPE;
