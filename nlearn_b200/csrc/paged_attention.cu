@@ -59,10 +59,11 @@ constexpr int kHeads = 8;                 // query heads of one product (its col
 constexpr int kMaxTiles = 2;              // products of 8 heads a CTA keeps: groups of up to 16 read the keys once
 constexpr int kMaxCluster = 8;
 constexpr int kJoinThreads = 256;
-// Starting a run and joining its warps costs a CTA about as much as one unit
-// (a fit of CTA times on ragged batches: 1.38 us a unit and 1.60 us a run, bf16,
-// d 128; 1.79 and 2.48 us, e4m3), so it is counted as one.
-constexpr int kOver = 1;
+// Starting and ending a run costs a CTA as much as one unit of work with a bf16 cache, two with
+// an e4m3 one (a fit of the CTAs' times on ragged batches, d 128: 1.34 us a unit
+// and 1.14 to 1.38 us a run; 1.39 us and 3.2 to 3.7 us), so it is counted as that.
+template <bool FP8>
+constexpr int kOver = FP8 ? 2 : 1;
 constexpr float kNoRef = -3.402823466e38f;  // before the first score: any finite one is above it
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;             // log2 of how far p may grow before the maximum moves
@@ -166,10 +167,10 @@ template <int UNIT>
 __device__ __forceinline__ int units_of(int len) {
   return (len + UNIT - 1) / UNIT;
 }
-// Length of one (sequence, head tile) in the flat list: its units, after kOver for its start and its join.
-template <int UNIT>
+// Length of one (sequence, head tile) in the flat list: its units, after OVER for its start and its end.
+template <int UNIT, int OVER>
 __device__ __forceinline__ int weight_of(int len) {
-  return len > 0 ? units_of<UNIT>(len) + kOver : 0;
+  return len > 0 ? units_of<UNIT>(len) + OVER : 0;
 }
 
 // First unit of CTA i of n over U units.
@@ -183,7 +184,7 @@ struct Run {
   int b, seg, len, nu, c0, c1;
 };
 // Walks a CTA's range of the flat list, run by run (a run is not empty).
-template <int UNIT>
+template <int UNIT, int OVER>
 struct Walk {
   int segs;      // segments of a sequence
   int u, u1;     // next unit, end of the range
@@ -193,18 +194,18 @@ struct Walk {
       int len, w;
       for (;; ++b) {
         len = clamp_len(p, b);
-        w = weight_of<UNIT>(len);
+        w = weight_of<UNIT, OVER>(len);
         if (u - base < w * segs) break;
         base += w * segs;
       }
       const int local = u - base;
       r.b = b;
       r.len = len;
-      r.nu = w - kOver;
+      r.nu = w - OVER;
       r.seg = local / w;
       const int c = local - r.seg * w, n = min(w - c, u1 - u);
-      r.c0 = max(0, c - kOver);
-      r.c1 = max(0, c + n - kOver);
+      r.c0 = max(0, c - OVER);
+      r.c1 = max(0, c + n - OVER);
       u += n;
       if (r.c1 > r.c0) return true;
     }
@@ -250,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   using S = Shape<HD, FP8>;
   constexpr bool CLUSTER = MODE == kClustered, HEADS = MODE == kByHeads;
   constexpr int UNIT = HEADS ? S::TILE : S::TILE * kWarps;  // keys of one unit of work
+  constexpr int OVER = kOver<FP8>;
   // p = 2^(y - ref) with ref the running maximum less kUp: below 2^15, in f16's range, with the slack
   constexpr float kUp = FP8 ? 7.f : 0.f;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -265,9 +267,9 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   const int segs = p.Hk * p.mtiles / (HEADS ? kWarps : 1);  // of a sequence
   int U = 0, ctas = 0, rank = 0, csize = 1;
   const int cta = blockIdx.x;
-  Walk<UNIT> walk;  // of the copies
+  Walk<UNIT, OVER> walk;  // of the copies
   Run first = {};      // of the products
-  Walk<UNIT> cwalk;
+  Walk<UNIT, OVER> cwalk;
   bool live;
   if constexpr (CLUSTER) {
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     for (int b = sb0; b < sb1; ++b) {
       const int n = p.lens[b];
       if (cta == 0 && (n < 0 || n > cap_of(p)) && p.err) atomicExch(p.err, kErrPos);
-      mine += weight_of<UNIT>(clamp_len(p, b));
+      mine += weight_of<UNIT, OVER>(clamp_len(p, b));
     }
     int inc = mine;
 #pragma unroll
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     if (x >= before && x < before + mine) {
       int b = sb0, pre = before;
       for (; b < sb1; ++b) {
-        const int n = weight_of<UNIT>(clamp_len(p, b));
+        const int n = weight_of<UNIT, OVER>(clamp_len(p, b));
         if (x < pre + n) break;
         pre += n;
       }
@@ -1017,7 +1019,7 @@ bool shape_ok(int B, int Hq, int Hk, int d, int page, int max_blocks) {
   const long long cap = static_cast<long long>(max_blocks) * page;
   // unit counts of a call are 32-bit
   return cap <= INT32_MAX - 256 &&
-         static_cast<double>(B) * Hk * mtiles * static_cast<double>((cap + 63) / 64 + kOver) <= INT32_MAX;
+         static_cast<double>(B) * Hk * mtiles * static_cast<double>((cap + 63) / 64 + kOver<true> + 1) <= INT32_MAX;
 }
 
 }  // namespace pa

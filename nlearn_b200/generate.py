@@ -415,13 +415,14 @@ class PagedDecoder(_DecodeStep):
             if not use_graph:
                 self._step(rules)
             else:
-                graph = self._graphs.get(rules)
+                key = (rules, self.seed, self.temperature)
+                graph = self._graphs.get(key)
                 if graph is None:
                     self._step(rules)  # (the first step of a kind runs eagerly: it sets the kernels up)
-                    self._graphs[rules] = False
+                    self._graphs[key] = False
                 else:
                     if graph is False:
-                        graph = self._graphs[rules] = torch.cuda.CUDAGraph()
+                        graph = self._graphs[key] = torch.cuda.CUDAGraph()
                         with torch.cuda.graph(graph):
                             self._step(rules)
                     graph.replay()
@@ -460,6 +461,8 @@ class PagedDecoder(_DecodeStep):
         counts = [int(n) for n in np.broadcast_to(n_tokens, (len(prompts),))]
         if any(n >= self.S for n in counts):
             raise ValueError(f"n_tokens {max(counts)} must be below max_len {self.S}")
+        if any(p.size < 1 for p, n in zip(prompts, counts) if n > 0):
+            raise ValueError("an empty prompt")
         prompts = [p[-(self.S - n):] if n > 0 else p for p, n in zip(prompts, counts)]
         done: list = [p.copy() if n <= 0 else None for p, n in zip(prompts, counts)]
         queue = [i for i in range(len(prompts)) if done[i] is None]
