@@ -116,8 +116,13 @@ inline int make_tmap_f32_rows64_3d(CUtensorMap* m, const void* base, uint64_t ro
 }
 
 inline int sm_count() {
+  constexpr int kMaxDev = 64;
+  static int known[kMaxDev] = {0};  // asked once per device
   int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (cudaGetDevice(&dev) != cudaSuccess) return n;
+  if (dev >= 0 && dev < kMaxDev && known[dev] > 0) return known[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && dev >= 0 && dev < kMaxDev)
+    known[dev] = n;
   return n;
 }
 

@@ -36,9 +36,14 @@
 //     keys (four warps, one tile each), cut into equal ranges, one per CTA, so any mix of
 //     lengths balances.  The cut ends leave partials (max, sum, o) that
 //     join_kernel merges in the order of the cache;
-//   * clustered, for short caches: a cluster of up to 8 CTAs per (sequence,
-//     head) merges over distributed shared memory: one launch, no prefix sums.
-// Neither depends on the order in which CTAs finish.
+//   * clustered, where the table allows at most 2048 keys a CTA: a cluster of up to 8 CTAs
+//     per (sequence, head) merges over distributed shared memory: one launch,
+//     no prefix sums.
+// Neither depends on the order in which CTAs finish.  Measured (B200, share of the 6.56 TB/s of a copy):
+// 48 sequences of up to 8192, 32/8 heads of 128, token-major: 130 us, 94 %; one of
+// 131072: 86 us, 95 %; 64 of up to 4097 on an e4m3 cache: 55.6 us, 74 % (the run's
+// start and end, and the join, are the rest: between them a unit takes what its bytes do);
+// 32 of up to 512, 8 heads of 64: 7.6 us, one of 512: 4.7 us (the chain of loads: length, page, tile).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -58,6 +63,10 @@ constexpr int kGroup = 16;                // keys of one product (its rows); a p
 constexpr int kHeads = 8;                 // query heads of one product (its columns)
 constexpr int kMaxTiles = 2;              // products of 8 heads a CTA keeps: groups of up to 16 read the keys once
 constexpr int kMaxCluster = 8;
+// Keys of a CTA up to which a call is clustered.  A flat call costs about 5 us
+// more (prefix sums, join) and balances sequences of different lengths: 32 sequences, 8 heads of 64, clustered /
+// flat, all of 2048: 25.1 / 29.9 us, of up to 2048: 18.0 / 21.8; of up to 8192 (4096 a CTA): 58.0 / 57.2.
+constexpr int kMaxShare = 2048;
 constexpr int kJoinThreads = 256;
 // Starting and ending a run costs a CTA as much as one unit of work with a bf16 cache, two with
 // an e4m3 one (a fit of the CTAs' times on ragged batches, d 128: 1.34 us a unit
@@ -262,7 +271,11 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   __shared__ float2 s_ml[kHeads * NH];  // clustered: this CTA's (max, sum)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  griddep_sync();
+  // Flat, the next grid (the join) is let in when a CTA is done, not here: its CTAs
+  // would take the place of this grid's on some SMs and stay there, waiting (128
+  // sequences of 2048, 8 heads of 64: 108 -> 92 us).
+  if constexpr (MODE == kClustered) griddep_sync();
+  else griddep_wait();
 
   const int segs = p.Hk * p.mtiles / (HEADS ? kWarps : 1);  // of a sequence
   int U = 0, ctas = 0, rank = 0, csize = 1;
@@ -816,8 +829,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     r = nr;
     live = again;
   }
-  if constexpr (!CLUSTER)
+  if constexpr (!CLUSTER) {
+    griddep_launch();
     if (tid == 0) p.desc[cta] = my_desc;
+  }
   if (bad_page && p.err) atomicExch(p.err, kErrPage);
 }
 
@@ -931,7 +946,7 @@ struct Plan {
 };
 
 template <int HD, bool FP8, int NH>
-Plan plan_of(int B, int heads, int max_blocks, int page) {
+Plan plan_of(int B, int heads, int rows, int max_blocks, int page) {
   const int occ = ctas_per_sm<HD, FP8, NH>();
   if (occ <= 0) return {0, 0, 0};
   const long long card = static_cast<long long>(sm_count()) * occ;
@@ -941,16 +956,17 @@ Plan plan_of(int B, int heads, int max_blocks, int page) {
   const long long units = (cap + unit - 1) / unit;  // of a full table row
   int c = 1;
   while (c < kMaxCluster && 2 * c <= units && segs * 2 * c <= card) c *= 2;
-  if (cap <= 512 * c && segs * c <= INT32_MAX) return {kClustered, static_cast<int>(segs * c), c};
-  // The four warps of a CTA on four heads (no join of the warps at a run's end, four
-  // times the partials at a CTA's) or on one: by heads where sequences end often,
-  // that is where there are at least half as many (sequence, head) pairs as
-  // CTAs, and the partials are small (groups of up to 8).  By heads / by keys: 64
-  // sequences of up to 2048, 16 heads of 64, token-major: 58.8 / 73.8 us; e4m3,
-  // 64 of up to 4097, 32/8 heads of 128: 59.1 / 62.0; but 1 of 131072: 94.4 / 86.1;
-  // 32 of up to 8192, 64/4 heads of 128: 84.6 / 59.4.
+  if (cap <= kMaxShare * c && segs * c <= INT32_MAX) return {kClustered, static_cast<int>(segs * c), c};
+  // The four warps of a CTA on four heads (nothing to join at a run's end, four
+  // times the rows of partials at a CTA's; token-major rows of neighbouring heads are read
+  // together) or on one head: by heads where partials are small (at most two query heads
+  // share a kv head) or few (sequences end often: at least half as many (sequence,
+  // head) pairs as CTAs).  By heads / by keys: 200 sequences of up to 4096, 8 heads of 64,
+  // token-major: 136 / 165 us, e4m3: 80 / 143; 32 of up to 8192: 52.0 / 57.9; 48
+  // of up to 8192, 32/8 heads of 128: 130.0 / 129.3; but 1 of 131072: 94.3 / 85.7, and 32
+  // of up to 8192, 64/4 heads of 128: 84.1 / 59.0.
   // (A unit is as many bytes either way, so there are as many of them.)
-  const int mode = heads % kWarps == 0 && NH == 1 && 2 * segs >= card ? kByHeads : kByKeys;
+  const int mode = heads % kWarps == 0 && NH == 1 && (rows <= 2 || 2 * segs >= card) ? kByHeads : kByKeys;
   return {mode, static_cast<int>(segs * units < card ? segs * units : card), 0};
 }
 
@@ -984,9 +1000,9 @@ auto dispatch(int d, bool fp8, int rows, F f) {
              : (two ? f.template operator()<128, false, 2>() : f.template operator()<128, false, 1>());
 }
 struct PlanCall {
-  int B, heads, max_blocks, page;
+  int B, heads, rows, max_blocks, page;
   template <int HD, bool FP8, int NH>
-  Plan operator()() const { return plan_of<HD, FP8, NH>(B, heads, max_blocks, page); }
+  Plan operator()() const { return plan_of<HD, FP8, NH>(B, heads, rows, max_blocks, page); }
 };
 struct LaunchCall {
   Params& p;
@@ -1033,7 +1049,7 @@ extern "C" size_t nl_paged_attention_workspace_bytes(int B, int Hq, int Hk, int 
   int rows, mtiles;
   pa::split_group(Hq / Hk, &rows, &mtiles);
   const pa::Plan plan =
-      pa::dispatch(d, cache_dtype == NL_E4M3, rows, pa::PlanCall{B, Hk * mtiles, max_blocks, page_size});
+      pa::dispatch(d, cache_dtype == NL_E4M3, rows, pa::PlanCall{B, Hk * mtiles, rows, max_blocks, page_size});
   return pa::workspace(plan, rows, d, nullptr, nullptr);
 }
 
@@ -1066,7 +1082,7 @@ extern "C" int nl_paged_attention(const nl_paged_attention_args* args, cudaStrea
   p.group = Hq / Hk;
   pa::split_group(p.group, &p.rows, &p.mtiles);
   const pa::Plan plan =
-      pa::dispatch(d, cache_dtype == NL_E4M3, p.rows, pa::PlanCall{B, Hk * p.mtiles, max_blocks, page_size});
+      pa::dispatch(d, cache_dtype == NL_E4M3, p.rows, pa::PlanCall{B, Hk * p.mtiles, p.rows, max_blocks, page_size});
   if (plan.grid <= 0) return NL_ERR_CUDA;
   size_t ml = 0, desc = 0;
   const size_t need = pa::workspace(plan, p.rows, d, &ml, &desc);
