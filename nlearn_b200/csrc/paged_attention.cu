@@ -67,6 +67,10 @@ constexpr int kMaxCluster = 8;
 // more (prefix sums, join) and balances sequences of different lengths: 32 sequences, 8 heads of 64, clustered /
 // flat, all of 2048: 25.1 / 29.9 us, of up to 2048: 18.0 / 21.8; of up to 8192 (4096 a CTA): 58.0 / 57.2.
 constexpr int kMaxShare = 2048;
+// Where the clusters leave most of the card idle (less than a third of its CTAs), what the flat mode gains by
+// taking all of it counts for more: one sequence, 8 heads of 64, of 4096: 8.4 / 10.2 us, of 8192: 12.6 / 10.1;
+// four of them fill 43 %, of 8192: 17.1 / 19.2.
+constexpr int kMaxShareFew = 512;
 constexpr int kJoinThreads = 256;
 // Starting and ending a run costs a CTA as much as one unit of work with a bf16 cache, two with
 // an e4m3 one (a fit of the CTAs' times on ragged batches, d 128: 1.34 us a unit
@@ -187,8 +191,8 @@ __device__ __forceinline__ int cut(int i, int U, int n) {
   return static_cast<int>(static_cast<long long>(i) * U / n);
 }
 
-// A run: consecutive units [c0, c1) of one sequence and one segment of its
-// heads (a tile of query heads, or four of them, one per warp).
+// A run: units [c0, c1) of one sequence and one segment of its heads (a tile of
+// query heads, or four of them, one per warp).
 struct Run {
   int b, seg, len, nu, c0, c1;
 };
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   else griddep_wait();
 
   const int segs = p.Hk * p.mtiles / (HEADS ? kWarps : 1);  // of a sequence
-  int U = 0, ctas = 0, rank = 0, csize = 1;
+  int U = 0, ctas = 0, rank = 0, csize = 1, ustep = 1;
   const int cta = blockIdx.x;
   Walk<UNIT, OVER> walk;  // of the copies
   Run first = {};      // of the products
@@ -292,8 +296,18 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     first.seg = seg - first.b * segs;
     first.len = clamp_len(p, first.b);
     first.nu = units_of<UNIT>(first.len);
-    first.c0 = rank * first.nu / csize;
-    first.c1 = (rank + 1) * first.nu / csize;
+    // heads of 64 and short tables: a CTA takes every csize-th unit, so that its first one does not
+    // depend on the length and the page of it is looked up beside that (1 of 512, 8 heads: 4.8 -> 4.6 us;
+    // of 2048, 8 units a CTA: 6.5 -> 6.1, both with the join in one piece); else shares are in one piece
+    // (32/8 heads of 128: 5.5 us, every csize-th unit 5.7)
+    if (HD == 64 && cap_of(p) <= 2 * csize * UNIT) {
+      ustep = csize;
+      first.c0 = rank;
+      first.c1 = first.nu;
+    } else {
+      first.c0 = rank * first.nu / csize;
+      first.c1 = (rank + 1) * first.nu / csize;
+    }
     live = first.c1 > first.c0;
     if (seg == 0 && rank == 0)
       for (int b = tid; b < p.B; b += kThreads)
@@ -389,6 +403,19 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     if constexpr (S::RB >= 128) return i * S::RPI * S::RB + (my_dst ^ (((i * S::RPI) & 7) << 4));
     return i * S::RPI * S::RB + my_dst;  // 64-byte rows: 8 rows an instruction, same permutation
   };
+  if (HD == 64 && ustep > 1) {
+    // (the table has an entry for every position below cap)
+    const int pos = unit * UNIT + warp_key + (whole ? 0 : (lane & 15));
+    const int* row = p.table + in.b * p.table_ld;
+#pragma unroll
+    for (int j = 0; j < S::NG; ++j) {
+      const int at = pos + j * kGroup;
+      const int page = at < cap_of(p) ? __ldg(row + block_of(at)) : 0;
+      pg[j] = more && at < in.len ? page : 0;
+    }
+  } else {
+    look_up();
+  }
   auto copy_tile = [&]() {
     if (more) {
       const int hm = tile_of(in), h = hm / p.mtiles;
@@ -463,9 +490,11 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
         }
       }
       if (lane == 0) s_valid[warp][in_stage] = mask;
-      if (++unit == in.c1) {
-        if constexpr (CLUSTER) more = false;
-        else more = walk.next(p, in);
+      if constexpr (CLUSTER) {
+        unit += HD == 64 ? ustep : 1;
+        more = unit < in.c1;
+      } else if (++unit == in.c1) {
+        more = walk.next(p, in);
         unit = in.c0;
       }
       look_up();
@@ -530,7 +559,6 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     }
   };
 
-  look_up();
   if (live) load_q(first);
 #pragma unroll
   for (int s = 0; s < S::STAGES - 1; ++s) copy_tile();
@@ -551,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
       for (int i = 0; i < S::KS; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
     }
 
-    for (int c = r.c0; c < r.c1; ++c) {
+    for (int c = r.c0; c < r.c1; c += CLUSTER && HD == 64 ? ustep : 1) {
       cp_wait<S::STAGES - 2>();
       __syncwarp();
       copy_tile();
@@ -747,7 +775,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
             s_m[warp][n * kHeads + 2 * t4 + e] = ref[n][e];
             s_l[warp][n * kHeads + 2 * t4 + e] = l[n][e];
           }
-      float* scratch = reinterpret_cast<float*>(smem + S::RING);
+      // clustered, a short o is joined at once, over the ring, which is idle by then
+      constexpr int MT = CLUSTER && HD == 64 ? S::KS : S::MT;
+      static_assert(!CLUSTER || kHeads * NH * HD * 4 + kWarps * MT * 4 * 32 * 4 <= S::SMEM, "join");
+      float* scratch = reinterpret_cast<float*>(smem + (CLUSTER ? kHeads * NH * HD * 4 : S::RING));
       float* part = reinterpret_cast<float*>(smem);  // clustered: [rows][HD] over the ring, which is idle by then
       if constexpr (CLUSTER) {
         cp_wait<0>();
@@ -759,11 +790,11 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
         const int col = n * kHeads + 2 * t4 + (warp & 1);
         float f[kWarps], M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int i0 = 0; i0 < S::KS; i0 += S::MT) {
+        for (int i0 = 0; i0 < S::KS; i0 += MT) {
 #pragma unroll
-          for (int i = 0; i < S::MT; ++i)
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) scratch[((warp * S::MT + i) * 4 + e) * 32 + lane] = acc[n][i0 + i][e];
+            for (int e = 0; e < 4; ++e) scratch[((warp * MT + i) * 4 + e) * 32 + lane] = acc[n][i0 + i][e];
           __syncthreads();
           if (i0 == 0) {
 #pragma unroll
@@ -777,10 +808,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
           }
           if (col < nrows) {
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i) {
+            for (int i = 0; i < MT; ++i) {
               float O = 0.f;
 #pragma unroll
-              for (int w = 0; w < kWarps; ++w) O += f[w] * scratch[((w * S::MT + i) * 4 + warp) * 32 + lane];
+              for (int w = 0; w < kWarps; ++w) O += f[w] * scratch[((w * MT + i) * 4 + warp) * 32 + lane];
               const int d = (i0 + i) * 16 + (FP8 ? 2 * g + (warp >> 1) : g + 8 * (warp >> 1));
               if constexpr (CLUSTER) {
                 part[col * HD + d] = O;
@@ -795,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
               }
             }
           }
-          __syncthreads();  // scratch and s_m are written again
+          if (!CLUSTER || n + 1 < NH || i0 + MT < S::KS) __syncthreads();  // scratch is written again (s_m after a run)
         }
       }
       if constexpr (CLUSTER) {
@@ -956,17 +987,18 @@ Plan plan_of(int B, int heads, int rows, int max_blocks, int page) {
   const long long units = (cap + unit - 1) / unit;  // of a full table row
   int c = 1;
   while (c < kMaxCluster && 2 * c <= units && segs * 2 * c <= card) c *= 2;
-  if (cap <= kMaxShare * c && segs * c <= INT32_MAX) return {kClustered, static_cast<int>(segs * c), c};
+  const int share = 3 * segs * c >= card ? kMaxShare : kMaxShareFew;
+  if (cap <= share * c && segs * c <= INT32_MAX) return {kClustered, static_cast<int>(segs * c), c};
   // The four warps of a CTA on four heads (nothing to join at a run's end, four
   // times the rows of partials at a CTA's; token-major rows of neighbouring heads are read
   // together) or on one head: by heads where partials are small (at most two query heads
-  // share a kv head) or few (sequences end often: at least half as many (sequence,
-  // head) pairs as CTAs).  By heads / by keys: 200 sequences of up to 4096, 8 heads of 64,
-  // token-major: 136 / 165 us, e4m3: 80 / 143; 32 of up to 8192: 52.0 / 57.9; 48
+  // share a kv head, and 32 (sequence, head) pairs share the CTAs) or few (sequences end
+  // often: at least half as many pairs as CTAs).  By heads / by keys: 200 sequences of up to 4096, 8 heads of 64,
+  // token-major: 136 / 165 us, e4m3: 80 / 143; 32 of up to 8192: 52.0 / 57.9; 1 of 8192: 13.5 / 10.1; 48
   // of up to 8192, 32/8 heads of 128: 130.0 / 129.3; but 1 of 131072: 94.3 / 85.7, and 32
   // of up to 8192, 64/4 heads of 128: 84.1 / 59.0.
   // (A unit is as many bytes either way, so there are as many of them.)
-  const int mode = heads % kWarps == 0 && NH == 1 && (rows <= 2 || 2 * segs >= card) ? kByHeads : kByKeys;
+  const int mode = heads % kWarps == 0 && NH == 1 && ((rows <= 2 && segs >= 32) || 2 * segs >= card) ? kByHeads : kByKeys;
   return {mode, static_cast<int>(segs * units < card ? segs * units : card), 0};
 }
 
