@@ -17,8 +17,8 @@
 // rules inside a pass over all columns nearly every warp held a named one and
 // took the long way; with the list worked off in global memory its scattered
 // 2-byte accesses were the longest part: 36 and 27 us for 256 rows of 50257 in
-// bf16 with 2048 tokens each.)  In place and without a mask the chunk is not
-// copied: only the columns on the list are read and written.
+// bf16 with 2048 tokens each; now 18.7.)  In place and without a mask a row with
+// few tokens is not copied: only the columns on its list are read and written.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <math.h>
@@ -33,8 +33,11 @@ namespace lg {
 constexpr int kThreads = 512;
 constexpr int kCtas = 2;              // resident CTAs of an SM: registers and shared memory are kept for them
 constexpr int kList = 128;            // biases of a row that are kept in shared memory
-constexpr int kSmem = 108 * 1024;     // dynamic shared memory of a CTA: kCtas of them fit an SM
-
+constexpr int kSmem = 111 * 1024;     // dynamic shared memory of a CTA: kCtas of them fit an SM
+// In place and without a mask: bytes of the row to a column on the list from which the list is worked off in
+// global memory, a sector read and written for each.  In place / through shared memory, 256 rows of 50257, us:
+// bf16 with 512 tokens 7.5 / 13.2, 1024 12.9 / 13.6, 2048 20.0 / 14.3; f32 1024 14.6 / 21.3, 2048 22.9 / 22.1.
+constexpr int kFew = 96;
 
 // A column's word: how often it was generated, and two flags.
 template <typename C>
@@ -64,7 +67,7 @@ struct Params {
   const uint32_t* mask;  // [R, words]
   long long ldm;
   const int* mask_rows;  // null: row b uses mask row b; < 0: row b has no mask
-  int V, L, n_bias, n_masks, chunk, staged;  // staged: the chunk goes through shared memory
+  int V, L, n_bias, n_masks, chunk, staged;  // staged: there is room for the chunk in shared memory
 };
 
 template <typename T>
@@ -80,14 +83,16 @@ __device__ __forceinline__ float put<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 put<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// 16 bytes of a row's columns: x[i .. i + VEC) of n columns that exist.  Rows that
-// are not 16-byte aligned are read by 32-bit words, shifted together.
+// 16 bytes of a row's columns, x[i .. i + VEC).  Pieces are cut where the output is
+// 16-byte aligned; an input that is not aligned there is read by 32-bit words,
+// shifted together.
 template <typename T>
 struct Piece {
   static constexpr int VEC = 16 / sizeof(T);
   uint4 w;
+  // of n columns that exist, all of the piece's among them
   __device__ __forceinline__ void load(const T* x, int i, int n, bool aligned) {
-    if (aligned && i + VEC <= n) {
+    if (aligned) {
       w = *reinterpret_cast<const uint4*>(x + i);
       return;
     }
@@ -105,7 +110,7 @@ struct Piece {
     }
     T e[VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) e[k] = i + k < n ? x[i + k] : put<T>(0.f);
+    for (int k = 0; k < VEC; ++k) e[k] = x[i + k];
     w = *reinterpret_cast<const uint4*>(e);
   }
   // From shared memory: the piece that begins `bytes` into the 16-byte unit at u
@@ -148,16 +153,21 @@ struct Piece {
       }
     }
   }
-  __device__ __forceinline__ void store(T* y, int i, int n, bool aligned) const {
-    if (aligned && i + VEC <= n) {
-      *reinterpret_cast<uint4*>(y + i) = w;
-      return;
-    }
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k)
-      if (i + k < n) y[i + k] = e[k];
+};
+
+// Where a chunk of n columns is cut into pieces: behind the columns before the output's first
+// 16-byte unit.
+template <typename T>
+struct Cut {
+  int phase, first, behind;
+  __device__ __forceinline__ Cut(const T* y, int n) {
+    constexpr int VEC = Piece<T>::VEC;
+    phase = static_cast<int>((reinterpret_cast<uintptr_t>(y) & 15) / sizeof(T));
+    first = min(n, (VEC - phase) % VEC);
+    behind = first + (n - first) / VEC * VEC;
   }
+  // the i-th column that is in no piece
+  __device__ __forceinline__ int rest(int i) const { return i < first ? i : behind + i - first; }
 };
 
 // Four of a row's tokens, -1 past the last.
@@ -167,32 +177,88 @@ __device__ __forceinline__ int4 four_tokens(const int* t, int i, int len, bool v
                    i + 3 < len ? t[i + 3] : -1);
 }
 
+// Bit v of row b's mask, as bytes from the chunk's first column on (null: no mask).
+__device__ __forceinline__ const uint8_t* mask_of(const Params& p, int b, int c0) {
+  if (!p.mask) return nullptr;
+  const int r = p.mask_rows ? p.mask_rows[b] : b;
+  return r >= 0 && r < p.n_masks ? reinterpret_cast<const uint8_t*>(p.mask + r * p.ldm) + (c0 >> 3) : nullptr;
+}
+
+// No rule but the mask: straight through, two pieces ahead.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kCtas) mask_kernel(const Params p) {
+  constexpr int VEC = Piece<T>::VEC, STEP = kThreads * VEC;
+  constexpr uint32_t kAll = (1u << VEC) - 1;
+  const int tid = threadIdx.x;
+  const int b = blockIdx.y, c0 = blockIdx.x * p.chunk, n = min(p.chunk, p.V - c0);
+  griddep_sync();
+  const T* x = static_cast<const T*>(p.x) + b * p.ldx + c0;
+  T* y = static_cast<T*>(p.y) + b * p.ldy + c0;
+  const bool in_place = p.x == p.y;
+  const uint8_t* mask = mask_of(p, b, c0);
+  if (in_place && !mask) return;
+  const Cut<T> cut(y, n);
+  const bool aligned = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) == cut.phase;
+  // bits i .. i + VEC, all of which exist
+  auto bits_of = [&](int i) -> uint32_t {
+    if (!mask) return kAll;
+    uint32_t bits = mask[i >> 3];
+    if ((i & 7) + VEC > 8) bits |= static_cast<uint32_t>(mask[(i >> 3) + 1]) << 8;
+    return bits >> (i & 7) & kAll;
+  };
+  const int rest = cut.rest(tid);
+  T single = put<T>(-INFINITY);
+  if (rest < n && (!mask || (mask[rest >> 3] >> (rest & 7) & 1))) single = x[rest];
+  Piece<T> next[2];
+  uint32_t next_bits[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = cut.first + tid * VEC + k * STEP;
+    if (i < cut.behind) {
+      next[k].load(x, i, n, aligned);
+      next_bits[k] = bits_of(i);
+    }
+  }
+#pragma unroll 2
+  for (int i = cut.first + tid * VEC; i < cut.behind; i += STEP) {
+    Piece<T> cur = next[0];
+    const uint32_t bits = next_bits[0];
+    next[0] = next[1];
+    next_bits[0] = next_bits[1];
+    if (i + 2 * STEP < cut.behind) {
+      next[1].load(x, i + 2 * STEP, n, aligned);
+      next_bits[1] = bits_of(i + 2 * STEP);
+    }
+    if (bits != kAll) cur.mask(bits);
+    if (!in_place || bits != kAll) *reinterpret_cast<uint4*>(y + i) = cur.w;
+  }
+  if (rest < n) y[rest] = single;
+}
+
 template <typename T, typename C>
 __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p) {
   using W = Word<C>;
   constexpr int VEC = Piece<T>::VEC;
   constexpr uint32_t kAll = (1u << VEC) - 1;
+  constexpr int STEP = kThreads * VEC;
   constexpr int HEADS = 2;  // groups of four tokens a thread asks for at the start
-  extern __shared__ __align__(16) uint8_t smem[];  // words C [chunk], if staged: logits T [chunk + 2 VEC], mask [chunk / 32]; the list
+  extern __shared__ __align__(16) uint8_t smem[];  // words C [chunk], if staged: logits T [chunk + 2 VEC], mask [chunk / 32 + 1]; the list
   uint8_t* s_chunk = smem + p.chunk * sizeof(C);
   uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_chunk + (p.staged ? (p.chunk + 2 * VEC) * sizeof(T) : 0));
-  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_mask + (p.staged && p.mask ? p.chunk / 32 : 0));
+  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_mask + (p.staged && p.mask ? p.chunk / 32 + 1 : 0));
   __shared__ int s_ids[kList];
   __shared__ float s_add[kList];
   __shared__ int s_n;
   const int tid = threadIdx.x;
   const int b = blockIdx.y, c0 = blockIdx.x * p.chunk, n = min(p.chunk, p.V - c0);
-  const bool counts = p.tokens != nullptr, biases = p.n_bias > 0, sparse = counts || biases;
-  if (sparse)
-    for (int i = tid; i < static_cast<int>(p.chunk * sizeof(C) / 16); i += kThreads)
-      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  const bool counts = p.tokens != nullptr, biases = p.n_bias > 0;
+  for (int i = tid; i < static_cast<int>(p.chunk * sizeof(C) / 16); i += kThreads)
+    reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) s_n = 0;
   griddep_sync();
   // ---- what depends on no other load is asked for first
   const T* x = static_cast<const T*>(p.x) + b * p.ldx + c0;
   T* y = static_cast<T*>(p.y) + b * p.ldy + c0;
-  const bool in_place = p.x == p.y;
-  const bool vec_in = (reinterpret_cast<uintptr_t>(x) & 15) == 0, vec_out = (reinterpret_cast<uintptr_t>(y) & 15) == 0;
   const int* t = counts ? p.tokens + b * p.ldt : nullptr;
   const bool vec_t = (reinterpret_cast<uintptr_t>(t) & 15) == 0;
   int4 head[HEADS];
@@ -210,63 +276,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
     if (p.frequency) freq = p.frequency[b];
     if (p.presence) pres = p.presence[b];
   }
-  const uint8_t* mask = nullptr;  // bit v of the row, as bytes from the chunk's first column on
-  if (p.mask) {
-    const int r = p.mask_rows ? p.mask_rows[b] : b;
-    if (r >= 0 && r < p.n_masks) mask = reinterpret_cast<const uint8_t*>(p.mask + r * p.ldm) + (c0 >> 3);
-  }
-  constexpr int STEP = kThreads * VEC;
-  // (chunks and steps are multiples of 64 columns: the bits of a piece lie in one byte)
-  auto bits_of = [&](int i) { return mask && i < n ? mask[i >> 3] >> (i & 7) & kAll : kAll; };
-  auto masked = [&](Piece<T>& piece, uint32_t bits) { if (bits != kAll) piece.mask(bits); };
-  if (!sparse) {  // no rule but the mask: straight through, two pieces ahead
-    if (in_place && !mask) return;
-    if (vec_in && vec_out && !in_place) {
-      const uint4* src = reinterpret_cast<const uint4*>(x) + tid;
-      uint4* dst = reinterpret_cast<uint4*>(y) + tid;
-      const uint8_t* bits = mask ? mask + (tid * VEC >> 3) : nullptr;
-      const int whole = n / VEC;
-#pragma unroll 4
-      for (int i = tid; i < whole; i += kThreads) {
-        Piece<T> cur{*src};
-        if (bits) {
-          masked(cur, *bits >> (tid * VEC & 7) & kAll);
-          bits += STEP >> 3;
-        }
-        *dst = cur.w;
-        src += kThreads;
-        dst += kThreads;
-      }
-      const int i = whole * VEC + tid;
-      if (i < n) y[i] = mask && !(mask[i >> 3] >> (i & 7) & 1) ? put<T>(-INFINITY) : x[i];
-      return;
-    }
-    Piece<T> next[2];
-    uint32_t next_bits[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = tid * VEC + k * STEP;
-      if (i < n) next[k].load(x, i, n, vec_in);
-      next_bits[k] = bits_of(i);
-    }
-    for (int i = tid * VEC; i < n; i += STEP) {
-      Piece<T> cur = next[0];
-      const uint32_t bits = next_bits[0];
-      next[0] = next[1];
-      next_bits[0] = next_bits[1];
-      if (i + 2 * STEP < n) {
-        next[1].load(x, i + 2 * STEP, n, vec_in);
-        next_bits[1] = bits_of(i + 2 * STEP);
-      }
-      masked(cur, bits);
-      if (!in_place || bits != kAll) cur.store(y, i, n, vec_out);
-    }
-    return;
-  }
+  const uint8_t* mask = mask_of(p, b, c0);
+  len = max(0, min(len, p.L));
+  prompt = min(prompt, len);
+  const bool few = (static_cast<long long>(len) + p.n_bias) * kFew < static_cast<long long>(p.V) * static_cast<int>(sizeof(T));
+  const bool staged = p.staged && !(p.x == p.y && !mask && few);
+  const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   // the chunk into shared memory, at the same place in a 16-byte unit as it has in memory
-  const int phase = p.staged ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
   T* s_x = reinterpret_cast<T*>(s_chunk) + phase;
-  if (p.staged) {
+  if (staged) {
     const int lead = min(n, (VEC - phase) % VEC), units = (n - lead) / VEC, done = lead + units * VEC;
     const T* src = x + lead + tid * VEC;
     uint32_t dst = smem_u32(s_x + lead + tid * VEC);
@@ -298,8 +316,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
     __syncthreads();  // a column with a bias is on the list before a token comes to it
   }
   if (counts) {
-    len = max(0, min(len, p.L));
-    prompt = min(prompt, len);
     // whole warps: the new columns of its 128 tokens get their places on the list with one addition
     auto count4 = [&](const int4& u, int i) {
       const int token[4] = {u.x, u.y, u.z, u.w};
@@ -338,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();  // counts, list and chunk
-  T* to = p.staged ? s_x : y;
+  T* to = staged ? s_x : y;
   const int on_list = s_n;
   auto rewrite = [&](unsigned j, float f) {
     const uint32_t w = *word_of(j) >> shift_of(j);
@@ -357,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
     }
     to[j] = put<T>(f);  // (rounded once: a masked column is overwritten below)
   };
-  if (p.staged) {
+  if (staged) {
     for (int i = tid; i < on_list; i += kThreads) rewrite(s_list[i], get<T>(s_x[s_list[i]]));
   } else {
     // in place the columns come from HBM: four are asked for before the first is worked on
@@ -372,33 +388,26 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
       }
     }
   }
-  if (!p.staged) return;
+  if (!staged) return;
   __syncthreads();
-  const int whole = n / VEC, shift = phase * static_cast<int>(sizeof(T));
-  const uint4* src = reinterpret_cast<const uint4*>(s_chunk) + tid;
-  T* dst = y + tid * VEC;
-  const uint8_t* row_bits = reinterpret_cast<const uint8_t*>(s_mask);
-  const uint8_t* bits = mask ? row_bits + (tid * VEC >> 3) : nullptr;
+  const Cut<T> cut(y, n);
+  const int rest = cut.rest(tid);
+  if (rest < n) y[rest] = mask && !(s_mask[rest >> 5] >> (rest & 31) & 1) ? put<T>(-INFINITY) : s_x[rest];
+  const int shift = (phase + cut.first) % VEC * static_cast<int>(sizeof(T));
+  const uint4* src = reinterpret_cast<const uint4*>(s_chunk) + (phase + cut.first) / VEC + tid;
+  uint4* dst = reinterpret_cast<uint4*>(y + cut.first) + tid;
 #pragma unroll 2
-  for (int i = tid; i < whole; i += kThreads) {
+  for (int i = cut.first + tid * VEC; i < cut.behind; i += STEP) {
     Piece<T> cur;
     cur.load_shared(src, shift);
-    if (bits) {
-      masked(cur, *bits >> (tid * VEC & 7) & kAll);
-      bits += STEP >> 3;
+    if (mask) {
+      const uint32_t bits = __funnelshift_r(s_mask[i >> 5], s_mask[(i >> 5) + 1], i & 31) & kAll;
+      if (bits != kAll) cur.mask(bits);
     }
-    if (vec_out) {
-      *reinterpret_cast<uint4*>(dst) = cur.w;
-    } else {
-      const T* e = reinterpret_cast<const T*>(&cur.w);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) dst[k] = e[k];
-    }
+    *dst = cur.w;
     src += kThreads;
-    dst += STEP;
+    dst += kThreads;
   }
-  const int i = whole * VEC + tid;
-  if (i < n) y[i] = mask && !(row_bits[i >> 3] >> (i & 7) & 1) ? put<T>(-INFINITY) : s_x[i];
 }
 
 // Columns of a CTA: a row in as many equal chunks as fill one wave of CTAs, of at most `most` columns.
@@ -412,21 +421,16 @@ int chunk_of(int B, int V, int most) {
 
 template <typename T, typename C>
 int launch(Params& p, int B, cudaStream_t stream) {
-  const bool sparse = p.tokens || p.n_bias > 0;
-  p.staged = sparse && !(p.x == p.y && !p.mask);
   // a list holds each column once, and no more than there are tokens and biases
+  const long long list = static_cast<long long>(p.tokens ? p.L : 0) + p.n_bias;
+  p.staged = p.x != p.y || p.mask || list * kFew >= static_cast<long long>(p.V) * static_cast<int>(sizeof(T));
   const double bytes = sizeof(C) + (p.staged ? sizeof(T) + (p.mask ? 0.125 : 0.) : 0.);
   constexpr int tail = 64;
-  const long long list = static_cast<long long>(p.tokens ? p.L : 0) + p.n_bias;
-  long long most = 65536;
-  if (sparse) {
-    most = static_cast<long long>((kSmem - tail) / (bytes + 2));
-    if (list < most) most = static_cast<long long>((kSmem - tail - 2 * list) / bytes);
-  }
+  long long most = static_cast<long long>((kSmem - tail) / (bytes + 2));
+  if (list < most) most = static_cast<long long>((kSmem - tail - 2 * list) / bytes);
   p.chunk = chunk_of(B, p.V, static_cast<int>(most / 64 * 64));
   const size_t smem =
-      sparse ? tail + static_cast<size_t>(p.chunk * bytes) + 2 * static_cast<size_t>(list < p.chunk ? list : p.chunk)
-             : 0;
+      tail + static_cast<size_t>(p.chunk * bytes) + 2 * static_cast<size_t>(list < p.chunk ? list : p.chunk);
   constexpr int kMaxDev = 64;
   static bool ready[kMaxDev] = {false};
   int dev = 0;
@@ -437,6 +441,18 @@ int launch(Params& p, int B, cudaStream_t stream) {
     ready[dev] = true;
   }
   launch_kernel(process_kernel<T, C>, dim3((p.V + p.chunk - 1) / p.chunk, B), dim3(kThreads), smem, stream, 1, p);
+  return launch_status();
+}
+
+template <typename T>
+int launch(Params& p, int B, cudaStream_t stream) {
+  if (p.tokens || p.n_bias > 0) {
+    const bool small = p.L <= static_cast<int>(Word<uint16_t>::kCount);  // no count can overflow
+    return small ? launch<T, uint16_t>(p, B, stream) : launch<T, uint32_t>(p, B, stream);
+  }
+  if (p.x == p.y && !p.mask) return NL_OK;
+  p.chunk = chunk_of(B, p.V, 65536);
+  launch_kernel(mask_kernel<T>, dim3((p.V + p.chunk - 1) / p.chunk, B), dim3(kThreads), 0, stream, 1, p);
   return launch_status();
 }
 
@@ -460,8 +476,5 @@ extern "C" int nl_process_logits(const nl_process_logits_args* args, cudaStream_
   lg::Params p{a.logits, a.ldx, a.out, a.ldy, a.tokens, a.ldt, a.lens, a.prompt_lens, a.repetition, a.frequency,
                a.presence, a.bias_ids, a.bias, a.ldb, static_cast<const uint32_t*>(a.mask), a.ldm, a.mask_rows, V,
                a.tokens ? a.L : 0, a.n_bias, a.n_masks, 0, 0};
-  const bool small = p.L <= static_cast<int>(lg::Word<uint16_t>::kCount);  // no count can overflow
-  if (dtype == NL_F32)
-    return small ? lg::launch<float, uint16_t>(p, B, stream) : lg::launch<float, uint32_t>(p, B, stream);
-  return small ? lg::launch<__nv_bfloat16, uint16_t>(p, B, stream) : lg::launch<__nv_bfloat16, uint32_t>(p, B, stream);
+  return dtype == NL_F32 ? lg::launch<float>(p, B, stream) : lg::launch<__nv_bfloat16>(p, B, stream);
 }

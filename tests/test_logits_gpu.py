@@ -92,6 +92,46 @@ def test_parts(cuda, parts, dtype):
     assert (wide[:, :3] == 7).all() and (wide[:, 5004:] == 7).all()
 
 
+@pytest.mark.parametrize("V", [1, 7, 1000, 4099])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_in_place_rows_with_few_and_many_tokens(cuda, V, dtype):
+    """Rows of one call that are worked on where they lie and through a copy, at every
+    place in a 16-byte unit; what lies between the rows stays."""
+    x, kw = make(cuda, 9, V, V, dtype, 700, 3, V)
+    kw.pop("mask")
+    kw["lens"][:] = [700, 0, 1, 3, 700, 20, 699, 512, 40]
+    kw["prompt_lens"] = kw["lens"] // 2
+    for off in (0, 1, 3):
+        buf = torch.full((9 * (V + 3) + off,), 77.0, device=cuda).to(dtype)
+        z = buf[off:].view(9, V + 3)[:, :V]
+        z.copy_(x)
+        assert call(z, kw, out=z) is z
+        torch.cuda.synchronize()
+        check(z, x, kw)
+        assert (buf[off:].view(9, V + 3)[:, V:] == 77).all() and (buf[:off] == 77).all()
+
+
+@pytest.mark.parametrize("rules", [("mask",), ("mask", "tokens", "lens", "repetition"), ("bias_ids", "bias"), ()])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_at_different_places_of_a_unit(cuda, rules, dtype):
+    """Input and output rows that begin at different bytes of a 16-byte unit, rows of a
+    few columns among them."""
+    for V in (1, 5, 9, 33, 2051, 9001):
+        x, kw = make(cuda, 5, V, V, dtype, 30, 3, V)
+        kw = {k: kw[k] for k in rules}
+        for a, b in ((0, 1), (1, 0), (3, 6), (2, 2), (5, 5)):
+            src = torch.full((5 * (V + a) + 8,), 77.0, device=cuda).to(dtype)
+            dst = torch.full((5 * (V + b) + 8,), 77.0, device=cuda).to(dtype)
+            xi, yi = src[a:a + 5 * (V + a)].view(5, V + a)[:, :V], dst[b:b + 5 * (V + b)].view(5, V + b)[:, :V]
+            xi.copy_(x)
+            call(xi, kw, out=yi)
+            torch.cuda.synchronize()
+            check(yi, x, kw)
+            left = dst.clone()
+            left[b:b + 5 * (V + b)].view(5, V + b)[:, :V] = 77.0
+            assert (left == 77).all()
+
+
 def test_mask_rows_and_nothing_left(cuda):
     x = torch.randn(4, 100, device=cuda)
     mask = torch.zeros(2, 4, dtype=torch.int32, device=cuda)
