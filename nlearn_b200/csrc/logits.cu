@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   uint8_t* s_chunk = smem + p.chunk * sizeof(C);
   uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_chunk + (p.staged ? (p.chunk + 2 * VEC) * sizeof(T) : 0));
   uint16_t* s_list = reinterpret_cast<uint16_t*>(s_mask + (p.staged && p.mask ? p.chunk / 32 + 1 : 0));
-  __shared__ int s_ids[kList];
-  __shared__ float s_add[kList];
+  __shared__ __align__(16) int s_ids[kList];  // -1 past the last
+  __shared__ __align__(16) float s_add[kList];
   __shared__ int s_n;
   const int tid = threadIdx.x;
   const int b = blockIdx.y, c0 = blockIdx.x * p.chunk, n = min(p.chunk, p.V - c0);
@@ -365,9 +365,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
     }
     if (w & W::kNamed) {  // its entries of the list, in order
       const int id = c0 + static_cast<int>(j), kept = min(p.n_bias, kList);
-#pragma unroll 4
-      for (int m = 0; m < kept; ++m)
-        if (s_ids[m] == id) f += s_add[m];
+#pragma unroll 2
+      for (int m = 0; m < kept; m += 4) {
+        const int4 at = *reinterpret_cast<const int4*>(s_ids + m);
+        const float4 by = *reinterpret_cast<const float4*>(s_add + m);
+        if (at.x == id) f += by.x;
+        if (at.y == id) f += by.y;
+        if (at.z == id) f += by.z;
+        if (at.w == id) f += by.w;
+      }
       for (int m = kept; m < p.n_bias; ++m)
         if (ids[m] == id) f += add[m];
     }

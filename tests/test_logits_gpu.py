@@ -132,6 +132,14 @@ def test_rows_at_different_places_of_a_unit(cuda, rules, dtype):
             assert (left == 77).all()
 
 
+@pytest.mark.parametrize("n_bias", [1, 3, 4, 5, 127, 128, 129, 600])
+def test_lists_of_biases(cuda, n_bias):
+    x, kw = make(cuda, 3, 500, 500, torch.float32, 40, n_bias, n_bias)
+    y = call(x, kw)
+    torch.cuda.synchronize()
+    check(y, x, kw)
+
+
 def test_mask_rows_and_nothing_left(cuda):
     x = torch.randn(4, 100, device=cuda)
     mask = torch.zeros(2, 4, dtype=torch.int32, device=cuda)
