@@ -27,6 +27,8 @@ replaced by an integer seed).
 """
 from __future__ import annotations
 
+import functools
+
 import numpy as np
 import torch
 
@@ -210,6 +212,15 @@ class Decoder(_DecodeStep):
         return self.out[:, :Pl + n_tokens].cpu().numpy()
 
 
+def _on_device(method):
+    """Run a method with the decoder's device current."""
+    @functools.wraps(method)
+    def run(self, *args, **kw):
+        with torch.cuda.device(self.P.device):
+            return method(self, *args, **kw)
+    return run
+
+
 class PagedDecoder(_DecodeStep):
     """Generation for rows that come and go, each with a prompt, a length and
     rules of its own, over a paged KV cache.
@@ -325,20 +336,22 @@ class PagedDecoder(_DecodeStep):
             self._rules[row] = self._rules[row] - {"mask"}
             return
         ids = np.asarray(list(allowed), np.int64)
-        if ids.size and (ids.min() < 0 or ids.max() >= self.cfg.vocab):
-            raise ValueError("allowed token ids outside the vocabulary")
+        if not ids.size or ids.min() < 0 or ids.max() >= self.cfg.vocab:
+            raise ValueError("allowed must name at least one token, all inside the vocabulary")
         words = np.zeros(self.mask.shape[1], np.uint32)
         np.bitwise_or.at(words, ids // 32, np.uint32(1) << (ids % 32).astype(np.uint32))
         self.mask[row] = torch.from_numpy(words.view(np.int32)).to(self.mask.device)
         self.mask_rows[row] = row
         self._rules[row] = self._rules[row] | {"mask"}
 
+    @_on_device
     def add(self, prompts, *, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
             bias: dict | None = None, allowed=None) -> list[int]:
         """Admit prompts (a list of 1-D id arrays) to free rows, run them and
         draw the first token of each; -> the rows.  The rules (see
         ``process_logits``) hold for all of them; ``allowed`` is a set of token ids."""
         prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        allowed = None if allowed is None else list(allowed)  # (read once for each row)
         rows = self.free_rows()[:len(prompts)]
         if len(rows) < len(prompts):
             raise RuntimeError(f"{len(prompts)} prompts, {len(rows)} free rows")
@@ -400,6 +413,7 @@ class PagedDecoder(_DecodeStep):
             self.new[row] = 1
         return rows
 
+    @_on_device
     def step(self, n: int = 1, use_graph: bool = True) -> None:
         """Draw n tokens for every row in use."""
         for _ in range(n):
@@ -433,6 +447,7 @@ class PagedDecoder(_DecodeStep):
         """The row's prompt and the tokens drawn so far."""
         return self.out[row, :self._len[row]].cpu().numpy()
 
+    @_on_device
     def release(self, rows) -> None:
         """End rows: their pages are free, the rows may be admitted anew."""
         done = torch.zeros(self.B, dtype=torch.int32)

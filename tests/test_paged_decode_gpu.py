@@ -156,6 +156,15 @@ def test_entry_point(cuda, params):
     assert _lib.device_error() == 0
 
 
+def test_allowed_of_several_rows(cuda, params):
+    """Any iterable of ids holds for every row of the call."""
+    dec = PagedDecoder(params, CFG, max_batch=3)
+    rows = dec.add(prompts([4, 9, 5]), allowed=(i for i in range(50, 53)))
+    dec.step(4)
+    for r, n in zip(rows, (4, 9, 5)):
+        assert all(50 <= t < 53 for t in dec.tokens(r)[n:])
+
+
 def test_refusals(cuda, params):
     dec = PagedDecoder(params, CFG, max_batch=2, n_pages=3, page_size=16, max_len=48)
     with pytest.raises(RuntimeError):
@@ -170,6 +179,8 @@ def test_refusals(cuda, params):
         dec.add(prompts([3]), bias={i: 1.0 for i in range(33)})
     with pytest.raises(ValueError):
         dec.add(prompts([3]), allowed=[CFG.vocab])
+    with pytest.raises(ValueError):
+        dec.add(prompts([3]), allowed=[])
     with pytest.raises(ValueError):
         dec.release([0])
     r, s = dec.add(prompts([15, 32]))
