@@ -436,7 +436,7 @@ NL_API int nl_update_block_tables(const nl_update_block_tables_args* args, cudaS
  *   (bit v % 32 of word v / 32) is 0 becomes -inf; row b uses mask row
  *   mask_rows[b] (below 0 or past n_masks: none), or b where mask_rows is NULL.
  * Tokens and bias ids outside [0, V) are ignored.  Arithmetic is f32, rounded
- * once.  B <= 65535. */
+ * once.  B <= 65535; V, L and n_bias below 2^30. */
 typedef struct {
   const void* logits;
   void* out;

@@ -61,9 +61,9 @@ void same_place(const at::Tensor& t, const char* name, int index) {
   if (place(t, name) != index)
     refuse(PyExc_ValueError, "%s is on cuda:%d, expected cuda:%d", name, static_cast<int>(t.get_device()), index);
 }
-void no_grad(const at::Tensor& t, const char* op) {
+void no_grad(const at::Tensor& t, const char* name) {
   if (t.requires_grad() && c10::GradMode::is_enabled())
-    refuse(PyExc_RuntimeError, "%s has no backward: call it under torch.no_grad()", op);
+    refuse(PyExc_RuntimeError, "%s: the serving operators have no backward, call them under torch.no_grad()", name);
 }
 int whole(PyObject* o, const char* name) {
   const long long x = PyLong_AsLongLong(o);
@@ -91,6 +91,7 @@ E* vector(const at::Tensor& t, const char* name, at::ScalarType type, int64_t n,
     refuse(type == at::kInt ? PyExc_TypeError : PyExc_ValueError, "%s must be %s, got %s", name, c10::toString(type),
            type_name(t));
   }
+  if (type == at::kFloat) no_grad(t, name);
   if (t.dim() != 1 || t.size(0) != n || (n > 1 && t.stride(0) != 1))
     refuse(PyExc_ValueError, "%s must be a contiguous vector of %lld elements, got shape %s with strides %s", name,
            static_cast<long long>(n), list(t.sizes()).c_str(), list(t.strides()).c_str());
@@ -138,6 +139,8 @@ struct Caches {
 Caches caches(const at::Tensor& k, const at::Tensor& v, int index) {
   same_place(k, "k_cache", index);
   same_place(v, "v_cache", index);
+  no_grad(k, "k_cache");
+  no_grad(v, "v_cache");
   const auto type = k.scalar_type();
   if ((type != at::kBFloat16 && type != at::kFloat8_e4m3fn) || v.scalar_type() != type)
     refuse(PyExc_TypeError, "caches must both be BFloat16 or Float8_e4m3fn, got %s and %s", type_name(k), type_name(v));
@@ -203,7 +206,7 @@ class Cutter {
 PyObject* attention(PyObject* const* a) {
   const at::Tensor& q0 = tensor(a[0], "q");
   const int index = place(q0, "q");
-  no_grad(q0, "paged_decode_attention");
+  no_grad(q0, "q");
   if (q0.dim() != 3) refuse(PyExc_ValueError, "q must be [batch, heads, head_dim], got %s", list(q0.sizes()).c_str());
   const Caches c = caches(tensor(a[1], "k_cache"), tensor(a[2], "v_cache"), index);
   const int64_t B = q0.size(0), Hq = q0.size(1), d = q0.size(2);
@@ -218,8 +221,8 @@ PyObject* attention(PyObject* const* a) {
   if ((a[5] == Py_None) != (a[6] == Py_None)) refuse(PyExc_ValueError, "k_new and v_new come together");
   if (a[5] != Py_None) {
     const at::Tensor &k0 = tensor(a[5], "k_new"), &v0 = tensor(a[6], "v_new");
-    no_grad(k0, "paged_decode_attention");
-    no_grad(v0, "paged_decode_attention");
+    no_grad(k0, "k_new");
+    no_grad(v0, "v_new");
     kn = rows(k0, "k_new", B, c.heads, d, index);
     vn = rows(v0, "v_new", B, c.heads, d, index);
     if (kn.strides() != vn.strides()) {
@@ -236,6 +239,7 @@ PyObject* attention(PyObject* const* a) {
   } else {
     out = tensor(a[10], "out");
     same_place(out, "out", index);
+    no_grad(out, "out");
     if (out.sizes() != q0.sizes() || out.scalar_type() != at::kBFloat16 || out.stride(2) != 1)
       refuse(PyExc_ValueError, "out must be bfloat16 %s with contiguous rows", list(q0.sizes()).c_str());
   }
@@ -244,6 +248,7 @@ PyObject* attention(PyObject* const* a) {
   if (a[11] != Py_None) {
     const at::Tensor& t = tensor(a[11], "lse");
     same_place(t, "lse", index);
+    no_grad(t, "lse");
     if (t.scalar_type() != at::kFloat || t.dim() != 2 || t.size(0) != B || t.size(1) != Hq ||
         (Hq > 1 && t.stride(1) != 1))
       refuse(PyExc_ValueError, "lse must be float32 (%lld, %lld) with contiguous rows", static_cast<long long>(B),
@@ -276,8 +281,8 @@ PyObject* attention(PyObject* const* a) {
 PyObject* kv_write(PyObject* const* a) {
   const at::Tensor &k0 = tensor(a[0], "k"), &v0 = tensor(a[1], "v");
   const int index = place(k0, "k");
-  no_grad(k0, "paged_kv_write");
-  no_grad(v0, "paged_kv_write");
+  no_grad(k0, "k");
+  no_grad(v0, "v");
   const Caches c = caches(tensor(a[2], "k_cache"), tensor(a[3], "v_cache"), index);
   if (c.d & (c.dtype == NL_E4M3 ? 15 : 7))
     refuse(PyExc_ValueError, "head_dim %d: cache rows must be whole 16-byte pieces", c.d);
@@ -358,17 +363,18 @@ PyObject* update_tables(PyObject* const* a) {
 PyObject* logits(PyObject* const* a) {
   const at::Tensor& x = tensor(a[0], "logits");
   const int index = place(x, "logits");
-  no_grad(x, "process_logits");
+  no_grad(x, "logits");
   const auto type = x.scalar_type();
   if (type != at::kFloat && type != at::kBFloat16)
     refuse(PyExc_TypeError, "logits must be float32 or bfloat16, got %s", type_name(x));
   const bool f32 = type == at::kFloat;
+  constexpr int kMost = (1 << 30) - 1;
   if (x.dim() != 2) refuse(PyExc_ValueError, "logits must be [batch, vocab], got %s", list(x.sizes()).c_str());
   const int64_t B = x.size(0), V = x.size(1);
   auto good_rows = [&](const at::Tensor& t) { return (V <= 1 || t.stride(1) == 1) && (B <= 1 || t.stride(0) >= V); };
   if (!good_rows(x)) refuse(PyExc_ValueError, "rows of logits must be contiguous and not overlap");
-  if (B > 65535 || V == 0 || V > INT32_MAX)
-    refuse(PyExc_ValueError, "logits must have at most 65535 rows and at least one column, got %s",
+  if (B > 65535 || V == 0 || V > kMost)
+    refuse(PyExc_ValueError, "logits must have at most 65535 rows and 1 to 2**30 - 1 columns, got %s",
            list(x.sizes()).c_str());
   at::Tensor y;
   if (a[11] == Py_None) {
@@ -378,6 +384,7 @@ PyObject* logits(PyObject* const* a) {
   } else {
     y = tensor(a[11], "out");
     same_place(y, "out", index);
+    no_grad(y, "out");
     if (y.sizes() != x.sizes() || y.scalar_type() != type)
       refuse(PyExc_ValueError, "out must have the shape and type of logits");
     if (!good_rows(y)) refuse(PyExc_ValueError, "rows of out must be contiguous and not overlap");
@@ -402,6 +409,7 @@ PyObject* logits(PyObject* const* a) {
     args.repetition = vector_or_none<float>(a[4], "repetition", at::kFloat, B, index);
     args.frequency = vector_or_none<float>(a[5], "frequency", at::kFloat, B, index);
     args.presence = vector_or_none<float>(a[6], "presence", at::kFloat, B, index);
+    if (t.cols > kMost) refuse(PyExc_ValueError, "tokens must have fewer than 2**30 columns, got %d", t.cols);
     if (t.cols > 0) {
       args.tokens = t.p;
       args.ldt = t.ld;
@@ -416,7 +424,7 @@ PyObject* logits(PyObject* const* a) {
   if (a[7] != Py_None) {
     bias_ids = tensor(a[7], "bias_ids");
     bias = tensor(a[8], "bias");
-    no_grad(bias, "process_logits");
+    no_grad(bias, "bias");
     same_place(bias, "bias", index);
     matrix(bias_ids, "bias_ids", B, index);
     if (bias.scalar_type() != at::kFloat || bias.sizes() != bias_ids.sizes())
@@ -430,6 +438,7 @@ PyObject* logits(PyObject* const* a) {
     args.bias = static_cast<const float*>(bias.data_ptr());
     args.ldb = m.ld;
     args.n_bias = m.cols;
+    if (m.cols > kMost) refuse(PyExc_ValueError, "bias must have fewer than 2**30 columns, got %d", m.cols);
   }
   if (a[9] != Py_None) {
     const Matrix m = matrix(tensor(a[9], "mask"), "mask", -1, index);

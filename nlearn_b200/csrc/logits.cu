@@ -471,6 +471,8 @@ extern "C" int nl_process_logits(const nl_process_logits_args* args, cudaStream_
   if (!args) return NL_ERR_SHAPE;
   const nl_process_logits_args& a = *args;
   const int B = a.B, V = a.V, dtype = a.dtype;
+  constexpr int kMost = (1 << 30) - 1;  // columns, tokens and biases of a row: indices and counts stay in 32 bits
+  if (V > kMost || a.n_bias > kMost || (a.tokens && a.L > kMost)) return NL_ERR_TOO_LARGE;
   if (B <= 0 || B > 65535 || V <= 0 || a.ldx < V || a.ldy < V || !a.logits || !a.out) return NL_ERR_SHAPE;
   if (dtype != NL_F32 && dtype != NL_BF16) return NL_ERR_DTYPE;
   if (a.logits == a.out && B > 1 && a.ldx != a.ldy) return NL_ERR_SHAPE;

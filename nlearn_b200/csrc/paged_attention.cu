@@ -204,13 +204,14 @@ struct Walk {
   int b, base;   // sequence of unit u (or an earlier one), units before it
   __device__ __forceinline__ bool next(const Params& p, Run& r) {
     while (u < u1) {
-      int len, w;
-      for (;; ++b) {
+      int len = 0, w = 0;
+      for (; b < p.B; ++b) {
         len = clamp_len(p, b);
         w = weight_of<UNIT, OVER>(len);
         if (u - base < w * segs) break;
         base += w * segs;
       }
+      if (b >= p.B) return false;  // (lengths that changed under the call)
       const int local = u - base;
       r.b = b;
       r.len = len;

@@ -234,7 +234,9 @@ __global__ void __launch_bounds__(kThreads) update_tables_kernel(const TablePara
 
   // ---- slots, four tokens a thread
   const bool vec = ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15) == 0;
-  for (int t = 4 * (rank * threads + tid); t < p.tokens; t += 4 * nctas * threads) {
+  // (unsigned: the last step may pass 2^31)
+  for (unsigned t0 = 4 * (rank * threads + tid); t0 < static_cast<unsigned>(p.tokens); t0 += 4 * nctas * threads) {
+    const int t = static_cast<int>(t0);
     int slot[4], pos[4];
     int lo = 0;
     if (t < tok) {
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) update_tables_kernel(const TablePara
     for (int k = 0; k < 4; ++k) slot[k] = entry[k] ? __ldcg(entry[k]) : -1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) slot[k] = slot[k] >= 0 && slot[k] < p.n_pages ? slot[k] * P + off[k] : -1;
-    if (vec && t + 4 <= p.tokens) {
+    if (vec && t <= p.tokens - 4) {
       *reinterpret_cast<int4*>(p.slots + t) = make_int4(slot[0], slot[1], slot[2], slot[3]);
       *reinterpret_cast<int4*>(p.positions + t) = make_int4(pos[0], pos[1], pos[2], pos[3]);
     } else {

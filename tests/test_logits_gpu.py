@@ -207,6 +207,8 @@ def test_graph_and_refusals(cuda):
            (TypeError, dict(tokens=i.long(), lens=t["lens"]), x), (ValueError, dict(bias=t["bias"]), x),
            (ValueError, dict(bias=t["bias"][:, :1], bias_ids=t["bias_ids"]), x),
            (ValueError, dict(mask=t["mask"][:, :5]), x), (ValueError, dict(mask=t["mask"][:2]), x),
+           (RuntimeError, dict(tokens=i, lens=t["lens"], presence=one.clone().requires_grad_()), x),
+           (RuntimeError, dict(), x.clone().requires_grad_()),
            (ValueError, dict(mask_rows=t["lens"]), x), (ValueError, dict(out=x[:, :10]), x),
            (ValueError, dict(tokens=i, lens=t["lens"], frequency=one.double()), x),
            (ValueError, dict(out=torch.empty(4, 3000, device=cuda).flatten()[100:9100].view(3, 3000)), x.cpu())]

@@ -88,6 +88,9 @@ def logits(**kw):
 
 @pytest.mark.parametrize("kw,code", [(dict(B=0), "NL_ERR_SHAPE"), (dict(B=65536), "NL_ERR_SHAPE"),
                                      (dict(ldx=99), "NL_ERR_SHAPE"), (dict(ldy=99), "NL_ERR_SHAPE"),
+                                     (dict(V=2**30, ldx=2**31, ldy=2**31), "NL_ERR_TOO_LARGE"),
+                                     (dict(tok=P, lens=P, ldt=2**31, L=2**30), "NL_ERR_TOO_LARGE"),
+                                     (dict(ids=P, bias=P, ldb=2**31, n_bias=2**30), "NL_ERR_TOO_LARGE"),
                                      (dict(dt=2), "NL_ERR_DTYPE"), (dict(tok=P, ldt=5, L=5), "NL_ERR_SHAPE"),
                                      (dict(tok=P, lens=P, ldt=4, L=5), "NL_ERR_SHAPE"),
                                      (dict(n_bias=3), "NL_ERR_SHAPE"), (dict(n_bias=-1), "NL_ERR_SHAPE"),

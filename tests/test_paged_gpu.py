@@ -514,6 +514,10 @@ def test_wrapper_refusals(cuda):
         (ValueError, lambda: call(q.cpu(), k, v, table, ln)),
         (ValueError, lambda: call(q, k, v, table, ln.cpu())),
         (RuntimeError, lambda: call(q.clone().requires_grad_(), k, v, table, ln)),
+        (RuntimeError, lambda: call(q, k.clone().requires_grad_(), v, table, ln)),
+        (RuntimeError, lambda: call(q, k, v, table, ln, out=torch.empty_like(q).requires_grad_())),
+        (RuntimeError, lambda: call(q, k.to(E4M3), v.to(E4M3), table, ln,
+                                    k_scale=torch.ones(2, device=cuda, requires_grad=True))),
         (ValueError, lambda: paged_kv_write(q, q, k, v, ln)),
         (TypeError, lambda: paged_kv_write(q[:, :2], q[:, :2], k, v, ln.float())),
         (ValueError, lambda: update_block_tables(table, ln, ln, ln, ln[:1], 0, 5)),
