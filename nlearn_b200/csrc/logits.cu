@@ -155,15 +155,24 @@ struct Piece {
   }
 };
 
-// Where a chunk of n columns is cut into pieces: behind the columns before the output's first
-// 16-byte unit.
+// Columns before the first 128-byte line of a row that begins at x.
+template <typename T>
+__device__ __forceinline__ int before_line(const T* x, int n) {
+  constexpr int LINE = 128 / sizeof(T);
+  return min(n, static_cast<int>(-(reinterpret_cast<uintptr_t>(x) / sizeof(T)) % LINE));
+}
+template <typename T>
+__device__ __forceinline__ int phase_of(const T* x) {  // place in a 16-byte unit
+  return static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+}
+// Where a chunk of n columns is cut into pieces: from the output's first line on, so that a warp
+// writes whole lines.
 template <typename T>
 struct Cut {
-  int phase, first, behind;
+  int first, behind;
   __device__ __forceinline__ Cut(const T* y, int n) {
     constexpr int VEC = Piece<T>::VEC;
-    phase = static_cast<int>((reinterpret_cast<uintptr_t>(y) & 15) / sizeof(T));
-    first = min(n, (VEC - phase) % VEC);
+    first = before_line(y, n);
     behind = first + (n - first) / VEC * VEC;
   }
   // the i-th column that is in no piece
@@ -198,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) mask_kernel(const Params p) {
   const uint8_t* mask = mask_of(p, b, c0);
   if (in_place && !mask) return;
   const Cut<T> cut(y, n);
-  const bool aligned = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) == cut.phase;
+  const bool aligned = phase_of(x) == phase_of(y);
   // bits i .. i + VEC, all of which exist
   auto bits_of = [&](int i) -> uint32_t {
     if (!mask) return kAll;
@@ -281,11 +290,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   prompt = min(prompt, len);
   const bool few = (static_cast<long long>(len) + p.n_bias) * kFew < static_cast<long long>(p.V) * static_cast<int>(sizeof(T));
   const bool staged = p.staged && !(p.x == p.y && !mask && few);
-  const int phase = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int phase = phase_of(x);
   // the chunk into shared memory, at the same place in a 16-byte unit as it has in memory
   T* s_x = reinterpret_cast<T*>(s_chunk) + phase;
   if (staged) {
-    const int lead = min(n, (VEC - phase) % VEC), units = (n - lead) / VEC, done = lead + units * VEC;
+    const int lead = before_line(x, n), units = (n - lead) / VEC, done = lead + units * VEC;
     const T* src = x + lead + tid * VEC;
     uint32_t dst = smem_u32(s_x + lead + tid * VEC);
     for (int i = tid; i < units; i += kThreads) {
