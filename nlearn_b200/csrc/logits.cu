@@ -143,12 +143,12 @@ struct Piece {
       if (!(bits & 8)) w.w = 0xff800000u;
     } else {
       uint32_t* u = &w.x;
+      const uint32_t both = bits | bits << 15;  // even bits below, odd ones 16 places above them
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         // bits 2 k and 2 k + 1 to the tops of the two halves, spread over them
-        const uint32_t lo = bits << (15 - 2 * k), hi = bits << (30 - 2 * k);
         uint32_t keep;
-        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(keep) : "r"((lo & 0xffffu) | (hi & 0xffff0000u)));
+        asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(keep) : "r"(both << (15 - 2 * k)));
         u[k] = (u[k] & keep) | (0xff80ff80u & ~keep);
       }
     }
@@ -411,13 +411,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   const int shift = (phase + cut.first) % VEC * static_cast<int>(sizeof(T));
   const uint4* src = reinterpret_cast<const uint4*>(s_chunk) + (phase + cut.first) / VEC + tid;
   uint4* dst = reinterpret_cast<uint4*>(y + cut.first) + tid;
+  const int begin = cut.first + tid * VEC;
+  const uint32_t* words = s_mask + (begin >> 5);  // (a step is whole words)
 #pragma unroll 2
-  for (int i = cut.first + tid * VEC; i < cut.behind; i += STEP) {
+  for (int i = begin; i < cut.behind; i += STEP) {
     Piece<T> cur;
     cur.load_shared(src, shift);
     if (mask) {
-      const uint32_t bits = __funnelshift_r(s_mask[i >> 5], s_mask[(i >> 5) + 1], i & 31) & kAll;
+      const uint32_t bits = __funnelshift_r(words[0], words[1], begin & 31) & kAll;
       if (bits != kAll) cur.mask(bits);
+      words += STEP / 32;
     }
     *dst = cur.w;
     src += kThreads;
