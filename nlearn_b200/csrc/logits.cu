@@ -24,6 +24,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "host_common.h"
 #include "sm100.cuh"
 
@@ -113,26 +115,23 @@ struct Piece {
     for (int k = 0; k < VEC; ++k) e[k] = x[i + k];
     w = *reinterpret_cast<const uint4*>(e);
   }
-  // From shared memory: the piece that begins `bytes` into the 16-byte unit at u
-  // (the same for all lanes; the unit after it can be read too).
-  __device__ __forceinline__ void load_shared(const uint4* u, int bytes) {
+  // From shared memory: the piece that begins WORD words and `half` bits into the
+  // 16-byte unit at u (WORD < 0: at u; the unit after it can be read too).
+  template <int WORD>
+  __device__ __forceinline__ void load_shared(const uint4* u, int half) {
     const uint4 lo = u[0];
-    if (bytes == 0) {
+    if constexpr (WORD < 0) {
       w = lo;
-      return;
+    } else {
+      const uint4 hi = u[1];
+      const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      if constexpr (sizeof(T) == 4)
+        w = make_uint4(v[WORD], v[WORD + 1], v[WORD + 2], v[WORD + 3]);
+      else
+        w = make_uint4(__funnelshift_r(v[WORD], v[WORD + 1], half), __funnelshift_r(v[WORD + 1], v[WORD + 2], half),
+                       __funnelshift_r(v[WORD + 2], v[WORD + 3], half),
+                       __funnelshift_r(v[WORD + 3], v[WORD + 4], half));
     }
-    const uint4 hi = u[1];
-    uint4 v;
-    uint32_t v4;  // the words from `bytes` on
-    switch (bytes >> 2) {
-      case 0: v = lo, v4 = hi.x; break;
-      case 1: v = make_uint4(lo.y, lo.z, lo.w, hi.x), v4 = hi.y; break;
-      case 2: v = make_uint4(lo.z, lo.w, hi.x, hi.y), v4 = hi.z; break;
-      default: v = make_uint4(lo.w, hi.x, hi.y, hi.z), v4 = hi.w; break;
-    }
-    const int half = (bytes & 2) * 8;
-    w = make_uint4(__funnelshift_r(v.x, v.y, half), __funnelshift_r(v.y, v.z, half),
-                   __funnelshift_r(v.z, v.w, half), __funnelshift_r(v.w, v4, half));
   }
   // columns whose bit is 0 become -inf
   __device__ __forceinline__ void mask(uint32_t bits) {
@@ -413,19 +412,26 @@ __global__ void __launch_bounds__(kThreads, kCtas) process_kernel(const Params p
   uint4* dst = reinterpret_cast<uint4*>(y + cut.first) + tid;
   const int begin = cut.first + tid * VEC;
   const uint32_t* words = s_mask + (begin >> 5);  // (a step is whole words)
+  auto write = [&](auto word) {
 #pragma unroll 2
-  for (int i = begin; i < cut.behind; i += STEP) {
-    Piece<T> cur;
-    cur.load_shared(src, shift);
-    if (mask) {
-      const uint32_t bits = __funnelshift_r(words[0], words[1], begin & 31) & kAll;
-      if (bits != kAll) cur.mask(bits);
-      words += STEP / 32;
+    for (int i = begin; i < cut.behind; i += STEP) {
+      Piece<T> cur;
+      cur.template load_shared<decltype(word)::value>(src, (shift & 2) * 8);
+      if (mask) {
+        const uint32_t bits = __funnelshift_r(words[0], words[1], begin & 31) & kAll;
+        if (bits != kAll) cur.mask(bits);
+        words += STEP / 32;
+      }
+      *dst = cur.w;
+      src += kThreads;
+      dst += kThreads;
     }
-    *dst = cur.w;
-    src += kThreads;
-    dst += kThreads;
-  }
+  };
+  if (shift == 0) write(std::integral_constant<int, -1>{});
+  else if (shift < 4) write(std::integral_constant<int, 0>{});
+  else if (shift < 8) write(std::integral_constant<int, 1>{});
+  else if (shift < 12) write(std::integral_constant<int, 2>{});
+  else write(std::integral_constant<int, 3>{});
 }
 
 // Columns of a CTA: a row in as many equal chunks as fill one wave of CTAs, of at most `most` columns.
