@@ -43,7 +43,7 @@
 // 48 sequences of up to 8192, 32/8 heads of 128, token-major: 130 us, 94 %; one of
 // 131072: 86 us, 95 %; 64 of up to 4097 on an e4m3 cache: 55.6 us, 74 % (the run's
 // start and end, and the join, are the rest: between them a unit takes what its bytes do);
-// 32 of up to 512, 8 heads of 64: 7.6 us, one of 512: 4.7 us (the chain of loads: length, page, tile).
+// 32 of up to 512, 8 heads of 64: 7.5 us, one of 512: 4.5 us (the chain of loads: length, page, tile).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
