@@ -423,6 +423,20 @@ def test_update_tables_wide_and_large_counts(cuda):
     assert plan.n_free.item() == 6 and (plan.slots == -1).all()
 
 
+def test_update_tables_longest_flat_list(cuda):
+    t = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    n = 2**31 - 1
+    table, free = torch.zeros(2, 4, dtype=torch.int32, device=cuda), t(list(range(6)))
+    plan = update_block_tables(table, t([0, 3]), t([20, 2]), free, t([6]), 16, n)
+    torch.cuda.synchronize()
+    assert plan.slots.numel() == n and plan.status.tolist() == [0, 0]
+    # row 0 takes pages 5 and 4, row 1 goes on in its page 0
+    assert plan.slots[:22].tolist() == list(range(80, 96)) + list(range(64, 68)) + [3, 4]
+    assert plan.positions[:22].tolist() == list(range(20)) + [3, 4]
+    for part in (plan.slots, plan.positions):
+        assert part[22:].max().item() == -1 and part[22:].min().item() == -1
+
+
 def test_tables_write_attention_together(cuda):
     """Prompts of ragged lengths, then decode steps with rows that end and
     start again, all in one captured step: outputs equal a plain recompute."""
