@@ -40,8 +40,8 @@
 //     per (sequence, head) merges over distributed shared memory: one launch,
 //     no prefix sums.
 // Neither depends on the order in which CTAs finish.  Measured (B200, share of the 6.56 TB/s of a copy):
-// 48 sequences of up to 8192, 32/8 heads of 128, token-major: 130 us, 94 %; one of
-// 131072: 86 us, 95 %; 64 of up to 4097 on an e4m3 cache: 55.6 us, 74 % (the run's
+// 48 sequences of up to 8192, 32/8 heads of 128, token-major: 128 us, 96 %; one of
+// 131072: 85 us, 96 %; 64 of up to 4097 on an e4m3 cache: 53 us, 78 % (the run's
 // start and end, and the join, are the rest: between them a unit takes what its bytes do);
 // 32 of up to 512, 8 heads of 64: 7.5 us, one of 512: 4.5 us (the chain of loads: length, page, tile).
 #include <cuda_runtime.h>
@@ -72,6 +72,7 @@ constexpr int kMaxShare = 2048;
 // four of them fill 43 %, of 8192: 17.1 / 19.2.
 constexpr int kMaxShareFew = 512;
 constexpr int kJoinThreads = 256;
+constexpr int kJoinCtas = 4;              // resident join blocks of an SM (registers)
 // Starting and ending a run costs a CTA as much as one unit of work with a bf16 cache, two with
 // an e4m3 one (a fit of the CTAs' times on ragged batches, d 128: 1.34 us a unit
 // and 1.14 to 1.38 us a run; 1.39 us and 3.2 to 3.7 us), so it is counted as that.
@@ -105,7 +106,8 @@ struct Params {
   long long lse_b;
   float* part_o;                    // [2 * ctas][rows][HD]
   float2* part_ml;                  // [2 * ctas][rows]
-  int4* desc;                       // [ctas]
+  int4* desc;                       // what the join's blocks join: [segments] or [ctas]
+  int by_seg;
   int B, Hq, Hk, group, mtiles, rows;  // rows: query heads of one CTA's product, at most 16
   int page, page_shift, max_blocks, n_pages;
   float scale_log2;
@@ -346,9 +348,11 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
         p.o[b * p.o_b + (i / HD) * p.o_h + i % HD] = __float2bfloat16_rn(0.f);
       if (p.lse)
         for (int i = tid; i < p.Hq; i += kThreads) p.lse[b * p.lse_b + i] = -INFINITY;
+      if (p.by_seg)
+        for (int i = tid; i < segs; i += kThreads) p.desc[b * segs + i] = make_int4(-1, 0, 0, 0);
     }
     if (cta >= ctas) {
-      if (tid == 0) p.desc[cta] = make_int4(-1, 0, 0, 0);
+      if (tid == 0 && !p.by_seg) p.desc[cta] = make_int4(-1, 0, 0, 0);
       return;
     }
     const int u0 = cut(cta, U, ctas), x = u0 / segs;
@@ -727,9 +731,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
     const bool begins = r.c0 == 0, ends = r.c1 == r.nu;
     const int slot = 2 * cta + (begins ? 1 : 0);  // a run that began in an earlier CTA goes to slot 0
     if constexpr (!CLUSTER)
-      if (begins && !ends) {
-        const int end = cut(cta + 1, U, ctas) - r.c1 + r.nu;  // unit after this segment's last
-        my_desc = make_int4(r.b, r.seg, static_cast<int>((static_cast<long long>(end) * ctas - 1) / U), 0);
+      if (begins) {
+        const int end = cut(cta + 1, U, ctas) - r.c1 + r.nu;  // unit after this segment's last (if it goes on)
+        if (!ends) my_desc = make_int4(r.b, r.seg, static_cast<int>((static_cast<long long>(end) * ctas - 1) / U), cta);
+        if (p.by_seg && tid == 0) p.desc[r.b * segs + r.seg] = my_desc;
       }
     const float vsc = (FP8 && p.v_scale) ? p.v_scale[h] : 1.f;
 #pragma unroll
@@ -863,13 +868,13 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   }
   if constexpr (!CLUSTER) {
     griddep_launch();
-    if (tid == 0) p.desc[cta] = my_desc;
+    if (tid == 0 && !p.by_seg) p.desc[cta] = my_desc;
   }
   if (bad_page && p.err) atomicExch(p.err, kErrPage);
 }
 
-// Joins the partials of each segment that more than one CTA worked on: block j
-// does the one that began in CTA j's range and went on past its end.  A group of
+// Joins the partials of each segment that more than one CTA worked on: a block for each segment, or,
+// where there are more segments than CTAs, for the one that began in a CTA's range and went on past its end.  A group of
 // lanes covers one row (query head) with 16 bytes each; the groups of a row take
 // every `per_row`-th partial, with a running maximum of their own, so that a
 // partial's sum and its values are loaded together, and are added up in a
@@ -881,10 +886,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, cons
   __shared__ float4 s_o[GR][LPR];
   __shared__ float2 s_ml[GR];
   griddep_sync();
-  const int j = blockIdx.x;
-  const int4 d = p.desc[j];
+  const int4 d = p.desc[blockIdx.x];
   if (d.x < 0) return;
-  const int b = d.x, n = d.z - j + 1;
+  const int b = d.x, j = d.w, n = d.z - j + 1;  // CTAs j .. d.z
   const int seg_rows = tiles * p.rows;            // `tiles` tiles of query heads lie in a segment
   const int li = threadIdx.x % LPR, gi = threadIdx.x / LPR;
   const int rows = (seg_rows - blockIdx.y + gridDim.y - 1) / static_cast<int>(gridDim.y);  // of this block
@@ -975,6 +979,8 @@ int ctas_per_sm() {
 struct Plan {
   int mode, grid, cluster;
   int tiles() const { return mode == kByHeads ? kWarps : 1; }  // tiles of query heads in a segment
+  bool by_seg(long long segs) const { return segs <= grid; }   // the join: a block per segment, or per CTA
+  int descs(long long segs) const { return by_seg(segs) ? static_cast<int>(segs) : grid; }
 };
 
 template <int HD, bool FP8, int NH>
@@ -1015,10 +1021,14 @@ int launch(Params& p, const Plan& plan, cudaStream_t stream) {
   else launch_kernel(decode_kernel<HD, FP8, NH, kByKeys>, grid, block, smem, stream, 1, p);
   const int st = launch_status();
   if (st != NL_OK) return st;
-  // few segments: many partials each, so their rows are split over blocks too
-  const int rows = plan.tiles() * p.rows;
-  const int ysplit = static_cast<long long>(p.B) * p.Hk * p.mtiles <= 16 * plan.tiles() ? rows : 1;
-  launch_kernel(join_kernel<HD, FP8>, dim3(plan.grid, ysplit), dim3(kJoinThreads), 0, stream, 1, p, plan.tiles());
+  // Rows of a segment are split over as many blocks as an SM holds at once: the fewer rows a block has, the more of
+  // a row's partials are loaded at the same time (64 sequences of up to 4097 on an e4m3 cache: 53.1 us, as many again
+  // 55.1, a block per CTA for all rows 55.5; 48 of up to 8192: 128.5, 130.3, 130.6).
+  const long long segs = static_cast<long long>(p.B) * p.Hk * p.mtiles / plan.tiles();
+  const int rows = plan.tiles() * p.rows, blocks = plan.descs(segs);
+  const int split = kJoinCtas * sm_count() / blocks;
+  launch_kernel(join_kernel<HD, FP8>, dim3(blocks, split < 1 ? 1 : (split < rows ? split : rows)), dim3(kJoinThreads),
+                0, stream, 1, p, plan.tiles());
   return launch_status();
 }
 
@@ -1147,6 +1157,7 @@ extern "C" int nl_paged_attention(const nl_paged_attention_args* args, cudaStrea
   p.lse = a.lse;
   p.lse_b = a.lse_b;
   p.B = B;
+  p.by_seg = plan.by_seg(static_cast<long long>(B) * Hk * p.mtiles / plan.tiles());
   p.Hq = Hq;
   p.Hk = Hk;
   p.page = page_size;
