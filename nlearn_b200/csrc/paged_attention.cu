@@ -25,11 +25,14 @@
 //   * the running maximum moves only when a score passes it by 2^8 (the sums
 //     hold that in f32), so the cross-lane maximum and the rescaling of o are
 //     rare.
-// p is split into two bf16 terms (p = hi + lo, error 2^-16) for the second
-// product: the tensor pipe has room and the output then keeps the accuracy of
-// f32 probabilities.  With an e4m3 cache both products run in f16: e4m3 values
-// are exact in f16, q is scaled by a power of two per head (exact), and p, kept
-// below 2^15, is rounded to f16's 11 bits, an eighth of the bf16 output's step.
+// p is split into two 16-bit terms (p = hi + lo) for the second product: the
+// tensor pipe has room and the output then keeps the accuracy of f32
+// probabilities.  In bf16 the two are off by 2^-16 at most.  With an e4m3 cache
+// both products run in f16: e4m3 values are exact in f16, q is scaled by a power
+// of two per head (exact), and p, kept below 2^15, is off by 2^-22, or by the
+// 2^-25 of f16's smallest step where the largest p is at least 2^7.  (One f16 term moved 9 % of the outputs of 64
+// sequences of up to 4097 by a bf16 step; the second takes 53.4 us there as without it, 51.9 us in
+// place of 49.6 for 32 of up to 8192 with 64/4 heads of 128, 25.9 in place of 24.4 with 16/4 heads of 64.)
 //
 // Two ways of dividing the work, both with lengths read on the device only:
 //   * flat: the work of all sequences and heads is one list of units of 64 or 128
@@ -679,7 +682,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             if constexpr (FP8) {
-              ph[n][e] = transpose8(pack_f16x2(pr[2 * e], pr[2 * e + 1]));
+              const uint32_t hi = pack_f16x2(pr[2 * e], pr[2 * e + 1]);
+              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              ph[n][e] = transpose8(hi);
+              pl[n][e] = transpose8(pack_f16x2(pr[2 * e] - h.x, pr[2 * e + 1] - h.y));
             } else {
               const uint32_t hi = pack_bf16x2(pr[2 * e], pr[2 * e + 1]);
               ph[n][e] = transpose8(hi);
@@ -712,7 +718,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
               const uint32_t a[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2(lo >> 16), e4m3x2_f16x2(hi),
                                      e4m3x2_f16x2(hi >> 16)};
 #pragma unroll
-              for (int n = 0; n < NH; ++n) mma16816<true>(acc[n][2 * ii + e], a, ph[n][0], ph[n][1]);
+              for (int n = 0; n < NH; ++n) {
+                mma16816<true>(acc[n][2 * ii + e], a, ph[n][0], ph[n][1]);
+                mma16816<true>(acc[n][2 * ii + e], a, pl[n][0], pl[n][1]);
+              }
             }
           }
         }
