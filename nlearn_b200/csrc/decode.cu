@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(1024) sample_kernel(const float* __restrict__ 
     float v = row[j];
     if (!greedy) {
       const uint64_t r = mix64(key + static_cast<uint64_t>(j));
-      const float u = (static_cast<float>(r >> 40) + 0.5f) * (1.0f / 16777216.0f);  // (0, 1), 24 bits
+      // (0, 1) in 24 bits; the sum rounds up to 2^24 for the last of them, where u = 1 would make the noise infinite
+      const float u = fminf((static_cast<float>(r >> 40) + 0.5f) * (1.0f / 16777216.0f), 1.0f - 1.0f / 16777216.0f);
       v = v * inv_temp - logf(-logf(u));
     }
     if (v > best || (v == best && j < bidx)) {

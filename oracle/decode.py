@@ -2,7 +2,8 @@
 
 * ``sample``: the B200 sampler's rule restated in NumPy, bit-exact in its
   random bits: token = argmax_j(logit_j / T + G_j) with Gumbel noise
-  G_j = -log(-log(u_j)), u_j = ((r >> 40) + 0.5) / 2^24 and r the SplitMix64
+  G_j = -log(-log(u_j)), u_j = min(((r >> 40) + 0.5) / 2^24, 1 - 2^-24) (in f32: the sum
+  rounds up to 2^24 for the last value) and r the SplitMix64
   finaliser (Steele, Lea & Flood, OOPSLA 2014) of key + j, key = mix(seed ^
   mix((pos << 32) ^ row)).  Gumbel-max draws from categorical(softmax(logits
   / T)), the distribution of the reference's jax.random.categorical
@@ -32,7 +33,8 @@ def uniforms(seed: int, pos: int, row: int, V: int) -> np.ndarray:
         inner = _mix(np.array([(pos << 32) ^ row], np.uint64))[0]
         key = _mix(np.array([np.uint64(seed) ^ inner], np.uint64))[0]
         r = _mix(key + np.arange(V, dtype=np.uint64))
-    return ((r >> np.uint64(40)).astype(np.float32) + np.float32(0.5)) * np.float32(1.0 / 16777216.0)
+    u = ((r >> np.uint64(40)).astype(np.float32) + np.float32(0.5)) * np.float32(1.0 / 16777216.0)
+    return np.minimum(u, np.float32(1.0 - 2.0**-24))
 
 
 def sample(logits: np.ndarray, seed: int, pos: int, temperature: float) -> np.ndarray:
