@@ -315,6 +315,11 @@ NL_API int nl_decode_embed_rows(const int* tok, const int* lens, const void* wte
 NL_API int nl_sample_tokens_rows(const float* logits, long long ldl, int V, float temperature,
                                  unsigned long long seed, const int* lens, int* tok, int* out, long long ldo, int B,
                                  cudaStream_t stream);
+/* nl_sample_tokens_rows with random bits of requests[b] (int32 [B], taken as 32 unsigned
+ * bits; NULL: b) in place of the row's: rows that are used again draw anew. */
+NL_API int nl_sample_tokens_requests(const float* logits, long long ldl, int V, float temperature,
+                                     unsigned long long seed, const int* lens, const int* requests, int* tok, int* out,
+                                     long long ldo, int B, cudaStream_t stream);
 /* C[M, N] = LayerNorm(x)[M, K] . W[K, N] with the nl_gemm_ex epilogues
  * (STORE / ACCUM / BIAS / BIAS_GELU / RESID), the LayerNorm (gamma, beta over
  * K, eps) applied while the small-M kernel stages x; M <= 8, x and W

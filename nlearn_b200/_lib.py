@@ -67,6 +67,8 @@ SIGNATURES: dict[str, list] = {
     "nl_decode_embed_rows": [c_void_p] * 5 + [c_int] * 4 + [c_void_p],
     "nl_sample_tokens_rows": [c_void_p, c_longlong, c_int, c_float, c_ulonglong, c_void_p, c_void_p, c_void_p,
                               c_longlong, c_int, c_void_p],
+    "nl_sample_tokens_requests": [c_void_p, c_longlong, c_int, c_float, c_ulonglong, c_void_p, c_void_p, c_void_p,
+                                  c_void_p, c_longlong, c_int, c_void_p],
     "nl_linear_ln_small": [c_void_p, c_longlong, c_void_p, c_void_p, c_float, c_void_p, c_longlong, c_void_p,
                            c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "nl_paged_attention_workspace_bytes": [c_int] * 7,

@@ -211,11 +211,13 @@ __host__ __device__ __forceinline__ uint64_t mix64(uint64_t z) {
 }
 
 // One CTA per row: argmax over the vocabulary of logit/T + Gumbel noise.  ROWS as
-// in decode_embed_kernel: row b is at position pos[b] - 1, idle rows keep their token.
+// in decode_embed_kernel: row b is at position pos[b] - 1, idle rows keep their token;
+// its random stream is that of request[b], or b where request is null.
 template <bool ROWS>
 __global__ void __launch_bounds__(1024) sample_kernel(const float* __restrict__ logits, long long ldl, int V,
                                                      float inv_temp, int greedy, unsigned long long seed,
-                                                     const int* __restrict__ pos, int* __restrict__ tok,
+                                                     const int* __restrict__ pos,
+                                                     const int* __restrict__ request, int* __restrict__ tok,
                                                      int* __restrict__ out, long long ldo, int* err) {
   griddep_sync();
   __shared__ float bv[32];
@@ -224,7 +226,8 @@ __global__ void __launch_bounds__(1024) sample_kernel(const float* __restrict__ 
   const int t = ROWS ? pos[b] - 1 : *pos;
   if (ROWS && t < 0) return;
   const float* row = logits + b * ldl;
-  const uint64_t key = mix64(seed ^ mix64((static_cast<uint64_t>(t) << 32) ^ static_cast<uint64_t>(b)));
+  const uint32_t who = ROWS && request ? static_cast<uint32_t>(request[b]) : static_cast<uint32_t>(b);
+  const uint64_t key = mix64(seed ^ mix64((static_cast<uint64_t>(t) << 32) ^ static_cast<uint64_t>(who)));
   float best = -INFINITY;
   int bidx = 0x7fffffff;
   for (int j = threadIdx.x; j < V; j += blockDim.x) {
@@ -345,18 +348,24 @@ extern "C" int nl_sample_tokens(const float* logits, long long ldl, int V, float
   if (B <= 0 || V <= 0 || ldl < V || !pos || !tok) return NL_ERR_SHAPE;
   const int greedy = temperature <= 0.f;
   launch_kernel(dec::sample_kernel<false>, dim3(B), dim3(1024), 0, stream, 1, logits, ldl, V,
-                greedy ? 1.f : 1.f / temperature, greedy, seed, pos, tok, out, ldo, device_error_word());
+                greedy ? 1.f : 1.f / temperature, greedy, seed, pos, nullptr, tok, out, ldo, device_error_word());
+  return launch_status();
+}
+
+extern "C" int nl_sample_tokens_requests(const float* logits, long long ldl, int V, float temperature,
+                                         unsigned long long seed, const int* lens, const int* requests, int* tok,
+                                         int* out, long long ldo, int B, cudaStream_t stream) {
+  if (B <= 0 || V <= 0 || ldl < V || !logits || !lens || !tok) return NL_ERR_SHAPE;
+  const int greedy = temperature <= 0.f;
+  launch_kernel(dec::sample_kernel<true>, dim3(B), dim3(1024), 0, stream, 1, logits, ldl, V,
+                greedy ? 1.f : 1.f / temperature, greedy, seed, lens, requests, tok, out, ldo, device_error_word());
   return launch_status();
 }
 
 extern "C" int nl_sample_tokens_rows(const float* logits, long long ldl, int V, float temperature,
                                      unsigned long long seed, const int* lens, int* tok, int* out, long long ldo,
                                      int B, cudaStream_t stream) {
-  if (B <= 0 || V <= 0 || ldl < V || !logits || !lens || !tok) return NL_ERR_SHAPE;
-  const int greedy = temperature <= 0.f;
-  launch_kernel(dec::sample_kernel<true>, dim3(B), dim3(1024), 0, stream, 1, logits, ldl, V,
-                greedy ? 1.f : 1.f / temperature, greedy, seed, lens, tok, out, ldo, device_error_word());
-  return launch_status();
+  return nl_sample_tokens_requests(logits, ldl, V, temperature, seed, lens, nullptr, tok, out, ldo, B, stream);
 }
 
 extern "C" int nl_decode_advance(int* pos, cudaStream_t stream) {

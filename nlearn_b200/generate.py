@@ -22,8 +22,8 @@ CUDA graph once and replayed per token.  ``Decoder`` does this for a batch of
 prompts of one length; ``PagedDecoder`` for rows that come and go with prompts
 of any lengths, over a paged cache (``nlearn_b200.paged``), with penalties,
 biases and masks on the logits (``nlearn_b200.kernels.logits``).  The random stream (seed, position,
-row) is this library's own counter-based one (the reference's JAX PRNG key is
-replaced by an integer seed).
+row; for ``PagedDecoder`` the request in place of the row) is this library's own counter-based one (the
+reference's JAX PRNG key is replaced by an integer seed).
 """
 from __future__ import annotations
 
@@ -230,6 +230,11 @@ class PagedDecoder(_DecodeStep):
     pages back; ``generate`` runs any number of prompts through the rows.  A
     step whose rows all fit is never refused: the host keeps count of the pages.
 
+    Prompts are numbered in the order of their admission (``next_request`` is the
+    next one's number), and a token's random bits depend on (seed, position,
+    number): prompts that use a row one after the other draw independently,
+    whichever rows they get, and a new decoder given the same prompts repeats the draws.
+
     cache_dtype bfloat16, or float8_e4m3fn (half the bytes; keys and values
     are stored as they are, scale 1).
     """
@@ -255,6 +260,8 @@ class PagedDecoder(_DecodeStep):
         self.new = torch.zeros(R, **i32)           # 1: the row is in use
         self.now = torch.zeros(R, **i32)           # lengths of the rows that draw a token
         self.prompt_lens = torch.zeros(R, **i32)
+        self.requests = torch.zeros(R, **i32)      # 32 bits of the number of the prompt a row was admitted with
+        self.next_request = 0
         self.repetition, self.frequency, self.presence = torch.ones(R, **f32), torch.zeros(R, **f32), torch.zeros(R,
                                                                                                                  **f32)
         self.bias_ids, self.bias = torch.full((R, max_bias), -1, **i32), torch.zeros(R, max_bias, **f32)
@@ -294,9 +301,10 @@ class PagedDecoder(_DecodeStep):
             kw.update(mask=self.mask, mask_rows=self.mask_rows)
         if kw:
             process_logits(self.logits[:, :V], out=self.logits[:, :V], **kw)
-        check(lib.nl_sample_tokens_rows(ptr(self.logits), self.logits.stride(0), V, self.temperature, self.seed,
-                                        ptr(lens), ptr(self.tok), ptr(self.out), self.out.stride(0), self.B,
-                                        stream_handle()), "nl_sample_tokens_rows")
+        check(lib.nl_sample_tokens_requests(ptr(self.logits), self.logits.stride(0), V, self.temperature, self.seed,
+                                            ptr(lens), ptr(self.requests), ptr(self.tok), ptr(self.out),
+                                            self.out.stride(0), self.B, stream_handle()),
+              "nl_sample_tokens_requests")
 
     def _embed(self, tok, lens, x):
         P, cfg = self.P, self.cfg
@@ -407,6 +415,9 @@ class PagedDecoder(_DecodeStep):
         self._ln_linear(self.x3, P.f("lnf.g"), P.f("lnf.b"), P.p("head.w")[:, :V], self.logits[:, :V])
         self.now.zero_()
         self.now[where] = self.lens[where]
+        numbers = (self.next_request + np.arange(len(rows))) & 0xFFFFFFFF
+        self.requests[where] = torch.from_numpy(numbers.astype(np.uint32).view(np.int32)).to(dev)
+        self.next_request += len(rows)
         self._draw(self.now, frozenset().union(*(self._rules[r] for r in rows)))
         for row in rows:
             self._len[row] += 1

@@ -1,0 +1,77 @@
+"""PagedDecoder when rows are used again: random bits, iterators, errors on the way."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from oracle import decode as OD  # noqa: E402
+from nlearn_b200 import _lib  # noqa: E402
+from nlearn_b200.generate import PagedDecoder, generate  # noqa: E402
+from nlearn_b200.model import FlatParams  # noqa: E402
+
+from test_paged_decode_gpu import CFG, check_row, oracle, prompts  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def params(cuda):
+    return FlatParams(CFG, cuda, seed=3)     # (flat logits: draws are all but uniform)
+
+
+def test_prompts_of_one_row_draw_independently(cuda, params):
+    """One prompt many times through fewer rows: every completion its own, each the
+    oracle's choice under the random bits of its number."""
+    p = prompts([7])[0]
+    out = PagedDecoder(params, CFG, max_batch=1, seed=4).generate([p] * 5, 12)
+    assert len({tuple(t[7:]) for t in out}) == 5
+    model = oracle(params)
+    for number, toks in enumerate(out):
+        check_row(model, toks, 7, number, 4, 1.0)
+    # another number of rows: the same draws (the logits' rounding may move a close one)
+    for number, toks in enumerate(PagedDecoder(params, CFG, max_batch=3, seed=4).generate([p] * 5, 12)):
+        check_row(model, toks, 7, number, 4, 1.0)
+    # many more prompts than rows through the entry point
+    many = generate(params, [p] * 35 + [p[:3]], 12, seed=4)
+    assert len({tuple(t[-12:]) for t in many}) == 36
+
+
+def test_a_second_run_draws_anew_and_a_new_decoder_repeats(cuda, params):
+    p = prompts([5, 9], 1)
+    dec = PagedDecoder(params, CFG, max_batch=2, seed=1)
+    first, second = dec.generate(p, 10), dec.generate(p, 10)
+    assert dec.next_request == 4
+    assert all(not np.array_equal(a, b) for a, b in zip(first, second))
+    dec.next_request = 0                      # the numbers decide, not the history
+    for got in (dec.generate(p, 10), PagedDecoder(params, CFG, max_batch=2, seed=1).generate(p, 10)):
+        for a, b in zip(first, got):
+            np.testing.assert_array_equal(a, b)
+
+
+def test_numbers_past_31_bits(cuda, params):
+    p = prompts([4])[0]
+    dec = PagedDecoder(params, CFG, max_batch=1, seed=2)
+    dec.next_request = 2**32 - 1
+    a, b = dec.generate([p, p], 6)            # numbers 2^32 - 1 and (wrapped) 0
+    model = oracle(params)
+    check_row(model, a, 4, 2**32 - 1, 2, 1.0)
+    check_row(model, b, 4, 0, 2, 1.0)
+
+
+def test_sampler_by_requests(cuda):
+    V, lib = 1000, _lib.lib
+    st = torch.cuda.current_stream().cuda_stream
+    i32 = dict(device=cuda, dtype=torch.int32)
+    lg = torch.randn(4, V, device=cuda) * 2
+    lens, req = torch.tensor([5, 0, 9, 1], **i32), torch.tensor([70000, 3, -1, 0], **i32)
+    tok, out = torch.full((4,), -3, **i32), torch.full((4, 10), -4, **i32)
+    assert lib.nl_sample_tokens_requests(lg.data_ptr(), V, V, 0.8, 11, lens.data_ptr(), req.data_ptr(), tok.data_ptr(),
+                                         out.data_ptr(), 10, 4, st) == 0
+    torch.cuda.synchronize()
+    for b, (n, r) in enumerate(zip(lens.tolist(), req.tolist())):
+        if n == 0:
+            assert tok[b] == -3 and (out[b] == -4).all()
+            continue
+        g = -np.log(-np.log(OD.uniforms(11, n - 1, r & 0xFFFFFFFF, V).astype(np.float64)))
+        want = int(np.argmax(lg[b].cpu().numpy().astype(np.float64) / 0.8 + g))
+        assert tok[b] == want and out[b, n] == want
+    assert _lib.device_error() == 0
