@@ -461,6 +461,7 @@ class PagedDecoder(_DecodeStep):
     @_on_device
     def release(self, rows) -> None:
         """End rows: their pages are free, the rows may be admitted anew."""
+        rows = list(rows)  # (walked twice)
         done = torch.zeros(self.B, dtype=torch.int32)
         for r in rows:
             if not self._len[r]:

@@ -75,3 +75,19 @@ def test_sampler_by_requests(cuda):
         want = int(np.argmax(lg[b].cpu().numpy().astype(np.float64) / 0.8 + g))
         assert tok[b] == want and out[b, n] == want
     assert _lib.device_error() == 0
+
+
+def test_release_takes_any_iterable(cuda, params):
+    dec = PagedDecoder(params, CFG, max_batch=3, temperature=0.0)
+    rows = dec.add(prompts([20, 3, 40]))
+    dec.step(2)
+    dec.release(r for r in rows[:2])
+    assert dec.free_rows() == rows[:2] and dec.new.tolist() == [0, 0, 1]
+    assert dec.free_page_count() == dec.n_free.item() == dec.n_pages - 3
+    again = dec.add(prompts([5], 1))
+    dec.step(3)
+    alone = PagedDecoder(params, CFG, max_batch=3, temperature=0.0)
+    alone.add(prompts([5], 1))
+    alone.step(3)
+    np.testing.assert_array_equal(dec.tokens(again[0]), alone.tokens(0))
+    assert dec.tokens(rows[1]).size == 0 and _lib.device_error() == 0
