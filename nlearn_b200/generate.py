@@ -484,6 +484,8 @@ class PagedDecoder(_DecodeStep):
         Long prompts keep their last ids, as in ``Decoder``."""
         if any(self._len):
             raise RuntimeError("generate needs all rows free")
+        if rules.get("allowed") is not None:
+            rules["allowed"] = list(rules["allowed"])  # (read by every admission)
         prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
         counts = [int(n) for n in np.broadcast_to(n_tokens, (len(prompts),))]
         if any(n >= self.S for n in counts):

@@ -91,3 +91,12 @@ def test_release_takes_any_iterable(cuda, params):
     alone.step(3)
     np.testing.assert_array_equal(dec.tokens(again[0]), alone.tokens(0))
     assert dec.tokens(rows[1]).size == 0 and _lib.device_error() == 0
+
+
+def test_allowed_holds_for_every_admission(cuda, params):
+    """An iterator of ids, and more prompts than rows."""
+    ps = prompts([3, 30, 8, 1, 12], 2)
+    out = PagedDecoder(params, CFG, max_batch=2).generate(ps, 5, allowed=(i for i in range(50, 53)))
+    assert all(50 <= t < 53 for p, toks in zip(ps, out) for t in toks[p.size:])
+    many = generate(params, [ps[0]] * 33 + [ps[1]], 2, allowed=iter([9]))
+    assert all((t[-2:] == 9).all() for t in many)
