@@ -336,6 +336,49 @@ class PagedDecoder(_DecodeStep):
             rules.add("mask")
         self._rules[row] = frozenset(rules)
 
+    def _run_prompts(self, rows, sizes, flat, plan):
+        """The prompts through the layers into their slots, and the first token of each."""
+        cfg, P, D, H, F = self.cfg, self.P, self.cfg.d_model, self.cfg.n_heads, self.cfg.d_ff
+        dev, T = self.P.device, sum(sizes)
+        at = [sum(sizes[:i]) for i in range(len(sizes))]
+        for row, a, n in zip(rows, at, sizes):
+            self.out[row, :n] = flat[a:a + n]
+            self.prompt_lens[row] = n
+        x = torch.empty(T, D, device=dev, dtype=torch.bfloat16)
+        self._embed(flat, plan.positions + 1, x)
+        h, o = torch.empty_like(x), torch.empty_like(x)
+        L = torch.empty(H, max(sizes), device=dev, dtype=torch.float32)
+        for layer in range(cfg.n_layers):
+            pre = f"blocks.{layer}."
+            self._ln(x, h, P.f(pre + "ln1.g"), P.f(pre + "ln1.b"), T)
+            qkv = gemm_ex(h, P.p(pre + "wqkv"), out_dtype=torch.bfloat16)
+            q, k, v = (qkv[:, i * D:(i + 1) * D] for i in range(3))
+            paged_kv_write(k.view(T, H, 64), v.view(T, H, 64), self.k_cache[layer], self.v_cache[layer], plan.slots)
+            for a, n in zip(at, sizes):  # (kernels on one stream: L may serve all)
+                check(lib.nl_flash_attention_fwd_strided(ptr(q[a:]), ptr(k[a:]), ptr(v[a:]), 3 * D, 64, n * 3 * D,
+                                                         ptr(o[a:]), D, 64, n * D, ptr(L), 1, H, n, 64,
+                                                         stream_handle()), "attn fwd")
+            x2 = gemm_ex(o, P.p(pre + "wo"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_RESID, resid=x)
+            self._ln(x2, h, P.f(pre + "ln2.g"), P.f(pre + "ln2.b"), T)
+            a_ = torch.empty(T, F, device=dev, dtype=torch.bfloat16)
+            u = gemm_ex(h, P.p(pre + "w1"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_BIAS_GELU,
+                        bias=P.f(pre + "b1"), aux=a_)
+            x = gemm_ex(u, P.p(pre + "w2"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_RESID,
+                        bias=P.f(pre + "b2"), resid=x2)
+        last = torch.tensor([a + n - 1 for a, n in zip(at, sizes)], device=dev)
+        where = torch.tensor(rows, device=dev)
+        self.x3.zero_()
+        self.x3[where] = x[last]
+        V = cfg.vocab
+        self._ln_linear(self.x3, P.f("lnf.g"), P.f("lnf.b"), P.p("head.w")[:, :V], self.logits[:, :V])
+        self.now.zero_()
+        self.now[where] = self.lens[where]
+        numbers = (self.next_request + np.arange(len(rows))) & 0xFFFFFFFF
+        self.requests[where] = torch.from_numpy(numbers.astype(np.uint32).view(np.int32)).to(dev)
+        self._draw(self.now, frozenset().union(*(self._rules[r] for r in rows)))
+        self.new[where] = 1
+        self.next_request += len(rows)
+
     # ------------------------------------------------------------------ API
     def set_allowed(self, row: int, allowed) -> None:
         """Token ids that row may draw from now on (None: all; a grammar calls this between steps)."""
@@ -370,7 +413,6 @@ class PagedDecoder(_DecodeStep):
             raise RuntimeError(f"prompts need {sum(self._pages(n) for n in sizes)} pages, {self.free_page_count()} free")
         if not rows:
             return rows
-        cfg, P, D, H, F = self.cfg, self.P, self.cfg.d_model, self.cfg.n_heads, self.cfg.d_ff
         dev, T = self.P.device, sum(sizes)
         # the flat list holds the prompts in the order of their rows, which is ascending
         flat = torch.from_numpy(np.concatenate(prompts)).to(dev)
@@ -381,47 +423,15 @@ class PagedDecoder(_DecodeStep):
         grow = grow.to(dev)
         plan = update_block_tables(self.block_table, self.lens, grow, self.free_pages, self.n_free, self.page_size, T,
                                    lens_out=self.lens, n_free_out=self.n_free)
-        at = [sum(sizes[:i]) for i in range(len(sizes))]
-        for row, a, n in zip(rows, at, sizes):
-            self.out[row, :n] = flat[a:a + n]
-            self.prompt_lens[row] = n
+        for row, n in zip(rows, sizes):
             self._len[row] = n
-        x = torch.empty(T, D, device=dev, dtype=torch.bfloat16)
-        self._embed(flat, plan.positions + 1, x)
-        h, o = torch.empty_like(x), torch.empty_like(x)
-        L = torch.empty(H, max(sizes), device=dev, dtype=torch.float32)
-        for layer in range(cfg.n_layers):
-            pre = f"blocks.{layer}."
-            self._ln(x, h, P.f(pre + "ln1.g"), P.f(pre + "ln1.b"), T)
-            qkv = gemm_ex(h, P.p(pre + "wqkv"), out_dtype=torch.bfloat16)
-            q, k, v = (qkv[:, i * D:(i + 1) * D] for i in range(3))
-            paged_kv_write(k.view(T, H, 64), v.view(T, H, 64), self.k_cache[layer], self.v_cache[layer], plan.slots)
-            for a, n in zip(at, sizes):  # (kernels on one stream: L may serve all)
-                check(lib.nl_flash_attention_fwd_strided(ptr(q[a:]), ptr(k[a:]), ptr(v[a:]), 3 * D, 64, n * 3 * D,
-                                                         ptr(o[a:]), D, 64, n * D, ptr(L), 1, H, n, 64,
-                                                         stream_handle()), "attn fwd")
-            x2 = gemm_ex(o, P.p(pre + "wo"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_RESID, resid=x)
-            self._ln(x2, h, P.f(pre + "ln2.g"), P.f(pre + "ln2.b"), T)
-            a_ = torch.empty(T, F, device=dev, dtype=torch.bfloat16)
-            u = gemm_ex(h, P.p(pre + "w1"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_BIAS_GELU,
-                        bias=P.f(pre + "b1"), aux=a_)
-            x = gemm_ex(u, P.p(pre + "w2"), out_dtype=torch.bfloat16, epilogue=_lib.EPI_RESID,
-                        bias=P.f(pre + "b2"), resid=x2)
-        last = torch.tensor([a + n - 1 for a, n in zip(at, sizes)], device=dev)
-        where = torch.tensor(rows, device=dev)
-        self.x3.zero_()
-        self.x3[where] = x[last]
-        V = cfg.vocab
-        self._ln_linear(self.x3, P.f("lnf.g"), P.f("lnf.b"), P.p("head.w")[:, :V], self.logits[:, :V])
-        self.now.zero_()
-        self.now[where] = self.lens[where]
-        numbers = (self.next_request + np.arange(len(rows))) & 0xFFFFFFFF
-        self.requests[where] = torch.from_numpy(numbers.astype(np.uint32).view(np.int32)).to(dev)
-        self.next_request += len(rows)
-        self._draw(self.now, frozenset().union(*(self._rules[r] for r in rows)))
+        try:
+            self._run_prompts(rows, sizes, flat, plan)
+        except BaseException:
+            self.release(rows)  # (the rows hold pages already)
+            raise
         for row in rows:
             self._len[row] += 1
-            self.new[row] = 1
         return rows
 
     @_on_device

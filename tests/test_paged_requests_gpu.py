@@ -100,3 +100,49 @@ def test_allowed_holds_for_every_admission(cuda, params):
     assert all(50 <= t < 53 for p, toks in zip(ps, out) for t in toks[p.size:])
     many = generate(params, [ps[0]] * 33 + [ps[1]], 2, allowed=iter([9]))
     assert all((t[-2:] == 9).all() for t in many)
+
+
+def fail_at(monkeypatch, call):
+    """The call-th product of the decoder's layers raises on the host."""
+    from nlearn_b200 import generate as G
+    count, real = [0], G.gemm_ex
+
+    def gemm(*args, **kw):
+        count[0] += 1
+        if count[0] == call:
+            raise MemoryError("planted")
+        return real(*args, **kw)
+    monkeypatch.setattr(G, "gemm_ex", gemm)
+
+
+def same_books(dec):
+    """The host's count of rows and pages is the device's."""
+    torch.cuda.synchronize()
+    assert dec.lens.tolist() == [max(0, n - 1) for n in dec._len]
+    assert dec.new.tolist() == [int(n > 0) for n in dec._len]
+    assert dec.n_free.item() == dec.free_page_count()
+    held = [p for r, n in enumerate(dec.lens.tolist()) for p in dec.block_table[r, :dec._pages(n)].tolist()]
+    assert sorted(held + dec.free_pages[:dec.n_free.item()].tolist()) == list(range(dec.n_pages))
+
+
+@pytest.mark.parametrize("call", [1, 3, 6])
+def test_an_admission_that_fails_leaves_no_rows(cuda, params, monkeypatch, call):
+    ps = prompts([20, 3, 40], 5)
+    dec = PagedDecoder(params, CFG, max_batch=3, n_pages=12, seed=8)
+    kept, = dec.add(ps[:1])
+    with monkeypatch.context() as m:
+        fail_at(m, call)
+        with pytest.raises(MemoryError):
+            dec.add(ps[1:])
+    assert dec.free_rows() == [1, 2] and dec.next_request == 1
+    same_books(dec)
+    dec.add(ps[1:])
+    dec.step(3)
+    want = PagedDecoder(params, CFG, max_batch=3, n_pages=12, seed=8)
+    want.add(ps[:1])
+    want.add(ps[1:])
+    want.step(3)
+    for r in range(3):
+        np.testing.assert_array_equal(dec.tokens(r), want.tokens(r))
+    same_books(dec)
+    assert _lib.device_error() == 0
