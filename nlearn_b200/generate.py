@@ -457,9 +457,10 @@ class PagedDecoder(_DecodeStep):
                     self._graphs[key] = False
                 else:
                     if graph is False:
-                        graph = self._graphs[key] = torch.cuda.CUDAGraph()
+                        graph = torch.cuda.CUDAGraph()
                         with torch.cuda.graph(graph):
                             self._step(rules)
+                        self._graphs[key] = graph  # (kept once the capture has succeeded)
                     graph.replay()
             for r in used:
                 self._len[r] += 1

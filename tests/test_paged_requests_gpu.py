@@ -146,3 +146,23 @@ def test_an_admission_that_fails_leaves_no_rows(cuda, params, monkeypatch, call)
         np.testing.assert_array_equal(dec.tokens(r), want.tokens(r))
     same_books(dec)
     assert _lib.device_error() == 0
+
+
+def test_a_capture_that_fails_is_made_again(cuda, params, monkeypatch):
+    ps = prompts([20, 3], 6)
+    dec = PagedDecoder(params, CFG, max_batch=2, seed=8)
+    dec.add(ps)
+    dec.step()
+    with monkeypatch.context() as m:
+        fail_at(m, 2)
+        with pytest.raises(MemoryError):
+            dec.step()
+    same_books(dec)
+    dec.step(3)
+    want = PagedDecoder(params, CFG, max_batch=2, seed=8)
+    want.add(ps)
+    want.step(4, use_graph=False)
+    for r in range(2):
+        np.testing.assert_array_equal(dec.tokens(r), want.tokens(r))
+    same_books(dec)
+    assert _lib.device_error() == 0
