@@ -318,6 +318,22 @@ class PagedDecoder(_DecodeStep):
         self._layers(self._attention)
         self._draw(self.lens, rules)
 
+    def _run_step(self, rules, use_graph):
+        if not use_graph:
+            return self._step(rules)
+        key = (rules, self.seed, self.temperature)
+        graph = self._graphs.get(key)
+        if graph is None:
+            self._step(rules)  # (the first step of a kind runs eagerly: it sets the kernels up)
+            self._graphs[key] = False
+            return
+        if graph is False:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                self._step(rules)
+            self._graphs[key] = graph  # (kept once the capture has succeeded)
+        graph.replay()
+
     def _set_rules(self, row, repetition, frequency, presence, bias, allowed):
         rules = set()
         if repetition != 1.0 or frequency != 0.0 or presence != 0.0:
@@ -447,21 +463,15 @@ class PagedDecoder(_DecodeStep):
             if grow > self.free_page_count():
                 raise RuntimeError(f"the step needs {grow} pages, {self.free_page_count()} free: release a row")
             rules = frozenset().union(*(self._rules[r] for r in used))
-            if not use_graph:
-                self._step(rules)
-            else:
-                key = (rules, self.seed, self.temperature)
-                graph = self._graphs.get(key)
-                if graph is None:
-                    self._step(rules)  # (the first step of a kind runs eagerly: it sets the kernels up)
-                    self._graphs[key] = False
-                else:
-                    if graph is False:
-                        graph = torch.cuda.CUDAGraph()
-                        with torch.cuda.graph(graph):
-                            self._step(rules)
-                        self._graphs[key] = graph  # (kept once the capture has succeeded)
-                    graph.replay()
+            try:
+                self._run_step(rules, use_graph)
+            except BaseException:
+                # back to before the step: the pages it took are still on the stack, above its size
+                last = torch.tensor([max(0, n - 1) for n in self._len], device=self.P.device)
+                self.lens.copy_(last)
+                self.n_free.fill_(self.free_page_count())
+                self.tok.copy_(self.out.gather(1, last[:, None])[:, 0])
+                raise
             for r in used:
                 self._len[r] += 1
 

@@ -115,6 +115,10 @@ def fail_at(monkeypatch, call):
     monkeypatch.setattr(G, "gemm_ex", gemm)
 
 
+def fail():
+    raise MemoryError("planted")
+
+
 def same_books(dec):
     """The host's count of rows and pages is the device's."""
     torch.cuda.synchronize()
@@ -163,6 +167,33 @@ def test_a_capture_that_fails_is_made_again(cuda, params, monkeypatch):
     want.add(ps)
     want.step(4, use_graph=False)
     for r in range(2):
+        np.testing.assert_array_equal(dec.tokens(r), want.tokens(r))
+    same_books(dec)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("call", [1, 4, "drawn"])
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_a_step_that_fails_is_taken_back(cuda, params, monkeypatch, call, use_graph):
+    """Rows on the edge of a page among them: the page is taken once."""
+    ps = prompts([16, 3, 15, 32], 7)
+    dec = PagedDecoder(params, CFG, max_batch=4, seed=8)
+    dec.add(ps)
+    for _ in range(2):
+        with monkeypatch.context() as m:
+            if call == "drawn":               # (stopped by hand when the step is already on its way)
+                real = dec._step
+                m.setattr(dec, "_step", lambda rules: (real(rules), fail()))
+            else:
+                fail_at(m, call)
+            with pytest.raises(MemoryError):
+                dec.step(use_graph=use_graph)
+        same_books(dec)
+    dec.step(4, use_graph=use_graph)
+    want = PagedDecoder(params, CFG, max_batch=4, seed=8)
+    want.add(ps)
+    want.step(4, use_graph=False)
+    for r in range(4):
         np.testing.assert_array_equal(dec.tokens(r), want.tokens(r))
     same_books(dec)
     assert _lib.device_error() == 0
