@@ -521,23 +521,27 @@ class PagedDecoder(_DecodeStep):
         for i in queue:
             if need(i) > self.n_pages:
                 raise ValueError(f"prompt {i} needs {need(i)} pages, the cache has {self.n_pages}")
-        while queue or running:
-            take, held = [], sum(need(i) for i in running.values())
-            for i in queue[:len(self.free_rows())]:
-                if held + need(i) > self.n_pages:
-                    break
-                held += need(i)
-                take.append(i)
-            if take:
-                del queue[:len(take)]
-                running.update(zip(self.add([prompts[i] for i in take], **rules), take))
-            left = {r: prompts[i].size + counts[i] - self._len[r] for r, i in running.items()}
-            if min(left.values()) > 0:
-                self.step(min(left.values()), use_graph)
-            ended = [r for r, n in left.items() if n == min(left.values())]
-            for r in ended:
-                done[running.pop(r)] = self.tokens(r)
-            self.release(ended)
+        try:
+            while queue or running:
+                take, held = [], sum(need(i) for i in running.values())
+                for i in queue[:len(self.free_rows())]:
+                    if held + need(i) > self.n_pages:
+                        break
+                    held += need(i)
+                    take.append(i)
+                if take:
+                    del queue[:len(take)]
+                    running.update(zip(self.add([prompts[i] for i in take], **rules), take))
+                left = {r: prompts[i].size + counts[i] - self._len[r] for r, i in running.items()}
+                if min(left.values()) > 0:
+                    self.step(min(left.values()), use_graph)
+                ended = [r for r, n in left.items() if n == min(left.values())]
+                for r in ended:
+                    done[running.pop(r)] = self.tokens(r)
+                self.release(ended)
+        except BaseException:
+            self.release(r for r in range(self.B) if self._len[r])  # (all rows were free at the start)
+            raise
         return done
 
 

@@ -197,3 +197,18 @@ def test_a_step_that_fails_is_taken_back(cuda, params, monkeypatch, call, use_gr
         np.testing.assert_array_equal(dec.tokens(r), want.tokens(r))
     same_books(dec)
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("call", [2, 20, 60])
+def test_a_generation_that_fails_leaves_no_rows(cuda, params, monkeypatch, call):
+    ps = prompts([20, 3, 40, 7], 9)
+    dec = PagedDecoder(params, CFG, max_batch=2, temperature=0.0)
+    with monkeypatch.context() as m:
+        fail_at(m, call)
+        with pytest.raises(MemoryError):
+            dec.generate(ps, 8, use_graph=False)
+    assert dec.free_rows() == [0, 1] and dec.n_free.item() == dec.n_pages
+    same_books(dec)
+    for a, b in zip(dec.generate(ps, 8), PagedDecoder(params, CFG, max_batch=2, temperature=0.0).generate(ps, 8)):
+        np.testing.assert_array_equal(a, b)
+    assert _lib.device_error() == 0
