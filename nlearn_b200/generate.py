@@ -239,6 +239,8 @@ class PagedDecoder(_DecodeStep):
     are stored as they are, scale 1).
     """
 
+    MAX_GRAPHS = 32
+
     def __init__(self, params: FlatParams, cfg: GPTConfig, max_batch: int = 8, n_pages: int | None = None,
                  page_size: int = 16, max_len: int | None = None, max_bias: int = 32, seed: int = 0,
                  temperature: float = 1.0, cache_dtype=torch.bfloat16):
@@ -322,17 +324,24 @@ class PagedDecoder(_DecodeStep):
         if not use_graph:
             return self._step(rules)
         key = (rules, self.seed, self.temperature)
-        graph = self._graphs.get(key)
+        graph = self._graphs.pop(key, None)
         if graph is None:
             self._step(rules)  # (the first step of a kind runs eagerly: it sets the kernels up)
-            self._graphs[key] = False
+            self._keep_graph(key, False)
             return
         if graph is False:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 self._step(rules)
-            self._graphs[key] = graph  # (kept once the capture has succeeded)
+        self._keep_graph(key, graph)  # (after the capture has succeeded)
         graph.replay()
+
+    def _keep_graph(self, key, graph):
+        """Keep the MAX_GRAPHS graphs used last (a seed and temperature have up to 8, one for each set of rules)."""
+        self._graphs[key] = graph
+        if len(self._graphs) > self.MAX_GRAPHS:
+            torch.cuda.current_stream().synchronize()  # (it may still run)
+            del self._graphs[next(iter(self._graphs))]
 
     def _set_rules(self, row, repetition, frequency, presence, bias, allowed):
         rules = set()

@@ -212,3 +212,23 @@ def test_a_generation_that_fails_leaves_no_rows(cuda, params, monkeypatch, call)
     for a, b in zip(dec.generate(ps, 8), PagedDecoder(params, CFG, max_batch=2, temperature=0.0).generate(ps, 8)):
         np.testing.assert_array_equal(a, b)
     assert _lib.device_error() == 0
+
+
+def test_graphs_of_many_seeds(cuda, params):
+    """A graph for each (rules, seed, temperature), the last ones kept; seeds in
+    turn use theirs again."""
+    ps = prompts([5, 9], 10)
+    dec = PagedDecoder(params, CFG, max_batch=2)
+    for seed in range(dec.MAX_GRAPHS + 5):
+        dec.seed = seed
+        dec.generate(ps, 5)
+        assert len(dec._graphs) <= dec.MAX_GRAPHS
+    assert [k[1] for k in dec._graphs] == list(range(5, dec.MAX_GRAPHS + 5))
+    kept = dict(dec._graphs)
+    for seed in (10, 11, 10):
+        dec.seed, dec.next_request = seed, 0
+        out = dec.generate(ps, 5)
+        want = PagedDecoder(params, CFG, max_batch=2, seed=seed).generate(ps, 5, use_graph=False)
+        assert all(np.array_equal(a, b) for a, b in zip(out, want))
+    assert all(dec._graphs[k] is g for k, g in kept.items())
+    assert _lib.device_error() == 0
