@@ -560,7 +560,8 @@ def generate(trainer_or_params, prompt_ids, n_tokens, seed: int = 0, temperature
     [B, P] prompt -> tokens (1-D for a 1-D prompt).  A list of prompts of
     different lengths, an n_tokens per prompt, or any of the rules of
     ``PagedDecoder.add`` (repetition, frequency, presence, bias, allowed) run on the
-    paged cache; a list of prompts then gives a list of arrays."""
+    paged cache; a list of prompts, or an n_tokens for each, then gives a list of
+    arrays, a [B, P] array with one n_tokens a [B, P + n_tokens] one."""
     P = getattr(trainer_or_params, "P", trainer_or_params)
     cfg = cfg or getattr(trainer_or_params, "cfg", None) or P.cfg
     several = isinstance(prompt_ids, (list, tuple)) and any(np.ndim(p) == 1 for p in prompt_ids)
@@ -568,7 +569,9 @@ def generate(trainer_or_params, prompt_ids, n_tokens, seed: int = 0, temperature
         prompts = prompt_ids if several or np.ndim(prompt_ids) == 2 else [prompt_ids]
         dec = PagedDecoder(P, cfg, max_batch=max(1, min(len(prompts), 32)), seed=seed, temperature=temperature)
         out = dec.generate(prompts, n_tokens, **rules)
-        return out if several or np.ndim(prompt_ids) == 2 else out[0]
+        if several or np.ndim(prompt_ids) == 2:
+            return out if several or np.ndim(n_tokens) or not out else np.stack(out)
+        return out[0]
     p = np.asarray(prompt_ids, np.int32)
     dec = Decoder(P, cfg, batch=1 if p.ndim == 1 else p.shape[0])
     out = dec.generate(p, n_tokens, seed, temperature)

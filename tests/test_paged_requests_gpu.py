@@ -232,3 +232,17 @@ def test_graphs_of_many_seeds(cuda, params):
         assert all(np.array_equal(a, b) for a, b in zip(out, want))
     assert all(dec._graphs[k] is g for k, g in kept.items())
     assert _lib.device_error() == 0
+
+
+def test_entry_point_keeps_the_shape_of_its_prompts(cuda, params):
+    ps = np.stack(prompts([9, 9, 9], 11))
+    plain = generate(params, ps, 4, temperature=0.0)
+    ruled = generate(params, ps, 4, temperature=0.0, repetition=1.0)     # a rule that changes nothing
+    assert isinstance(plain, np.ndarray) and isinstance(ruled, np.ndarray)
+    assert plain.shape == ruled.shape == (3, 13) and ruled.dtype == plain.dtype
+    np.testing.assert_array_equal(ruled[:, :9], ps)
+    by_list = generate(params, list(ps), 4, temperature=0.0, presence=0.5)
+    assert isinstance(by_list, list) and [t.shape for t in by_list] == [(13,)] * 3
+    each = generate(params, ps, [4, 1, 0], temperature=0.0)
+    assert [t.shape for t in each] == [(13,), (10,), (9,)]
+    assert generate(params, ps[0], 4, temperature=0.0, presence=0.5).shape == (13,)
