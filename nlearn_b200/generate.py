@@ -567,7 +567,8 @@ def generate(trainer_or_params, prompt_ids, n_tokens, seed: int = 0, temperature
     several = isinstance(prompt_ids, (list, tuple)) and any(np.ndim(p) == 1 for p in prompt_ids)
     if rules or np.ndim(n_tokens) or (several and len({len(p) for p in prompt_ids}) > 1):
         prompts = prompt_ids if several or np.ndim(prompt_ids) == 2 else [prompt_ids]
-        dec = PagedDecoder(P, cfg, max_batch=max(1, min(len(prompts), 32)), seed=seed, temperature=temperature)
+        dec = PagedDecoder(P, cfg, max_batch=max(1, min(len(prompts), 32)), max_bias=len(rules.get("bias") or ()),
+                           seed=seed, temperature=temperature)
         out = dec.generate(prompts, n_tokens, **rules)
         if several or np.ndim(prompt_ids) == 2:
             return out if several or np.ndim(n_tokens) or not out else np.stack(out)

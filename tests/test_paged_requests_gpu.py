@@ -246,3 +246,10 @@ def test_entry_point_keeps_the_shape_of_its_prompts(cuda, params):
     each = generate(params, ps, [4, 1, 0], temperature=0.0)
     assert [t.shape for t in each] == [(13,), (10,), (9,)]
     assert generate(params, ps[0], 4, temperature=0.0, presence=0.5).shape == (13,)
+
+
+@pytest.mark.parametrize("n", [1, 33, 300])
+def test_entry_point_takes_any_number_of_biases(cuda, params, n):
+    ids = np.random.default_rng(n).permutation(CFG.vocab)[:n]
+    toks = generate(params, prompts([6])[0], 5, temperature=0.0, bias={int(i): 500.0 for i in ids})
+    assert toks.shape == (11,) and np.isin(toks[6:], ids).all()
