@@ -356,7 +356,7 @@ class PagedDecoder(_DecodeStep):
             self.bias_ids[row, :len(ids)] = torch.tensor(ids, dtype=torch.int32)
             self.bias[row, :len(ids)] = torch.tensor([float(bias[i]) for i in ids])
             rules.add("bias")
-        self.set_allowed(row, allowed)
+        self._set_allowed(row, allowed)
         if allowed is not None:
             rules.add("mask")
         self._rules[row] = frozenset(rules)
@@ -406,7 +406,12 @@ class PagedDecoder(_DecodeStep):
 
     # ------------------------------------------------------------------ API
     def set_allowed(self, row: int, allowed) -> None:
-        """Token ids that row may draw from now on (None: all; a grammar calls this between steps)."""
+        """Token ids that a row in use may draw from now on (None: all; a grammar calls this between steps)."""
+        if not 0 <= row < self.B or not self._len[row]:
+            raise ValueError(f"row {row} is not in use")
+        self._set_allowed(row, allowed)
+
+    def _set_allowed(self, row, allowed):
         if allowed is None:
             self.mask_rows[row] = -1
             self._rules[row] = self._rules[row] - {"mask"}

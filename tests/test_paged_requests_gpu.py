@@ -253,3 +253,22 @@ def test_entry_point_takes_any_number_of_biases(cuda, params, n):
     ids = np.random.default_rng(n).permutation(CFG.vocab)[:n]
     toks = generate(params, prompts([6])[0], 5, temperature=0.0, bias={int(i): 500.0 for i in ids})
     assert toks.shape == (11,) and np.isin(toks[6:], ids).all()
+
+
+@pytest.mark.parametrize("row", [-1, -3, 1, 3])
+def test_allowed_of_a_row_that_is_not_in_use(cuda, params, row):
+    """A row counted from the end, a free one, one past the last: refused, and nothing changed."""
+    dec = PagedDecoder(params, CFG, max_batch=3, temperature=0.0)
+    used = dec.add(prompts([4, 5, 6], 3))
+    dec.release(used[1:2])
+    if row < 0:
+        dec.add(prompts([5], 4))                    # (all rows in use: -1 would name the last)
+    before, rules = dec.mask_rows.tolist(), list(dec._rules)
+    with pytest.raises(ValueError):
+        dec.set_allowed(row, [5])
+    with pytest.raises(ValueError):
+        dec.set_allowed(row, None)
+    assert dec.mask_rows.tolist() == before and dec._rules == rules
+    dec.set_allowed(0, [5])
+    dec.step(2)
+    assert (dec.tokens(0)[-2:] == 5).all()
