@@ -40,6 +40,12 @@ from .model import FlatParams, GPTConfig
 from .paged import paged_decode_attention, paged_kv_write, update_block_tables
 
 
+def _check_ids(ids: np.ndarray, vocab: int) -> None:
+    """Refuses token ids that no row of the embedding belongs to (the kernels would read past it)."""
+    if ids.size and (ids.min() < 0 or ids.max() >= vocab):
+        raise ValueError(f"prompt ids must lie in [0, {vocab}), got {ids.min()} to {ids.max()}")
+
+
 class _DecodeStep:
     """Static buffers of one decode step of `batch` rows and its layers around the attention."""
 
@@ -189,13 +195,16 @@ class Decoder(_DecodeStep):
     def generate(self, prompt_ids, n_tokens: int, seed: int = 0, temperature: float = 1.0,
                  use_graph: bool = True) -> np.ndarray:
         """[P] or [B, P] prompt ids -> [B, P' + n_tokens] (P' after trimming)."""
-        p = np.asarray(prompt_ids, np.int32)
+        p = np.asarray(prompt_ids)
+        if n_tokens > 0:
+            _check_ids(p, self.cfg.vocab)
+        p = p.astype(np.int32)
         if p.ndim == 1:
             p = p[None]
         if p.shape[0] != self.B:
             raise ValueError(f"decoder built for batch {self.B}, prompt batch {p.shape[0]}")
         if n_tokens <= 0:
-            return p.copy()
+            return p
         if n_tokens >= self.S:
             raise ValueError(f"n_tokens {n_tokens} must be below max_len {self.S}")
         if p.shape[1] + n_tokens > self.S:  # keep the most recent prompt tokens (model.py:462-463)
@@ -431,7 +440,9 @@ class PagedDecoder(_DecodeStep):
         """Admit prompts (a list of 1-D id arrays) to free rows, run them and
         draw the first token of each; -> the rows.  The rules (see
         ``process_logits``) hold for all of them; ``allowed`` is a set of token ids."""
-        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        prompts = [np.asarray(p).reshape(-1) for p in prompts]
+        for p in prompts:
+            _check_ids(p, self.cfg.vocab)
         allowed = None if allowed is None else list(allowed)  # (read once for each row)
         rows = self.free_rows()[:len(prompts)]
         if len(rows) < len(prompts):
@@ -445,7 +456,7 @@ class PagedDecoder(_DecodeStep):
             return rows
         dev, T = self.P.device, sum(sizes)
         # the flat list holds the prompts in the order of their rows, which is ascending
-        flat = torch.from_numpy(np.concatenate(prompts)).to(dev)
+        flat = torch.from_numpy(np.concatenate(prompts).astype(np.int32)).to(dev)
         for row in rows:
             self._set_rules(row, repetition, frequency, presence, bias, allowed)
         grow = torch.zeros(self.B, dtype=torch.int32)
@@ -521,8 +532,12 @@ class PagedDecoder(_DecodeStep):
             raise RuntimeError("generate needs all rows free")
         if rules.get("allowed") is not None:
             rules["allowed"] = list(rules["allowed"])  # (read by every admission)
-        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        prompts = [np.asarray(p).reshape(-1) for p in prompts]
         counts = [int(n) for n in np.broadcast_to(n_tokens, (len(prompts),))]
+        for p, n in zip(prompts, counts):
+            if n > 0:
+                _check_ids(p, self.cfg.vocab)
+        prompts = [p.astype(np.int32) for p in prompts]
         if any(n >= self.S for n in counts):
             raise ValueError(f"n_tokens {max(counts)} must be below max_len {self.S}")
         if any(p.size < 1 for p, n in zip(prompts, counts) if n > 0):
@@ -578,7 +593,7 @@ def generate(trainer_or_params, prompt_ids, n_tokens, seed: int = 0, temperature
         if several or np.ndim(prompt_ids) == 2:
             return out if several or np.ndim(n_tokens) or not out else np.stack(out)
         return out[0]
-    p = np.asarray(prompt_ids, np.int32)
+    p = np.asarray(prompt_ids)
     dec = Decoder(P, cfg, batch=1 if p.ndim == 1 else p.shape[0])
     out = dec.generate(p, n_tokens, seed, temperature)
     return out[0] if p.ndim == 1 else out

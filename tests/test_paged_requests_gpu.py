@@ -7,7 +7,7 @@ pytestmark = pytest.mark.gpu
 
 from oracle import decode as OD  # noqa: E402
 from nlearn_b200 import _lib  # noqa: E402
-from nlearn_b200.generate import PagedDecoder, generate  # noqa: E402
+from nlearn_b200.generate import Decoder, PagedDecoder, generate  # noqa: E402
 from nlearn_b200.model import FlatParams  # noqa: E402
 
 from test_paged_decode_gpu import CFG, check_row, oracle, prompts  # noqa: E402
@@ -272,3 +272,25 @@ def test_allowed_of_a_row_that_is_not_in_use(cuda, params, row):
     dec.set_allowed(0, [5])
     dec.step(2)
     assert (dec.tokens(0)[-2:] == 5).all()
+
+
+def test_prompt_ids_outside_the_vocabulary(cuda, params):
+    """Refused before anything is launched; 64-bit ids do not wrap."""
+    dec, one = PagedDecoder(params, CFG, max_batch=2, temperature=0.0), Decoder(params, CFG, batch=1)
+    for bad in (np.array([3, CFG.vocab]), np.array([-1, 3]), np.array([2**32 + 5]), [CFG.vocab]):
+        with pytest.raises(ValueError):
+            dec.add([np.array([1, 2]), bad])
+        with pytest.raises(ValueError):
+            dec.generate([np.array([1, 2]), bad], 3)
+        with pytest.raises(ValueError):
+            one.generate(bad, 3)
+        with pytest.raises(ValueError):
+            generate(params, bad, 3)
+        with pytest.raises(ValueError):
+            generate(params, [[1, 2, 3], bad], 3)
+    assert dec.free_rows() == [0, 1] and dec.n_free.item() == dec.n_pages
+    edge = [0, CFG.vocab - 1]
+    a = generate(params, edge, 4, temperature=0.0)
+    b, = dec.generate([torch.tensor(edge)], 4)
+    assert a.dtype == b.dtype == np.int32 and a[:2].tolist() == b[:2].tolist() == edge
+    assert generate(params, edge, 0).tolist() == edge and _lib.device_error() == 0
