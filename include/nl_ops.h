@@ -62,7 +62,8 @@ typedef enum {
 NL_API const char* nl_version(void);
 /* Reads and clears the device-side error word (1 = a bounded wait timed out,
  * 2 = misaligned shared memory, 3 = a decode position outside the KV cache or
- * the output row, 4 = a page or slot outside a paged cache).  Synchronises `stream`. */
+ * the output row, 4 = a page or slot outside a paged cache, 5 = a row of logits
+ * to sample from that holds nothing but NaN: token 0).  Synchronises `stream`. */
 NL_API int nl_get_device_error(cudaStream_t stream);
 /* Kernels launched by this library so far in this process (host-side count). */
 NL_API long long nl_launch_count(void);

@@ -145,7 +145,8 @@ def device_error() -> int:
     or the output row (the cache and the output row are not written; the
     attention output keeps its previous contents, the sampled token is still
     written), 4 = a page or slot outside a paged cache (its keys take no part,
-    nothing is written to it)."""
+    nothing is written to it), 5 = a row of logits that holds nothing but NaN
+    (token 0 is drawn)."""
     return lib.nl_get_device_error(stream_handle())
 
 

@@ -272,6 +272,10 @@ __global__ void __launch_bounds__(1024) sample_kernel(const float* __restrict__ 
       }
     }
     if (lane == 0) {
+      if (bidx >= V) {  // no logit is a number: a token that the embedding has, reported
+        bidx = 0;
+        if (err) atomicExch(err, 5);
+      }
       tok[b] = bidx;
       if (out) {
         if (t + 1 >= 0 && t + 1 < ldo) out[b * ldo + t + 1] = bidx;

@@ -33,3 +33,30 @@ def test_extreme_bits(cuda, pos, row, col):
                                           stream()) == 0
     assert tok.tolist() == want.tolist()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("T", [0.0, 0.7])
+def test_rows_of_nan(cuda, T):
+    """A row of NaN draws a token of the vocabulary and is reported; -inf and NaN
+    beside numbers are not drawn; a row of -inf draws its first column."""
+    V, nan, inf = 700, float("nan"), float("inf")
+    lg = torch.randn(5, V, device=cuda)
+    lg[1] = nan
+    lg[2, :650], lg[2, 660:] = nan, -inf
+    lg[3] = -inf
+    i32 = dict(device=cuda, dtype=torch.int32)
+    pos, lens = torch.tensor([4], **i32), torch.full((5,), 5, **i32)
+    assert _lib.device_error() == 0
+    for rows in (False, True):
+        tok, out = torch.full((5,), -1, **i32), torch.full((5, 9), -1, **i32)
+        fn = _lib.lib.nl_sample_tokens_rows if rows else _lib.lib.nl_sample_tokens
+        assert fn(lg.data_ptr(), V, V, T, 3, (lens if rows else pos).data_ptr(), tok.data_ptr(), out.data_ptr(), 9, 5,
+                  stream()) == 0
+        t = tok.tolist()
+        assert t[1] == 0 and 650 <= t[2] < 660 and t[3] == 0 and out[:, 5].tolist() == t
+        want = OD.sample(lg.cpu().numpy(), 3, 4, T)
+        assert (t[0], t[4]) == (want[0], want[4])
+        assert _lib.device_error() == 5
+    lg[1] = 0.0
+    assert _lib.lib.nl_sample_tokens(lg.data_ptr(), V, V, T, 3, pos.data_ptr(), tok.data_ptr(), None, 0, 5, stream()) == 0
+    assert _lib.device_error() == 0
