@@ -19,10 +19,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
-#include <optional>
 #include <string>
+#include <utility>
 
 #include "../../../include/nl_ops.h"
 
@@ -131,6 +132,22 @@ at::Tensor rows(const at::Tensor& t, const char* name, int64_t n, int64_t heads,
   return t.clone(at::MemoryFormat::Contiguous);
 }
 
+// Whether a tensor that is written is free of elements that share memory: every stride steps over
+// all that the smaller ones reach.
+bool apart(const at::Tensor& t) {
+  std::pair<int64_t, int64_t> dims[4];  // (stride, size); caches have the most dimensions
+  int n = 0;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) dims[n++] = {t.stride(i), t.size(i)};
+  std::sort(dims, dims + n);
+  int64_t span = 1;
+  for (int i = 0; i < n; ++i) {
+    if (dims[i].first < span) return false;
+    span += (dims[i].second - 1) * dims[i].first;
+  }
+  return true;
+}
+
 struct Caches {
   void *k, *v;
   int dtype, n_pages, heads, page, d;
@@ -158,6 +175,12 @@ Caches caches(const at::Tensor& k, const at::Tensor& v, int index) {
   size32(k.size(0) * k.size(2), "slots of a cache");
   return {k.data_ptr(), v.data_ptr(), fp8 ? NL_E4M3 : NL_BF16, size32(k.size(0), "pages"), size32(k.size(1), "heads"),
           size32(k.size(2), "page_size"), size32(k.size(3), "head_dim"), k.stride(0), k.stride(1), k.stride(2)};
+}
+// Caches that a call writes into.
+void writable(const at::Tensor& k, const at::Tensor& v) {
+  if (!apart(k)) refuse(PyExc_ValueError, "slots of the caches share memory, got strides %s", list(k.strides()).c_str());
+  if (k.numel() > 0 && k.data_ptr() == v.data_ptr())
+    refuse(PyExc_ValueError, "k_cache and v_cache are the same memory");
 }
 const float* cache_scale(PyObject* o, const char* name, const Caches& c, int index) {
   if (o == Py_None) return nullptr;
@@ -221,6 +244,7 @@ PyObject* attention(PyObject* const* a) {
   if ((a[5] == Py_None) != (a[6] == Py_None)) refuse(PyExc_ValueError, "k_new and v_new come together");
   if (a[5] != Py_None) {
     const at::Tensor &k0 = tensor(a[5], "k_new"), &v0 = tensor(a[6], "v_new");
+    writable(tensor(a[1], "k_cache"), tensor(a[2], "v_cache"));
     no_grad(k0, "k_new");
     no_grad(v0, "v_new");
     kn = rows(k0, "k_new", B, c.heads, d, index);
@@ -240,8 +264,9 @@ PyObject* attention(PyObject* const* a) {
     out = tensor(a[10], "out");
     same_place(out, "out", index);
     no_grad(out, "out");
-    if (out.sizes() != q0.sizes() || out.scalar_type() != at::kBFloat16 || out.stride(2) != 1)
-      refuse(PyExc_ValueError, "out must be bfloat16 %s with contiguous rows", list(q0.sizes()).c_str());
+    if (out.sizes() != q0.sizes() || out.scalar_type() != at::kBFloat16 || out.stride(2) != 1 || !apart(out))
+      refuse(PyExc_ValueError, "out must be bfloat16 %s with contiguous rows that do not overlap",
+             list(q0.sizes()).c_str());
   }
   float* lse = nullptr;
   long long lse_b = 0;
@@ -250,9 +275,9 @@ PyObject* attention(PyObject* const* a) {
     same_place(t, "lse", index);
     no_grad(t, "lse");
     if (t.scalar_type() != at::kFloat || t.dim() != 2 || t.size(0) != B || t.size(1) != Hq ||
-        (Hq > 1 && t.stride(1) != 1))
-      refuse(PyExc_ValueError, "lse must be float32 (%lld, %lld) with contiguous rows", static_cast<long long>(B),
-             static_cast<long long>(Hq));
+        (Hq > 1 && t.stride(1) != 1) || !apart(t))
+      refuse(PyExc_ValueError, "lse must be float32 (%lld, %lld) with contiguous rows that do not overlap",
+             static_cast<long long>(B), static_cast<long long>(Hq));
     lse = static_cast<float*>(t.data_ptr());
     lse_b = t.stride(0);
   }
@@ -284,6 +309,7 @@ PyObject* kv_write(PyObject* const* a) {
   no_grad(k0, "k");
   no_grad(v0, "v");
   const Caches c = caches(tensor(a[2], "k_cache"), tensor(a[3], "v_cache"), index);
+  writable(tensor(a[2], "k_cache"), tensor(a[3], "v_cache"));
   if (c.d & (c.dtype == NL_E4M3 ? 15 : 7))
     refuse(PyExc_ValueError, "head_dim %d: cache rows must be whole 16-byte pieces", c.d);
   const int64_t T = k0.dim() == 3 ? k0.size(0) : -1;

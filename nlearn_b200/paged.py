@@ -58,7 +58,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     its slot in the caches; without them it is in the cache already.  scale
     defaults to d**-0.5; k_scale, v_scale (f32 [Hk]) multiply an e4m3
     cache's values.  lse (f32 [B, Hq]), if given, is filled with the log of the sum of
-    exp(scaled scores).  -> out [B, Hq, d] bf16.
+    exp(scaled scores).  -> out [B, Hq, d] bf16; an ``out`` that is given may
+    be q itself and shares no other memory with the operands.
     """
     return _host.paged_decode_attention(q, k_cache, v_cache, block_table, lens, k_new, v_new, k_scale, v_scale, scale,
                                         out, lse)
