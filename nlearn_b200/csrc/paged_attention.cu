@@ -396,14 +396,16 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
   Run in = first;           // run being copied
   int unit = first.c0;      // its next unit
   int in_stage = 0;
-  int pg[S::NG];            // page of the next tile's groups (of key lane % 16, if groups are not whole)
+  // Page of the next tile's groups (of key lane % 16, if groups are not whole).  Ordinary loads: the kernel before
+  // may write the table while this one is already resident, so it is not read-only for this kernel's life.
+  int pg[S::NG];
   auto block_of = [&](int pos) { return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page; };
   auto look_up = [&]() {
     const int pos = unit * UNIT + warp_key + (whole ? 0 : (lane & 15));
     const int* row = p.table + in.b * p.table_ld;
 #pragma unroll
     for (int j = 0; j < S::NG; ++j)
-      pg[j] = (more && pos + j * kGroup < in.len) ? __ldg(row + block_of(pos + j * kGroup)) : 0;
+      pg[j] = (more && pos + j * kGroup < in.len) ? row[block_of(pos + j * kGroup)] : 0;
   };
   // key of this lane in the shared tile: i-th row of a group, relative to my_dst (my_row < RPI)
   auto row_dst = [&](int i) -> uint32_t {
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas<HD, FP8, NH>()) decode_kern
 #pragma unroll
     for (int j = 0; j < S::NG; ++j) {
       const int at = pos + j * kGroup;
-      const int page = at < cap_of(p) ? __ldg(row + block_of(at)) : 0;
+      const int page = at < cap_of(p) ? row[block_of(at)] : 0;
       pg[j] = more && at < in.len ? page : 0;
     }
   } else {
