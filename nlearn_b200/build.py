@@ -54,12 +54,19 @@ def _compile(nvcc: str, src: Path, obj: Path, dep_mtime: float, verbose: bool) -
     return f"compiled: {src.name}" + (f"\n{r.stderr}" if verbose and r.stderr else "")
 
 
+def _ext_made_for() -> str:
+    """What the extension module is compiled against besides its sources: torch's headers and Python's."""
+    import torch
+    return f"torch {torch.__version__} {Path(torch.__file__).resolve().parent} python {sys.version}"
+
+
 def _build_ext() -> str:
     """The extension module (linked against libnl_ops.so, which lies beside it)."""
-    newest = max(EXT_SRC.stat().st_mtime, (INCLUDE / "nl_ops.h").stat().st_mtime)
-    if EXT.exists() and EXT.stat().st_mtime >= newest:
-        return f"up to date: {EXT_SRC.name}"
     import torch
+    newest = max(EXT_SRC.stat().st_mtime, (INCLUDE / "nl_ops.h").stat().st_mtime)
+    stamp, made_for = BUILD_DIR / "ops_py.made_for", _ext_made_for()
+    if (EXT.exists() and EXT.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == made_for):
+        return f"up to date: {EXT_SRC.name}"
     tdir = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parents[1] / "include"
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
@@ -70,6 +77,7 @@ def _build_ext() -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {EXT_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(made_for)
     return f"compiled: {EXT_SRC.name}"
 
 
