@@ -255,11 +255,12 @@ class PagedDecoder(_DecodeStep):
                  temperature: float = 1.0, cache_dtype=torch.bfloat16):
         super().__init__(params, cfg, max_batch, max_len)
         R, H, dev = max_batch, cfg.n_heads, params.device
-        if page_size < 1 or max_bias < 0 or max_batch < 1:
-            raise ValueError(f"page_size {page_size}, max_bias {max_bias}, max_batch {max_batch}: out of range")
+        if page_size < 1 or max_bias < 0 or max_batch < 1 or (n_pages is not None and n_pages < 1):
+            raise ValueError(f"page_size {page_size}, max_bias {max_bias}, max_batch {max_batch}, n_pages {n_pages}: "
+                             "out of range")
         self.page_size, self.seed, self.temperature = page_size, int(seed), float(temperature)
         self.blocks = -(-self.S // page_size)
-        self.n_pages = n_pages or R * self.blocks
+        self.n_pages = R * self.blocks if n_pages is None else n_pages
         i32, f32 = dict(device=dev, dtype=torch.int32), dict(device=dev, dtype=torch.float32)
         shape = (self.n_pages, H, page_size, 64)
         self.k_cache, self.v_cache = ([torch.zeros(shape, device=dev, dtype=torch.bfloat16).to(cache_dtype)

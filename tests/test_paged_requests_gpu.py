@@ -294,3 +294,10 @@ def test_prompt_ids_outside_the_vocabulary(cuda, params):
     b, = dec.generate([torch.tensor(edge)], 4)
     assert a.dtype == b.dtype == np.int32 and a[:2].tolist() == b[:2].tolist() == edge
     assert generate(params, edge, 0).tolist() == edge and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [0, -3])
+def test_a_cache_of_no_pages(cuda, params, n):
+    with pytest.raises(ValueError):
+        PagedDecoder(params, CFG, n_pages=n)
+    assert PagedDecoder(params, CFG, max_batch=2, n_pages=1).n_pages == 1
