@@ -53,9 +53,11 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     q [B, Hq, d] bf16 (d 64 or 128; Hq a multiple of the caches' head count, query
     head h reads kv head h // (Hq / Hk)); lens int32 [B] counts the keys, the
-    new token's included (0: the row's output is 0 and its lse -inf).  With k_new
-    and v_new [B, Hk, d], key lens - 1 comes from there and is written into
-    its slot in the caches; without them it is in the cache already.  scale
+    new token's included (0: the row's output is 0 and its lse -inf, as where every
+    score is -inf).  With k_new and v_new [B, Hk, d], key lens - 1 comes from
+    there and is written into its slot in the caches (the page that takes it
+    stands in no other place of the tables); without them it is in the cache
+    already.  An infinite element of v_cache gives NaN in its column.  scale
     defaults to d**-0.5; k_scale, v_scale (f32 [Hk]) multiply an e4m3
     cache's values.  lse (f32 [B, Hq]), if given, is filled with the log of the sum of
     exp(scaled scores).  -> out [B, Hq, d] bf16; an ``out`` that is given may
@@ -70,13 +72,14 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
                    v_scale: torch.Tensor | None = None) -> None:
     """Write k, v [T, kv_heads, head_dim] (bf16; strided views of a fused qkv
     projection are read in place) into slots[t] (int32 [T]) of the caches.
-    Negative slots are padding; no slot may occur twice.  An e4m3 cache holds
-    round(x / scale), saturating at 448."""
+    Negative slots are padding; no slot may occur twice, and k and v lie in none
+    of them.  An e4m3 cache holds round(x / scale), saturating at 448."""
     _host.paged_kv_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
 
 
 class BlockPlan(NamedTuple):
-    """What one serving step writes and where (all int32, on the device)."""
+    """What one serving step writes and where (all int32, on the device).  The tensors
+    that the call made are parts of one allocation, which lives as long as any of them."""
     slots: torch.Tensor      # [n_tokens] slot of each token of the flat list, -1: none
     positions: torch.Tensor  # [n_tokens] its position in its sequence, -1: none
     cu: torch.Tensor         # [batch + 1] first token of each row
