@@ -19,7 +19,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libnl_ops.so")
 
 STATUS = {0: "NL_OK", -1: "NL_ERR_SHAPE", -2: "NL_ERR_ALIGN", -3: "NL_ERR_LAUNCH", -4: "NL_ERR_CUDA",
           -5: "NL_ERR_DTYPE", -6: "NL_ERR_WORKSPACE", -7: "NL_ERR_TOO_LARGE"}
-F32, BF16, E4M3 = 0, 1, 2
+F32, BF16 = 0, 1
 EPI_STORE, EPI_ACCUM, EPI_BIAS, EPI_BIAS_GELU, EPI_RESID, EPI_DGELU = 0, 1, 2, 3, 4, 5
 
 # name -> argtypes (restype is int unless listed in _RESTYPE)
@@ -95,6 +95,7 @@ _RESTYPE = {"nl_version": ctypes.c_char_p, "nl_launch_count": c_longlong,
             "nl_flash_attention_bwd_noalloc_max_rows": c_longlong, "nl_flash_attention_workspace_bytes": c_size_t, "nl_lce_workspace_bytes": ctypes.c_size_t,
             "nl_decode_workspace_bytes": ctypes.c_size_t, "nl_paged_attention_workspace_bytes": ctypes.c_size_t}
 
+
 class NlError(RuntimeError):
     """A kernel entry point returned a non-zero nl_status."""
 
@@ -151,5 +152,5 @@ def device_error() -> int:
 
 
 __all__ = ["lib", "check", "ptr", "stream_handle", "device_error", "NlError", "LIB_PATH", "SIGNATURES",
-           "F32", "BF16", "E4M3", "EPI_STORE", "EPI_ACCUM", "EPI_BIAS", "EPI_BIAS_GELU", "EPI_RESID", "EPI_DGELU",
+           "F32", "BF16", "EPI_STORE", "EPI_ACCUM", "EPI_BIAS", "EPI_BIAS_GELU", "EPI_RESID", "EPI_DGELU",
            "c_longlong"]
