@@ -350,7 +350,7 @@ class PagedDecoder(_DecodeStep):
         """Keep the MAX_GRAPHS graphs used last (a seed and temperature have up to 8, one for each set of rules)."""
         self._graphs[key] = graph
         if len(self._graphs) > self.MAX_GRAPHS:
-            torch.cuda.current_stream().synchronize()  # (it may still run)
+            torch.cuda.synchronize()  # (it may still run, on any stream)
             del self._graphs[next(iter(self._graphs))]
 
     def _set_rules(self, row, repetition, frequency, presence, bias, allowed):
