@@ -346,7 +346,8 @@ NL_API int nl_linear_ln_small(const void* x, long long ldx, const float* gamma, 
  * Attention of ONE new token per sequence: for query head h of Hq (kv head
  * h / (Hq / Hk)), o[b, h] = softmax(scale q[b, h] . k_j) v_j over j < lens[b].
  *   q, o     bf16 [B, Hq, d], strides q_b, q_h / o_b, o_h; d is 64 or 128
- *   lens     int32 [B], the new token included; 0: o = 0, lse = -inf
+ *            (rows of o and of lse do not overlap; o may be q)
+ *   lens     int32 [B], the new token included; 0, or every score -inf: o = 0, lse = -inf
  *   k_new, v_new  (both or neither NULL) bf16 [B, Hk, d], strides n_b, n_h: key
  *            lens[b] - 1 is taken from here and written into its slot, rounded
  *            to e4m3 first where the cache is.  The page that takes it is in no

@@ -463,14 +463,14 @@ class PagedDecoder(_DecodeStep):
         grow = torch.zeros(self.B, dtype=torch.int32)
         grow[rows] = torch.tensor(sizes, dtype=torch.int32)
         grow = grow.to(dev)
-        plan = update_block_tables(self.block_table, self.lens, grow, self.free_pages, self.n_free, self.page_size, T,
-                                   lens_out=self.lens, n_free_out=self.n_free)
         for row, n in zip(rows, sizes):
             self._len[row] = n
         try:
+            plan = update_block_tables(self.block_table, self.lens, grow, self.free_pages, self.n_free, self.page_size,
+                                       T, lens_out=self.lens, n_free_out=self.n_free)
             self._run_prompts(rows, sizes, flat, plan)
         except BaseException:
-            self.release(rows)  # (the rows hold pages already)
+            self.release(rows)  # (whether or not the device has given them their pages)
             raise
         for row in rows:
             self._len[row] += 1

@@ -301,3 +301,25 @@ def test_a_cache_of_no_pages(cuda, params, n):
     with pytest.raises(ValueError):
         PagedDecoder(params, CFG, n_pages=n)
     assert PagedDecoder(params, CFG, max_batch=2, n_pages=1).n_pages == 1
+
+
+def test_an_admission_without_block_tables(cuda, params, monkeypatch):
+    """It fails before the device has given the rows any page."""
+    from nlearn_b200 import generate as G
+    dec = PagedDecoder(params, CFG, max_batch=3, n_pages=12, seed=8)
+    kept, = dec.add(prompts([20], 5))
+    real, calls = G.update_block_tables, []
+
+    def tables(*args, **kw):
+        calls.append(1)
+        return fail() if len(calls) == 1 else real(*args, **kw)
+    with monkeypatch.context() as m:
+        m.setattr(G, "update_block_tables", tables)
+        with pytest.raises(MemoryError):
+            dec.add(prompts([3, 40], 6))
+    assert dec.free_rows() == [1, 2] and len(calls) == 2
+    same_books(dec)
+    dec.add(prompts([3, 40], 6))
+    dec.step(3)
+    same_books(dec)
+    assert _lib.device_error() == 0
